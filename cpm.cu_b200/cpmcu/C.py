@@ -13,6 +13,7 @@ _LIB_PATH = os.path.join(_HERE, "libcpmcu_b200.so")
 _lib = None
 
 _c_int, _c_float, _c_void_p, _c_char_p = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_char_p
+_c_longlong = ctypes.c_longlong
 
 
 class LayerSpec(ctypes.Structure):
@@ -106,6 +107,13 @@ _SIGNATURES = {
     "cpmcu_debug_moe_pairs": (_c_int, [_c_int] * 5),
     "cpmcu_debug_launch_order": (_c_int, [_c_void_p, _c_int, _c_void_p]),
     "cpmcu_debug_linear_schedule": (_c_int, [_c_int] * 4 + [_c_void_p, _c_int]),
+    "cpmcu_stream_check": (_c_int, [_c_void_p]),
+    "cpmcu_w8a8_packed_bytes": (ctypes.c_long, [_c_int] * 3),
+    "cpmcu_w8a8_pack": (_c_int, [_c_void_p] * 2 + [_c_int] * 3 + [_c_void_p] * 2),
+    "cpmcu_w8a8_quantize": (_c_int, [_c_void_p, _c_longlong, _c_int, _c_int] + [_c_void_p] * 3),
+    "cpmcu_w8a8_workspace_bytes": (ctypes.c_long, [_c_int] * 4),
+    "cpmcu_w8a8_linear": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 4 + [_c_longlong] + [_c_int] * 3 + [_c_void_p, _c_longlong, _c_void_p]),
+    "cpmcu_w8a8_ffn": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 4 + [_c_longlong] + [_c_int] * 3 + [_c_void_p, _c_longlong, _c_void_p]),
     "cpmcu_argmax": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p]),
     "cpmcu_argmax_noalloc": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p]),
     "cpmcu_draft_tree_from_logits": (_c_int, [_c_void_p] + [_c_int] * 4 + [_c_void_p] * 9),

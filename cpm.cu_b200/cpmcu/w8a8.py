@@ -1,0 +1,180 @@
+"""Linear layers in 8-bit integers: weights int8 with a scale for each output channel, rows of bf16 rounded to 8-bit integers with a
+scale each, exact 32-bit sums (formulas at cpmcu_w8a8_norm in include/cpmcu_b200.h).
+
+    w = PackedLinear(q, scale)                     # once: int8 [out, in] and fp32 [out] of a checkpoint, or PackedLinear.from_bf16(weight)
+    y = linear(x, w)                               # x [rows, in] bf16 -> [rows, out] bf16
+    y, t = linear(x, w, norm_weight=g, delta=d)    # t = x + d, y of rms_norm(t) * g
+    y = gated_ffn(x, PackedGateUp(...), w_down)    # down(silu(gate(x)) * up(x))
+
+Calls run on torch's current stream and return without waiting; they can be captured into CUDA graphs.
+"""
+import ctypes
+
+import torch
+
+from . import C
+
+_BF16, _I8, _F32 = torch.bfloat16, torch.int8, torch.float32
+
+
+class Norm(ctypes.Structure):
+    """cpmcu_w8a8_norm of include/cpmcu_b200.h."""
+    _fields_ = [("weight", ctypes.c_void_p), ("eps", ctypes.c_float), ("delta", ctypes.c_void_p), ("delta_scale", ctypes.c_float),
+                ("total", ctypes.c_void_p)]
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _check(t, what, dtype, shape, device=None, rows=False):
+    """rows: any distance between the rows; otherwise contiguous."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {dtype} of shape {tuple(shape)}" +
+                         (f", got {t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else ""))
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{what} must be on {device or 'the GPU'}, got {t.device}")
+    if rows and t.dim() == 2:
+        if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+            raise ValueError(f"{what} must have consecutive elements in rows that do not overlap")
+    elif not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
+
+
+def quantize(x):
+    """(q, scale) of the rows of x [rows, in] bf16: q = round(127 x / max|x|), int8, scale = max|x| / 127, fp32."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a matrix")
+    _check(x, "x", _BF16, x.shape, rows=True)
+    q, scale = torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[0], dtype=_F32, device=x.device)
+    with torch.cuda.device(x.device):
+        C.call("cpmcu_w8a8_quantize", x.data_ptr(), _ld(x), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr(), _stream(x.device))
+    return q, scale
+
+
+class _Packed:
+    def __init__(self, out, width, gated, parts):
+        if out < 1 or width < 1:
+            raise ValueError("weights must not be empty")
+        self.out, self.width, self.device = out, width, parts[0][0].device
+        n = C.load().cpmcu_w8a8_packed_bytes(out, width, int(gated))
+        if n < 0:
+            raise ValueError(C.load().cpmcu_last_error().decode())
+        self.data = torch.empty(n, dtype=torch.uint8, device=self.device)
+        self.ptr = self.data.data_ptr()
+        with torch.cuda.device(self.device):
+            for part, (q, scale) in enumerate(parts, start=int(gated)):
+                C.call("cpmcu_w8a8_pack", q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr, _stream(self.device))
+
+
+class PackedLinear(_Packed):
+    """A weight matrix in the kernels' layout: q [out, in] int8, scale [out] fp32."""
+
+    def __init__(self, q, scale):
+        if not isinstance(q, torch.Tensor) or q.dim() != 2:
+            raise ValueError("q must be a matrix")
+        _check(q, "q", _I8, q.shape)
+        _check(scale, "scale", _F32, q.shape[:1], q.device)
+        super().__init__(q.shape[0], q.shape[1], False, [(q, scale)])
+
+    @classmethod
+    def from_bf16(cls, weight):
+        """Rounds a bf16 matrix [out, in], a scale for each row."""
+        return cls(*quantize(weight))
+
+
+class PackedGateUp(_Packed):
+    """The gate and the up projection of a feed-forward block: q [inter, in] int8 and scale [inter] fp32 each."""
+
+    def __init__(self, gate, gate_scale, up, up_scale):
+        if not isinstance(gate, torch.Tensor) or gate.dim() != 2:
+            raise ValueError("gate must be a matrix")
+        _check(gate, "gate", _I8, gate.shape)
+        _check(up, "up", _I8, gate.shape, gate.device)
+        _check(gate_scale, "gate_scale", _F32, gate.shape[:1], gate.device)
+        _check(up_scale, "up_scale", _F32, gate.shape[:1], gate.device)
+        super().__init__(gate.shape[0], gate.shape[1], True, [(gate, gate_scale), (up, up_scale)])
+
+    @classmethod
+    def from_bf16(cls, gate, up):
+        return cls(*quantize(gate), *quantize(up))
+
+
+def _rows(x, width, device):
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a matrix")
+    _check(x, "x", _BF16, (x.shape[0], width), device, rows=True)
+
+
+def _norm(x, norm_weight, eps, delta, delta_scale):
+    """(argument, total)"""
+    if norm_weight is None:
+        if delta is not None:
+            raise ValueError("delta needs norm_weight")
+        return None, None
+    _check(norm_weight, "norm_weight", _BF16, x.shape[1:], x.device)
+    total = None
+    if delta is not None:
+        _check(delta, "delta", _BF16, x.shape, x.device)
+        total = torch.empty(x.shape, dtype=_BF16, device=x.device)
+    n = Norm(norm_weight.data_ptr(), eps, None if delta is None else delta.data_ptr(), delta_scale, None if total is None else total.data_ptr())
+    return n, total
+
+
+def _out(out, rows, width, device):
+    if out is None:
+        return torch.empty(rows, width, dtype=_BF16, device=device)
+    _check(out, "out", _BF16, (rows, width), device, rows=True)
+    return out
+
+
+def _workspace(rows, out, width, inter, device):
+    n = C.load().cpmcu_w8a8_workspace_bytes(rows, out, width, inter)
+    if n < 0:
+        raise ValueError(C.load().cpmcu_last_error().decode())
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _call(name, device, *args):
+    if device.index == torch.cuda.current_device():
+        C.call(name, *args, _stream(device))
+        return
+    with torch.cuda.device(device):
+        C.call(name, *args, _stream(device))
+
+
+def linear(x, weight, bias=None, norm_weight=None, eps=1e-5, delta=None, delta_scale=1.0, out=None):
+    """y [rows, out] of x [rows, in].  With norm_weight the rows are RMS norms; with delta, of t = x + delta_scale * delta, and (y, t) is
+    returned.  bias [out] bf16.  x (and out) may be rows of a wider matrix."""
+    _rows(x, weight.width, weight.device)
+    if not isinstance(weight, PackedLinear):
+        raise ValueError("weight must be a PackedLinear")
+    if bias is not None:
+        _check(bias, "bias", _BF16, (weight.out,), x.device)
+    rows = x.shape[0]
+    y = _out(out, rows, weight.out, x.device)
+    norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
+    ws = _workspace(rows, weight.out, weight.width, 0, x.device)
+    _call("cpmcu_w8a8_linear", x.device, x.data_ptr(), _ld(x), None if norm is None else ctypes.addressof(norm), weight.ptr,
+          None if bias is None else bias.data_ptr(), y.data_ptr(), _ld(y), rows, weight.out, weight.width, ws.data_ptr(), ws.numel())
+    return y if total is None else (y, total)
+
+
+def gated_ffn(x, gate_up, down, norm_weight=None, eps=1e-5, delta=None, delta_scale=1.0, out=None):
+    """down(silu(gate(x)) * up(x)) of x [rows, in]; norm_weight, delta and out as for linear."""
+    if not isinstance(gate_up, PackedGateUp) or not isinstance(down, PackedLinear):
+        raise ValueError("gate_up must be a PackedGateUp and down a PackedLinear")
+    if (down.width, down.out) != (gate_up.out, gate_up.width) or down.device != gate_up.device:
+        raise ValueError(f"down must be [{gate_up.width}, {gate_up.out}] on {gate_up.device}")
+    _rows(x, gate_up.width, gate_up.device)
+    rows, width, inter = x.shape[0], gate_up.width, gate_up.out
+    y = _out(out, rows, width, x.device)
+    norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
+    ws = _workspace(rows, width, width, inter, x.device)
+    _call("cpmcu_w8a8_ffn", x.device, x.data_ptr(), _ld(x), None if norm is None else ctypes.addressof(norm), gate_up.ptr, down.ptr, y.data_ptr(),
+          _ld(y), rows, width, inter, ws.data_ptr(), ws.numel())
+    return y if total is None else (y, total)

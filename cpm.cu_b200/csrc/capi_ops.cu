@@ -1,0 +1,283 @@
+// extern "C" surface of the operators that run on a stream of the caller's choice (part 4 of include/cpmcu_b200.h): 8-bit linear
+// layers and rotations.  They launch and return: no allocation, no synchronisation, no host copy.
+#include <algorithm>
+
+#include "../../include/cpmcu_b200.h"
+#include "w8a8.cuh"
+
+namespace {
+
+template <typename F>
+auto guarded(F&& f) -> decltype(f()) {
+    try {
+        cpm_set_error("");
+        return f();
+    } catch (const std::exception& e) {
+        cpm_set_error(e.what());
+        return -1;
+    } catch (...) {
+        cpm_set_error("unknown error");
+        return -1;
+    }
+}
+
+uintptr_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// Rows of `cols` elements of `size` bytes, `ld` elements apart.
+struct Rows {
+    const void* p;
+    long long rows, cols, ld;
+    int size;
+    uintptr_t end() const { return addr(p) + static_cast<uintptr_t>(((rows - 1) * ld + cols) * size); }
+};
+// Whether two sets of rows share an element.  Columns of one wider matrix do not, although their rows interleave.
+bool overlap(const Rows& a, const Rows& b) {
+    if (a.p == nullptr || b.p == nullptr || a.rows < 1 || b.rows < 1 || a.end() <= addr(b.p) || b.end() <= addr(a.p)) return false;
+    const long long pitch = a.ld * a.size;
+    if (a.rows > 1 && b.rows > 1 && pitch == b.ld * b.size) {
+        const bool a_first = addr(a.p) <= addr(b.p);
+        const Rows &lo = a_first ? a : b, &hi = a_first ? b : a;
+        const long long off = static_cast<long long>((addr(hi.p) - addr(lo.p)) % static_cast<uintptr_t>(pitch));
+        if (off >= lo.cols * lo.size && off + hi.cols * hi.size <= pitch) return false;
+    }
+    return true;
+}
+
+// The library serves the GPU that was current at its first call (one process per GPU).
+void require_device(const char* what) {
+    int device = -1;
+    CUDA_CHECK(cudaGetDevice(&device));
+    if (device != runtime().device) {
+        throw std::invalid_argument(std::string("cpmcu_b200: ") + what + ": the current device is " + std::to_string(device) +
+                                    ", the library runs on device " + std::to_string(runtime().device));
+    }
+}
+
+cudaStream_t stream_of(void* s) { return static_cast<cudaStream_t>(s); }
+
+void require_sizes(const char* what, int rows, int N, int K) {
+    const std::string name = std::string("cpmcu_b200: ") + what;
+    if (rows < 0 || N < 1 || K < 1) throw std::invalid_argument(name + ": sizes must be positive");
+    if (K > w8::MAX_COLS) throw std::invalid_argument(name + ": sums of more than 131072 products do not fit 32 bits");
+    const long long tiles = (N + 63) / 64;
+    if (tiles * (w8::pad_cols(K) / w8::BLOCK_COLS) > (1ll << 23) || ((static_cast<long long>(rows) + 15) / 16) * tiles > (1ll << 30)) {
+        throw std::invalid_argument(name + ": too many tiles");
+    }
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// A call's workspace: what is where.  Nothing in it is kept from one call for the next.
+struct Layout {
+    size_t q = 0, xs = 0, tickets = 0, partials = 0, act = 0, total = 0;
+    int n_tickets = 0;
+    long long act_ld = 0;
+};
+Layout layout_of(int rows, int N, int K, int inter) {
+    Layout l;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += align256(bytes); return here; };
+    if (inter > 0) {
+        l.act_ld = (inter + 7) / 8 * 8;
+        l.act = take(static_cast<size_t>(rows) * l.act_ld * sizeof(float));
+    }
+    if (rows > 1) {
+        l.q = take(static_cast<size_t>(rows) * std::max(w8::pad_cols(K), inter > 0 ? w8::pad_cols(inter) : 0));
+        l.xs = take(align256(rows) * sizeof(float));
+        // the down projection's, or the only product's
+        const int k_last = inter > 0 ? inter : K;
+        l.n_tickets = w8::product_tickets(rows, N, false);
+        l.tickets = take(l.n_tickets * sizeof(int));
+        l.partials = take(w8::product_partial_bytes(rows, N, k_last, false));
+    }
+    l.total = at;
+    return l;
+}
+
+w8::RowSource source_of(const char* what, const void* x, long long ldx, const cpmcu_w8a8_norm* norm, int rows, int K, const void* y, long long ldy, int out) {
+    const std::string name = std::string("cpmcu_b200: ") + what;
+    auto require = [&](bool ok, const char* msg) { if (!ok) throw std::invalid_argument(name + ": " + msg); };
+    require(x != nullptr && y != nullptr, "x and y must not be null");
+    require(ldx >= K && ldy >= out, "rows overlap: a leading dimension is smaller than the row");
+    require(ldy < (1ll << 31), "the leading dimension of y does not fit 32 bits");
+    w8::RowSource s;
+    s.x = static_cast<const bf16*>(x);
+    s.ldx = ldx;
+    const Rows xr{x, rows, K, ldx, 2}, yr{y, rows, out, ldy, 2};
+    require(!overlap(xr, yr), "y must not overlap x");
+    if (norm != nullptr) {
+        require(norm->weight != nullptr, "a norm needs its weights");
+        require((norm->delta == nullptr) == (norm->total == nullptr), "delta and total come together");
+        s.norm = static_cast<const bf16*>(norm->weight);
+        s.eps = norm->eps;
+        s.delta = static_cast<const bf16*>(norm->delta);
+        s.total = static_cast<bf16*>(norm->total);
+        s.delta_scale = norm->delta_scale;
+        const Rows dr{norm->delta, rows, K, K, 2}, tr{norm->total, rows, K, K, 2}, wr{norm->weight, 1, K, K, 2};
+        require(!overlap(tr, xr) && !overlap(tr, dr) && !overlap(tr, yr) && !overlap(tr, wr), "total must not overlap x, delta, y or the weights");
+        require(!overlap(yr, dr) && !overlap(yr, wr), "y must not overlap delta or the weights");
+    }
+    return s;
+}
+
+void require_workspace(const char* what, void* ws, long long bytes, const Layout& l) {
+    if (l.total == 0) return;
+    const std::string name = std::string("cpmcu_b200: ") + what;
+    if (ws == nullptr || bytes < 0 || static_cast<size_t>(bytes) < l.total) {
+        throw std::invalid_argument(name + ": the workspace needs " + std::to_string(l.total) + " bytes");
+    }
+    if ((addr(ws) & 255) != 0) throw std::invalid_argument(name + ": the workspace must be 256-byte aligned");
+}
+
+void require_packed(const char* what, const void* packed) {
+    if (packed == nullptr || (addr(packed) & 255) != 0) {
+        throw std::invalid_argument(std::string("cpmcu_b200: ") + what + ": packed weights must be 256-byte aligned");
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int cpmcu_stream_check(void* stream) {
+    return guarded([&] {
+        Runtime& rt = runtime();
+        require_device("stream_check");
+        int flags = 0;
+        CUDA_CHECK(cudaStreamSynchronize(stream_of(stream)));
+        CUDA_CHECK(cudaMemcpyAsync(&flags, rt.d_op_error, sizeof(int), cudaMemcpyDeviceToHost, stream_of(stream)));
+        CUDA_CHECK(cudaMemsetAsync(rt.d_op_error, 0, sizeof(int), stream_of(stream)));
+        CUDA_CHECK(cudaStreamSynchronize(stream_of(stream)));
+        if (flags != 0) throw std::runtime_error("cpmcu_b200: kernel error flags " + std::to_string(flags));
+        return 0;
+    });
+}
+
+long cpmcu_w8a8_packed_bytes(int N, int K, int gated) {
+    return guarded([&]() -> long {
+        require_sizes("w8a8_packed_bytes", 1, N, K);
+        return static_cast<long>(w8::packed_bytes(N, K, gated != 0));
+    });
+}
+
+int cpmcu_w8a8_pack(const void* q, const float* scale, int N, int K, int part, void* packed, void* stream) {
+    return guarded([&] {
+        require_sizes("w8a8_pack", 1, N, K);
+        CPM_REQUIRE(q != nullptr && scale != nullptr, "w8a8_pack: q and scale must not be null");
+        CPM_REQUIRE(part >= 0 && part <= 2, "w8a8_pack: part is 0, 1 (gate) or 2 (up)");
+        require_packed("w8a8_pack", packed);
+        require_device("w8a8_pack");
+        w8::launch_pack(static_cast<const int8_t*>(q), scale, N, K, static_cast<w8::Role>(part), packed, stream_of(stream));
+        return 0;
+    });
+}
+
+int cpmcu_w8a8_quantize(const void* x, long long ldx, int rows, int K, void* q, float* scale, void* stream) {
+    return guarded([&] {
+        require_sizes("w8a8_quantize", rows, 1, K);
+        if (rows == 0) return 0;
+        CPM_REQUIRE(x != nullptr && q != nullptr && scale != nullptr, "w8a8_quantize: x, q and scale must not be null");
+        CPM_REQUIRE(ldx >= K, "w8a8_quantize: rows overlap: a leading dimension is smaller than the row");
+        const Rows xr{x, rows, K, ldx, 2}, qr{q, rows, K, K, 1}, sr{scale, 1, rows, rows, 4};
+        CPM_REQUIRE(!overlap(xr, qr) && !overlap(xr, sr) && !overlap(qr, sr), "w8a8_quantize: x, q and scale must not overlap");
+        require_device("w8a8_quantize");
+        w8::RowSource src;
+        src.x = static_cast<const bf16*>(x);
+        src.ldx = ldx;
+        w8::launch_quantize(src, rows, K, static_cast<int8_t*>(q), K, K, scale, nullptr, 0, stream_of(stream));
+        return 0;
+    });
+}
+
+long cpmcu_w8a8_workspace_bytes(int rows, int N, int K, int inter) {
+    return guarded([&]() -> long {
+        require_sizes("w8a8_workspace_bytes", rows, N, K);
+        CPM_REQUIRE(inter >= 0, "w8a8_workspace_bytes: inter must not be negative");
+        if (inter > 0) {
+            require_sizes("w8a8_workspace_bytes", rows, inter, K);
+            require_sizes("w8a8_workspace_bytes", rows, N, inter);
+        }
+        return static_cast<long>(layout_of(rows, N, K, inter).total);
+    });
+}
+
+int cpmcu_w8a8_linear(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, const void* packed, const void* bias, void* y, long long ldy,
+                      int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream) {
+    return guarded([&] {
+        require_sizes("w8a8_linear", rows, N, K);
+        if (rows == 0) return 0;
+        require_packed("w8a8_linear", packed);
+        const w8::RowSource src = source_of("w8a8_linear", x, ldx, norm, rows, K, y, ldy, N);
+        const Layout l = layout_of(rows, N, K, 0);
+        require_workspace("w8a8_linear", workspace, workspace_bytes, l);
+        require_device("w8a8_linear");
+        cudaStream_t s = stream_of(stream);
+        const w8::Packed w = w8::packed_view(packed, N, K, false);
+        if (rows == 1) {
+            w8::launch_one_row(src, N, K, w, static_cast<const bf16*>(bias), static_cast<bf16*>(y), nullptr, s);
+            return 0;
+        }
+        char* ws = static_cast<char*>(workspace);
+        w8::Product p;
+        p.M = rows; p.N = N; p.K = K;
+        p.w = w;
+        int8_t* q = reinterpret_cast<int8_t*>(ws + l.q);
+        float* xs = reinterpret_cast<float*>(ws + l.xs);
+        p.q = q; p.xs = xs;
+        p.bias = static_cast<const bf16*>(bias);
+        p.y = static_cast<bf16*>(y); p.ldy = ldy;
+        p.partials = ws + l.partials;
+        p.tickets = reinterpret_cast<int*>(ws + l.tickets);
+        w8::launch_quantize(src, rows, K, q, w8::pad_cols(K), w8::pad_cols(K), xs, p.tickets, l.n_tickets, s);
+        w8::launch_product(p, s);
+        return 0;
+    });
+}
+
+int cpmcu_w8a8_ffn(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, const void* gate_up, const void* down, void* y, long long ldy, int rows,
+                   int K, int inter, void* workspace, long long workspace_bytes, void* stream) {
+    return guarded([&] {
+        require_sizes("w8a8_ffn", rows, inter, K);
+        require_sizes("w8a8_ffn", rows, K, inter);
+        if (rows == 0) return 0;
+        require_packed("w8a8_ffn", gate_up);
+        require_packed("w8a8_ffn", down);
+        const w8::RowSource src = source_of("w8a8_ffn", x, ldx, norm, rows, K, y, ldy, K);
+        const Layout l = layout_of(rows, K, K, inter);
+        require_workspace("w8a8_ffn", workspace, workspace_bytes, l);
+        require_device("w8a8_ffn");
+        cudaStream_t s = stream_of(stream);
+        const w8::Packed wg = w8::packed_view(gate_up, inter, K, true), wd = w8::packed_view(down, K, inter, false);
+        char* ws = static_cast<char*>(workspace);
+        float* act = reinterpret_cast<float*>(ws + l.act);
+        w8::RowSource middle;
+        middle.x32 = act;
+        middle.ldx = l.act_ld;
+        if (rows == 1) {
+            w8::launch_one_row(src, inter, K, wg, nullptr, nullptr, act, s);
+            w8::launch_one_row(middle, K, inter, wd, nullptr, static_cast<bf16*>(y), nullptr, s);
+            return 0;
+        }
+        int8_t* q = reinterpret_cast<int8_t*>(ws + l.q);
+        float* xs = reinterpret_cast<float*>(ws + l.xs);
+        w8::Product p;
+        p.M = rows; p.N = inter; p.K = K;
+        p.w = wg;
+        p.q = q; p.xs = xs;
+        p.act = act; p.ldy = l.act_ld;
+        w8::launch_quantize(src, rows, K, q, w8::pad_cols(K), w8::pad_cols(K), xs, nullptr, 0, s);
+        w8::launch_product(p, s);
+        p = w8::Product();
+        p.M = rows; p.N = K; p.K = inter;
+        p.w = wd;
+        p.q = q; p.xs = xs;
+        p.y = static_cast<bf16*>(y); p.ldy = ldy;
+        p.partials = ws + l.partials;
+        p.tickets = reinterpret_cast<int*>(ws + l.tickets);
+        w8::launch_quantize(middle, rows, inter, q, w8::pad_cols(inter), w8::pad_cols(inter), xs, p.tickets, l.n_tickets, s);
+        w8::launch_product(p, s);
+        return 0;
+    });
+}
+
+}  // extern "C"

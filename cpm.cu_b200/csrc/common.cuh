@@ -75,6 +75,7 @@ struct Runtime {
     cudaStream_t stream = nullptr;
     int* d_error = nullptr;  // device error word, or-ed into by kernels
     int* h_error = nullptr;  // pinned copy of it
+    int* d_op_error = nullptr;  // the same for operators on the caller's streams (capi_ops.cu)
     unsigned* d_accept_ticket = nullptr;  // CTAs of the acceptance kernel that have read the tree (zero between launches)
     int num_sms = 148;
     int device = 0;
@@ -198,6 +199,9 @@ CUtensorMap make_tmap_2d(const void* base, uint64_t inner, uint64_t outer, uint6
 // Untyped byte matrix without swizzle (packed int4 weights).
 CUtensorMap make_tmap_2d_u8(const void* base, uint64_t inner_bytes, uint64_t outer, uint64_t outer_stride_bytes,
                             uint32_t box_inner_bytes, uint32_t box_outer);
+// Byte matrix with 128-byte swizzle and an inner box extent of 128 bytes (8-bit integers).
+CUtensorMap make_tmap_2d_u8_sw128(const void* base, uint64_t inner_bytes, uint64_t outer, uint64_t outer_stride_bytes,
+                                  uint32_t box_inner_bytes, uint32_t box_outer);
 CUtensorMap make_tmap_3d(const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_bytes,
                          uint64_t stride2_bytes, uint32_t b0, uint32_t b1, uint32_t b2);
 

@@ -1,0 +1,716 @@
+// Products of 8-bit integers, sm_100a:  Y[M,N] = (Q[M,K] W[N,K]^T) * xs[m] * ws[n] (+ bias[n]), int8 in, int32 sums in tensor memory, bf16 out; with
+// gate/up weights silu(gate) * up in fp32 instead.
+//
+// Operand mapping as for the bf16 products (gemm_umma.cu): weights are the A operand (128 rows of a tile), token rows the B operand, the
+// accumulator is Y^T.  A k-block is 128 integers, one 128-byte swizzle row, so a stage has the bytes of a bf16 stage and twice the products.
+//   M <= 64, and few tiles        clusters of 2 to 4 CTAs that cut a tile's k-blocks evenly and sum it in distributed shared memory
+//   M <= 256                      single CTAs, the line of all (tile, k-block) units cut evenly (stream-K)
+//   M > 256, tiles in twos        pairs of CTAs on tiles of 256 x 256 (tcgen05 cta_group::2): half of the operand bytes per product; whole
+//                                 tiles in waves, only those of the last wave are cut
+// Bound: the weights' bytes from HBM up to some 300 rows, the tensor pipe (and, with warm passes, the power cap) beyond.
+//
+// Cut tiles: each piece but the last counted one leaves its int32 sums in a workspace slot, the one counted last adds them to its own.  Integer
+// sums have no order, so the result does not depend on who is last, and no CTA waits for another one: the launch need not be resident as
+// a whole, and may share the device with launches of other streams.  (Clusters are resident as a whole by definition.)
+#include <algorithm>
+
+#include "gemm_common.cuh"
+#include "row_ops.cuh"
+#include "w8a8.cuh"
+
+using gemm::SegIter;
+
+namespace w8 {
+namespace {
+
+constexpr int UMMA_K = 32;
+constexpr int NUM_THREADS = 192;   // warp 0 TMA, warp 1 MMA + TMEM, warps 2-5 epilogue
+constexpr int CTRL_BYTES = 256;
+
+struct ProductArgs {
+    gemm::LinearArgs sched;        // shape, raster and division of the work only
+    int N;                         // output features
+    const float *xs, *ws;
+    const bf16* bias;
+    bf16* y;
+    long long ldy;
+    float* act;
+    int* partials;
+    int* tickets;
+    int* error;
+};
+
+// kind::i8, both operands signed, K-major, int32 accumulator: bits [4,6) D (2 = s32), [7,10) A (1 = s8), [10,13) B, [17,23) N>>3, [24,29) M>>4
+__host__ __device__ constexpr uint32_t idesc_s8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma_s8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR) {
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+            "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+    } else {
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+            "}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+    }
+}
+// one k-block
+template <bool PAIR>
+__device__ __forceinline__ void umma_block(uint32_t d, uint32_t wa, uint32_t xa, uint32_t idesc, bool first) {
+#pragma unroll
+    for (int j = 0; j < BLOCK_COLS / UMMA_K; ++j) {
+        umma_s8<PAIR>(d, ptx::umma_desc_sw128(wa + j * UMMA_K, 16, 1024), ptx::umma_desc_sw128(xa + j * UMMA_K, 16, 1024), idesc, (!first || j > 0) ? 1u : 0u);
+    }
+}
+
+template <int MT, bool PAIR>
+struct Cfg {
+    static constexpr int X_ROWS = PAIR ? MT / 2 : MT;           // token rows that this CTA loads
+    static constexpr int STAGE_BYTES = BLOCK_BYTES + X_ROWS * BLOCK_COLS;
+    static constexpr int STAGES = PAIR ? 6 : (MT <= 16) ? 10 : (MT <= 32) ? 9 : (MT <= 64) ? 8 : (MT <= 128) ? 6 : 4;
+    static constexpr int TMEM_COLS = 2 * MT;
+    static constexpr int SCALE_BYTES = 4 * MT * 4;              // per epilogue warp the token scales of its tile
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CTRL_BYTES + gemm::EPI_XCH_BYTES + SCALE_BYTES + 1024;
+    static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+};
+
+// 16 sums of feature `lane` of this warp, tokens c0 .. c0 + 15, times the scales
+__device__ __forceinline__ void scale16(const int (&r)[16], const float* xs, float ws, float bias, float (&v)[16]) {
+#pragma unroll
+    for (int c = 0; c < 16; c += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(xs + c);
+        v[c] = fmaf(static_cast<float>(r[c]) * s.x, ws, bias);
+        v[c + 1] = fmaf(static_cast<float>(r[c + 1]) * s.y, ws, bias);
+        v[c + 2] = fmaf(static_cast<float>(r[c + 2]) * s.z, ws, bias);
+        v[c + 3] = fmaf(static_cast<float>(r[c + 3]) * s.w, ws, bias);
+    }
+}
+
+__device__ __forceinline__ void load16(uint32_t taddr, int (&r)[16]) {
+    ptx::tmem_ld16(taddr, reinterpret_cast<uint32_t*>(r));
+}
+
+// bf16 rows from 16 tokens' values; y rows are ldy apart (64 bits)
+__device__ __forceinline__ void store16(bf16* y, long long ldy, int N, long long y_row, int cnt, int n0, const float (&v)[16], uint8_t* buf, int lane, bool vec) {
+    gemm::store_tokens<16>(y + y_row * ldy, static_cast<int>(ldy), N, 0, cnt, n0, v, buf, lane, vec);
+}
+
+// silu(gate) * up of a whole tile: lanes 0-63 hold the gate sums of 64 features, 64-127 the up sums of the same ones.  Warps q and q + 2 hand
+// each other half of the tokens of a batch, scaled, so that all four compute.  fp32: what is rounded next is the row of 8-bit integers.
+template <int MT>
+__device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act, long long ld, int N, long long row0, int n0, const float* xs, float ws,
+                                          float* xch, int q, int lane) {
+    constexpr int HB = MT >= 32 ? 16 : 8;
+    float* out = xch + q * (gemm::EPI_WARP_BYTES / 4);
+    const float* in = xch + (q ^ 2) * (gemm::EPI_WARP_BYTES / 4);
+    const int pair_bar = 2 + (q & 1);
+    const bool gates = q < 2;
+#pragma unroll 1
+    for (int c0 = 0; c0 < m_cnt; c0 += 2 * HB) {   // uniform across the CTA
+        uint32_t r[2 * HB];
+        ptx::tmem_ld16(t_addr + c0, r);
+        if constexpr (HB == 16) ptx::tmem_ld16(t_addr + c0 + 16, r + 16);
+        ptx::tmem_wait_ld();
+        float mine[HB];
+        // gate warps keep the first half of the tokens, up warps the second
+#pragma unroll
+        for (int c = 0; c < HB; ++c) {
+            const float lo = static_cast<float>(static_cast<int>(r[c])) * xs[c0 + c] * ws, hi = static_cast<float>(static_cast<int>(r[HB + c])) * xs[c0 + HB + c] * ws;
+            out[c * 32 + lane] = gates ? hi : lo;
+            mine[c] = gates ? lo : hi;
+        }
+        ptx::named_bar_sync(pair_bar, 64);
+        const int first = c0 + (gates ? 0 : HB);
+        float* dst = act + (row0 + first) * ld + n0 + lane;
+#pragma unroll
+        for (int c = 0; c < HB; ++c) {
+            const float other = in[c * 32 + lane];
+            const float v = silu_f32(gates ? mine[c] : other) * (gates ? other : mine[c]);
+            if (first + c < m_cnt && n0 + lane < N) dst[c * ld] = v;
+        }
+        ptx::named_bar_sync(pair_bar, 64);   // the partner may write `in` again
+    }
+}
+
+// The 128 epilogue threads of one CTA walk the segments of `it`; rank: of a pair's CTA, which has 128 of the tile's 256 weight rows.
+template <int MT, bool PAIR>
+__device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint32_t tmem_base, uint64_t* acc_full, uint64_t* acc_empty,
+                                         volatile int* abort_flag, volatile int* s_last, int warp, int lane, int epi_tid, int g, int G, float* xch,
+                                         float* scales, int rank) {
+    constexpr int CSZ = PAIR ? 2 : 1;
+    const gemm::LinearArgs& w = a.sched;
+    const int q = warp & 3, row = q * 32 + lane;
+    uint8_t* buf = reinterpret_cast<uint8_t*>(xch) + q * gemm::EPI_WARP_BYTES;
+    float* xs = scales + q * MT;
+    const bool vec = a.act == nullptr && ((reinterpret_cast<uintptr_t>(a.y) | (static_cast<uintptr_t>(a.ldy) * 2) | (static_cast<uintptr_t>(a.N) * 2)) & 15) == 0;
+    const int gt = w.tail_grid > 0 ? w.tail_grid : G;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    int tile, kb0, kb1;
+    while (it.next(tile, kb0, kb1)) {
+        int m_tile, n_tile;
+        gemm::tile_to_mn(w, tile, m_tile, n_tile);
+        n_tile = n_tile * CSZ + rank;
+        const int m_base = m_tile * MT;
+        const int m_cnt = min(w.M - m_base, MT);
+        // scales of the tokens and of this feature, while the sums are being made
+        for (int t = lane; t < MT; t += 32) xs[t] = t < m_cnt ? a.xs[m_base + t] : 0.f;
+        const float ws = a.ws[n_tile * TILE_ROWS + row];
+        __syncwarp();
+        if (!ptx::mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag)) break;
+        ptx::tc_fence_after();
+        const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * MT;
+        const int n0 = n_tile * TILE_ROWS + q * 32;
+        int* const slot = a.partials + (static_cast<size_t>(g * CSZ + rank) * 2 + (kb0 == 0 ? 1 : 0)) * (MT * TILE_ROWS);
+        bool whole = kb0 == 0 && kb1 == w.kblocks;
+        int first = 0, pieces = 1;
+        if (!whole) {
+            const long long u0 = static_cast<long long>(tile - w.wave_tiles) * w.kblocks;
+            first = gemm::unit_owner(u0, w.total_units, gt);
+            pieces = gemm::unit_owner(u0 + w.kblocks - 1, w.total_units, gt) - first + 1;
+        }
+        if (a.act != nullptr) {
+            gate_tile<MT>(t_addr, m_cnt, a.act, a.ldy, a.N, m_base, n_tile * 64 + (q & 1) * 32, xs, ws, xch, q, lane);
+        } else if (whole) {
+            const float bias = a.bias != nullptr && n0 + lane < a.N ? __bfloat162float(a.bias[n0 + lane]) : 0.f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < m_cnt; c0 += 16) {
+                int r[16];
+                float v[16];
+                load16(t_addr + c0, r);
+                ptx::tmem_wait_ld();
+                scale16(r, xs + c0, ws, bias, v);
+                store16(a.y, a.ldy, a.N, m_base + c0, m_cnt - c0, n0, v, buf, lane, vec);
+            }
+        } else {
+#pragma unroll 1
+            for (int c0 = 0; c0 < m_cnt; c0 += 16) {
+                int r[16];
+                load16(t_addr + c0, r);
+                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    if (c0 + c < m_cnt) __stcg(slot + (c0 + c) * TILE_ROWS + row, r[c]);
+                }
+            }
+        }
+        ptx::tc_fence_before();
+        if constexpr (PAIR) ptx::mbar_arrive_cluster(ptx::cluster_map(ptx::smem_u32(&acc_empty[acc]), 0));
+        else ptx::mbar_arrive(&acc_empty[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+
+        if (!whole) {
+            __threadfence();   // this thread's sums are visible before the count
+            ptx::named_bar_sync(1, 128);
+            if (epi_tid == 0) *s_last = atomicAdd(&a.tickets[tile * CSZ + rank], 1) == pieces - 1;
+            ptx::named_bar_sync(1, 128);
+            const bool last = *s_last != 0;
+            ptx::named_bar_sync(1, 128);   // everyone has read s_last before it can change
+            if (last) {
+                __threadfence();
+                const float bias = a.bias != nullptr && n0 + lane < a.N ? __bfloat162float(a.bias[n0 + lane]) : 0.f;
+#pragma unroll 1
+                for (int c0 = 0; c0 < m_cnt; c0 += 16) {
+                    int sum[16];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) sum[c] = 0;
+#pragma unroll 1
+                    for (int p0 = 0; p0 < pieces; p0 += 4) {
+                        int r[4][16];
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            const int gg = first + p0 + s;
+                            const int* from = a.partials + (static_cast<size_t>(gg * CSZ + rank) * 2 + (gg == first ? 1 : 0)) * (MT * TILE_ROWS) + c0 * TILE_ROWS + row;
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) r[s][c] = p0 + s < pieces && c0 + c < m_cnt ? __ldcg(from + c * TILE_ROWS) : 0;
+                        }
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) sum[c] += r[s][c];
+                        }
+                    }
+                    float v[16];
+                    scale16(sum, xs + c0, ws, bias, v);
+                    store16(a.y, a.ldy, a.N, m_base + c0, m_cnt - c0, n0, v, buf, lane, vec);
+                }
+            }
+        }
+        __syncwarp();   // the scales may be replaced
+    }
+}
+
+// Lets its successor start at once: what a successor fetches before its own wait are packed weights only.
+template <int MT, bool PAIR>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const ProductArgs a) {
+    using C = Cfg<MT, PAIR>;
+    constexpr int CSZ = PAIR ? 2 : 1;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);   // pairs: rank 0's count both CTAs' copies
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* acc_full = empty + C::STAGES;
+    uint64_t* acc_empty = acc_full + 2;                                                // pairs: rank 0's
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* s_last = abort_flag + 1;
+    float* xch = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + CTRL_BYTES);
+    float* scales = xch + gemm::EPI_XCH_BYTES / 4;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+    const int G = gridDim.x / CSZ, g = blockIdx.x / CSZ;
+    const gemm::LinearArgs& sched = a.sched;
+    grid_dep_trigger();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            ptx::mbar_init(&acc_full[s], 1);
+            ptx::mbar_init(&acc_empty[s], CSZ * 128);
+        }
+        *abort_flag = 0;
+        *s_last = 0;
+        ptx::mbar_fence_init();
+        ptx::prefetch_tensormap(&tm_w);
+        ptx::prefetch_tensormap(&tm_x);
+    }
+    if (warp == 1) {
+        if constexpr (PAIR) {
+            ptx::tmem_alloc_pair(tmem_slot, C::TMEM_COLS);
+        } else {
+            ptx::tmem_alloc(tmem_slot, C::TMEM_COLS);
+            ptx::tmem_relinquish();
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) ptx::cluster_sync();   // both CTAs' barriers are there before either copies or arrives
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    SegIter it = gemm::make_seg_iter(sched, g, G);
+    if (warp != 0) grid_dep_wait();
+
+    if (warp == 0) {
+        // ------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            int tile, kb0, kb1;
+            bool ok = true;
+            auto load_w = [&](int s, int kb, int n_tile) {
+                uint8_t* dst = smem + s * C::STAGE_BYTES;
+                const int y = ((CSZ * n_tile + rank) * sched.kblocks + kb) * TILE_ROWS;
+                if (rank == 0) ptx::mbar_arrive_expect_tx(&full[s], CSZ * C::STAGE_BYTES);
+                if constexpr (PAIR) ptx::tma_load_2d_pair(dst, &tm_w, ptx::cluster_map(ptx::smem_u32(&full[s]), 0), 0, y);
+                else ptx::tma_load_2d(dst, &tm_w, &full[s], 0, y);
+            };
+            auto load_x = [&](int s, int kb, int m_tile) {
+                uint8_t* dst = smem + s * C::STAGE_BYTES + BLOCK_BYTES;
+                const int y = m_tile * MT + rank * C::X_ROWS;
+                if constexpr (PAIR) ptx::tma_load_2d_pair(dst, &tm_x, ptx::cluster_map(ptx::smem_u32(&full[s]), 0), kb * BLOCK_COLS, y);
+                else ptx::tma_load_2d(dst, &tm_x, &full[s], kb * BLOCK_COLS, y);
+            };
+            // the first stages' weights: older than the predecessor (w8a8.cuh)
+            int pre = 0;
+            {
+                SegIter pit = it;
+                while (pre < C::STAGES && pit.next(tile, kb0, kb1)) {
+                    int m_tile, n_tile;
+                    gemm::tile_to_mn(sched, tile, m_tile, n_tile);
+                    for (int kb = kb0; kb < kb1 && pre < C::STAGES; ++kb, ++pre) load_w(pre, kb, n_tile);
+                }
+            }
+            grid_dep_wait();
+            int issued = 0;
+            while (ok && it.next(tile, kb0, kb1)) {
+                int m_tile, n_tile;
+                gemm::tile_to_mn(sched, tile, m_tile, n_tile);
+                for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+                    if (issued >= pre) {
+                        if (!ptx::mbar_wait(&empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+                        load_w(stage, kb, n_tile);
+                    }
+                    load_x(stage, kb, m_tile);
+                    if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+                }
+            }
+            if (!ok) {   // copies already in flight land before the CTA retires
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) {}
+            }
+        } else {
+            grid_dep_wait();
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer (pairs: rank 0)
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_s8(CSZ * TILE_ROWS, MT);
+            int stage = 0;
+            uint32_t phase = 0;
+            int acc = 0;
+            uint32_t acc_phase = 0;
+            int tile, kb0, kb1;
+            bool ok = true;
+            while (ok && it.next(tile, kb0, kb1)) {
+                if (!ptx::mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) break;
+                ptx::tc_fence_after();
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!ptx::mbar_wait(&full[stage], phase, abort_flag)) { ok = false; break; }
+                    ptx::tc_fence_after();
+                    const uint32_t wa = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
+                    umma_block<PAIR>(tmem_base + acc * MT, wa, wa + BLOCK_BYTES, idesc, kb == kb0);
+                    if constexpr (PAIR) ptx::umma_commit_pair(&empty[stage]);
+                    else ptx::umma_commit(&empty[stage]);
+                    if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (!ok) break;
+                if constexpr (PAIR) ptx::umma_commit_pair(&acc_full[acc]);
+                else ptx::umma_commit(&acc_full[acc]);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1;
+            }
+        }
+    } else {
+        epilogue<MT, PAIR>(a, it, tmem_base, acc_full, acc_empty, abort_flag, s_last, warp, lane, threadIdx.x - 64, g, G, xch, scales, rank);
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) {
+        __syncwarp();
+        ptx::cluster_sync();   // neither CTA leaves while the other may still read its memory or arrive at its barriers
+    }
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        if constexpr (PAIR) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+        else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(a.error, ERR_GEMM_TIMEOUT);
+}
+
+// A tile per cluster: CTA `rank` of CS has k-blocks [rank * kblocks / CS, (rank + 1) * kblocks / CS).  When every CTA's products are done (a cluster
+// barrier), the operand rings are idle in all of them and take the sums: each CTA sends each peer that peer's share of the tokens straight from
+// tensor memory, a second barrier, and every CTA adds and stores its own share.  All threads reach both barriers whatever the bounded waits
+// before returned.
+template <int MT, int CS>
+struct ClusterCfg {
+    static constexpr int STAGE_BYTES = Cfg<MT, false>::STAGE_BYTES;
+    static constexpr int STAGES = Cfg<MT, false>::STAGES;
+    static constexpr int TPR = MT / CS + (MT % CS != 0);            // tokens summed and stored by each rank
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CTRL_BYTES + 1024;
+    static_assert(CS * TPR * TILE_ROWS * 4 <= STAGES * STAGE_BYTES, "sums must fit the ring");
+};
+
+template <int MT, int CS>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const ProductArgs a) {
+    using C = ClusterCfg<MT, CS>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    int* red = reinterpret_cast<int*>(smem);   // [source][token][row], over the ring
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* acc_full = empty + C::STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(ptx::cluster_ctarank());
+    const int tile = blockIdx.x / CS, kblocks = a.sched.kblocks;
+    const int kb_begin = kblocks * rank / CS, kpc = kblocks * (rank + 1) / CS - kb_begin;
+    grid_dep_trigger();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            ptx::mbar_init(&full[s], 1);
+            ptx::mbar_init(&empty[s], 1);
+        }
+        ptx::mbar_init(acc_full, 1);
+        *abort_flag = 0;
+        ptx::mbar_fence_init();
+        ptx::prefetch_tensormap(&tm_w);
+        ptx::prefetch_tensormap(&tm_x);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(tmem_slot, Cfg<MT, false>::TMEM_COLS);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    if (warp != 0) grid_dep_wait();
+
+    const int q = warp & 3, row = q * 32 + lane;
+    bool summed = false;   // epilogue threads: this CTA's sums are in tensor memory
+    if (warp == 0) {
+        if (lane == 0) {
+            const int pre = min(kpc, C::STAGES);
+            for (int i = 0; i < pre; ++i) {   // weights: older than the predecessor
+                ptx::mbar_arrive_expect_tx(&full[i], C::STAGE_BYTES);
+                ptx::tma_load_2d(smem + i * C::STAGE_BYTES, &tm_w, &full[i], 0, (tile * kblocks + kb_begin + i) * TILE_ROWS);
+            }
+            grid_dep_wait();
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int i = 0; i < kpc; ++i) {
+                uint8_t* dst = smem + stage * C::STAGE_BYTES;
+                if (i >= pre) {
+                    if (!ptx::mbar_wait(&empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+                    ptx::mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
+                    ptx::tma_load_2d(dst, &tm_w, &full[stage], 0, (tile * kblocks + kb_begin + i) * TILE_ROWS);
+                }
+                ptx::tma_load_2d(dst + BLOCK_BYTES, &tm_x, &full[stage], (kb_begin + i) * BLOCK_COLS, 0);
+                if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) {   // copies already in flight land before peers write over the ring
+                const long long t0 = clock64();
+                while (clock64() - t0 < 2000000LL) {}
+            }
+        } else {
+            grid_dep_wait();
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_s8(TILE_ROWS, MT);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int i = 0; i < kpc; ++i) {
+                if (!ptx::mbar_wait(&full[stage], phase, abort_flag)) { ok = false; break; }
+                ptx::tc_fence_after();
+                const uint32_t wa = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
+                umma_block<false>(tmem_base, wa, wa + BLOCK_BYTES, idesc, i == 0);
+                ptx::umma_commit(&empty[stage]);
+                if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
+            }
+            if (ok) ptx::umma_commit(acc_full);
+        }
+    } else {
+        summed = ptx::mbar_wait_warp(acc_full, 0, abort_flag);   // every product has read its operands
+        ptx::tc_fence_after();
+    }
+    __syncwarp();
+    ptx::cluster_sync();   // all CTAs' products are done: the rings may be written by peers
+
+    const int m_cnt = min(a.sched.M, MT);
+    const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+    if (warp >= 2 && summed) {
+        const uint32_t mine = ptx::smem_u32(red + rank * C::TPR * TILE_ROWS + row);
+        // token t goes to rank t / TPR, place t % TPR
+#pragma unroll 1
+        for (int c0 = 0; c0 < m_cnt; c0 += 16) {
+            int r[16];
+            load16(t_addr + c0, r);
+            ptx::tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const int t = c0 + c, d = t / C::TPR;
+                if (t < m_cnt) {
+                    const uint32_t at = ptx::cluster_map(mine, static_cast<uint32_t>(d)) + (t - d * C::TPR) * TILE_ROWS * 4;
+                    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(r[c]) : "memory");
+                }
+            }
+        }
+    }
+    ptx::tc_fence_before();
+    __syncwarp();
+    ptx::cluster_sync();   // this CTA's share has arrived
+    if (warp >= 2 && *abort_flag == 0) {
+        const float ws = a.ws[tile * TILE_ROWS + row];
+        const int t0 = rank * C::TPR, cnt = min(m_cnt - t0, C::TPR);
+        if (a.act == nullptr) {
+            const int n = tile * TILE_ROWS + row;
+            const float bias = a.bias != nullptr && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
+#pragma unroll 4
+            for (int t = 0; t < cnt; ++t) {
+                int sum = 0;
+#pragma unroll
+                for (int s = 0; s < CS; ++s) sum += red[(s * C::TPR + t) * TILE_ROWS + row];
+                if (n < a.N) a.y[static_cast<long long>(t0 + t) * a.ldy + n] = __float2bfloat16(fmaf(static_cast<float>(sum) * a.xs[t0 + t], ws, bias));
+            }
+        } else {
+            // gate rows 0-63 and up rows 64-127 meet in the first source's place, scaled
+            float* meet = reinterpret_cast<float*>(red);
+#pragma unroll 4
+            for (int t = 0; t < cnt; ++t) {
+                int sum = 0;
+#pragma unroll
+                for (int s = 0; s < CS; ++s) sum += red[(s * C::TPR + t) * TILE_ROWS + row];
+                meet[t * TILE_ROWS + row] = static_cast<float>(sum) * a.xs[t0 + t] * ws;
+            }
+            ptx::named_bar_sync(1, 128);
+            const int f = row & 63, n = tile * 64 + f;
+            for (int t = row >> 6; t < cnt; t += 2) {
+                if (n < a.N) a.act[static_cast<long long>(t0 + t) * a.ldy + n] = silu_f32(meet[t * TILE_ROWS + f]) * meet[t * TILE_ROWS + 64 + f];
+            }
+        }
+    }
+
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, Cfg<MT, false>::TMEM_COLS);
+    }
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(a.error, ERR_GEMM_TIMEOUT);
+}
+
+// ---------------------------------------------------------------- host
+CUtensorMap map_rows(const void* base, long long rows, long long cols, int box_rows) {
+    return make_tmap_2d_u8_sw128(base, cols, rows, cols, BLOCK_COLS, box_rows);
+}
+
+// A kernel's shared memory limit; harmless when two threads set it at once
+template <typename... A>
+void allow_smem(void (*kernel)(A...), int bytes) { CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)); }
+
+template <int MT, bool PAIR>
+void run(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
+    using C = Cfg<MT, PAIR>;
+    allow_smem(product_s8_kernel<MT, PAIR>, C::SMEM_BYTES);
+    launch(product_s8_kernel<MT, PAIR>, grid, NUM_THREADS, C::SMEM_BYTES, s, PAIR ? 2 : 1, true, tw, tx, a);
+}
+template <int MT, int CS>
+void run_cluster(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
+    using C = ClusterCfg<MT, CS>;
+    allow_smem(product_s8_cluster_kernel<MT, CS>, C::SMEM_BYTES);
+    launch(product_s8_cluster_kernel<MT, CS>, grid, NUM_THREADS, C::SMEM_BYTES, s, CS, true, tw, tx, a);
+}
+template <int MT>
+void run_cluster(int cs, const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
+    if (cs == 2) run_cluster<MT, 2>(tw, tx, a, grid, s);
+    else if (cs == 3) run_cluster<MT, 3>(tw, tx, a, grid, s);
+    else run_cluster<MT, 4>(tw, tx, a, grid, s);
+}
+template <int MT, int CS>
+int capacity_of() {
+    static const int n = [] {
+        allow_smem(product_s8_cluster_kernel<MT, CS>, ClusterCfg<MT, CS>::SMEM_BYTES);
+        return max_active_clusters(product_s8_cluster_kernel<MT, CS>, dim3(NUM_THREADS), ClusterCfg<MT, CS>::SMEM_BYTES, CS);
+    }();
+    return n;
+}
+// clusters the device runs at once; the kernels differ in their stages only by the token tile, and by less than a CTA's worth
+template <int MT>
+int capacity(int cs) { return cs == 2 ? capacity_of<MT, 2>() : cs == 3 ? capacity_of<MT, 3>() : capacity_of<MT, 4>(); }
+int cluster_capacity(int mt, int cs) { return mt == 16 ? capacity<16>(cs) : mt == 32 ? capacity<32>(cs) : capacity<64>(cs); }
+
+// How a product is divided: by its sizes alone.
+struct Division {
+    int mt = 0, m_tiles = 0;
+    int cluster = 0;       // CTAs per tile, one tile per cluster
+    bool pair = false;
+    int workers = 0;       // CTAs, pairs, or clusters
+    int wave_tiles = 0, tail_grid = 0;
+};
+Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
+    Division d;
+    d.mt = linear_pick_mt(M);
+    d.m_tiles = ceil_div(M, d.mt);
+    if (d.m_tiles == 1 && d.mt <= 64) {
+        // the most CTAs per tile that run at once and have two k-blocks each
+        for (int cs = 4; cs >= 2; --cs) {
+            if (kblocks >= 2 * cs && static_cast<long long>(tiles) * cs <= sms && cluster_capacity(d.mt, cs) >= tiles) {
+                d.cluster = cs;
+                d.workers = tiles;
+                return d;
+            }
+        }
+    }
+    d.pair = d.m_tiles > 1 && tiles % 2 == 0;
+    const int n_tiles = d.pair ? tiles / 2 : tiles, most = d.pair ? sms / 2 : sms;
+    const long long all = static_cast<long long>(n_tiles) * d.m_tiles;
+    if (gated) {
+        // whole tiles only: the activation needs a tile's complete sums
+        d.workers = static_cast<int>(std::min<long long>(all, most));
+        d.wave_tiles = static_cast<int>(all);
+        d.tail_grid = 1;
+        return d;
+    }
+    const long long units = all * kblocks;
+    if (d.m_tiles == 1) {
+        // a piece per CTA; whole tiles where those occupy at least three quarters of the SMs for every round
+        const long long rounds = (all + most - 1) / most;
+        if (all >= rounds * most * 3 / 4) {
+            d.workers = static_cast<int>((all + rounds - 1) / rounds);
+            d.wave_tiles = static_cast<int>(all);
+            d.tail_grid = 1;
+        } else {
+            d.workers = static_cast<int>(std::max<long long>(1, std::min<long long>(most, units / 4)));
+        }
+        return d;
+    }
+    d.workers = static_cast<int>(std::max<long long>(1, std::min<long long>(most, units / 4)));
+    gemm::plan_waves(all, kblocks, d.workers, d.wave_tiles, d.tail_grid);
+    return d;
+}
+
+int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TILE_ROWS); }
+
+}  // namespace
+
+size_t product_partial_bytes(int M, int N, int K, bool gated) {
+    if (gated || M <= 1) return 0;
+    const Division d = divide(M, tiles_of(N, gated), pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms);
+    return d.cluster > 0 ? 0 : static_cast<size_t>(d.workers) * (d.pair ? 2 : 1) * 2 * d.mt * TILE_ROWS * sizeof(int);
+}
+int product_tickets(int M, int N, bool gated) {
+    return gated || M <= 1 ? 0 : tiles_of(N, gated) * ceil_div(M, linear_pick_mt(M));
+}
+
+void launch_product(const Product& p, cudaStream_t s) {
+    const bool gated = p.act != nullptr;
+    const Division d = divide(p.M, p.w.tiles, p.w.kblocks, gated, runtime().num_sms);
+    ProductArgs a;
+    gemm::LinearArgs& w = a.sched;
+    w = gemm::LinearArgs();
+    w.M = p.M; w.N = p.N; w.K = p.K;
+    w.n_tiles = d.pair ? p.w.tiles / 2 : p.w.tiles;
+    w.m_tiles = d.m_tiles;
+    w.kblocks = p.w.kblocks;
+    w.wave_tiles = d.wave_tiles;
+    w.tail_grid = d.tail_grid;
+    w.total_units = (static_cast<long long>(w.n_tiles) * w.m_tiles - w.wave_tiles) * w.kblocks;
+    w.band = gemm::raster_band(d.mt, p.w.kblocks * BLOCK_COLS / 2);   // bytes of a token row as the rule counts them
+    a.N = p.N;
+    a.xs = p.xs; a.ws = p.w.scales; a.bias = p.bias;
+    a.y = p.y; a.ldy = p.ldy; a.act = p.act;
+    a.partials = static_cast<int*>(p.partials);
+    a.tickets = p.tickets;
+    a.error = runtime().d_op_error;
+    const CUtensorMap tw = map_rows(p.w.blocks, static_cast<long long>(p.w.tiles) * p.w.kblocks * TILE_ROWS, BLOCK_COLS, TILE_ROWS);
+    const CUtensorMap tx = map_rows(p.q, p.M, static_cast<long long>(p.w.kblocks) * BLOCK_COLS, d.pair ? d.mt / 2 : d.mt);
+    if (d.cluster > 0) {
+        const int grid = d.workers * d.cluster;
+        if (d.mt == 16) run_cluster<16>(d.cluster, tw, tx, a, grid, s);
+        else if (d.mt == 32) run_cluster<32>(d.cluster, tw, tx, a, grid, s);
+        else run_cluster<64>(d.cluster, tw, tx, a, grid, s);
+        return;
+    }
+    if (d.pair) { run<256, true>(tw, tx, a, 2 * d.workers, s); return; }
+    switch (d.mt) {
+        case 16: run<16, false>(tw, tx, a, d.workers, s); break;
+        case 32: run<32, false>(tw, tx, a, d.workers, s); break;
+        case 64: run<64, false>(tw, tx, a, d.workers, s); break;
+        case 128: run<128, false>(tw, tx, a, d.workers, s); break;
+        default: run<256, false>(tw, tx, a, d.workers, s); break;
+    }
+}
+
+}  // namespace w8

@@ -29,32 +29,36 @@ EncodeTiledFn encode_fn() {
 
 }  // namespace
 
-Runtime& runtime() {
-    static Runtime rt;
-    static bool ready = false;
-    if (!ready) {
-        int count = 0;
-        cudaError_t e = cudaGetDeviceCount(&count);
-        if (e != cudaSuccess || count == 0) {
-            throw std::runtime_error("cpmcu_b200: no CUDA device visible; this library has no CPU path");
-        }
-        CUDA_CHECK(cudaGetDevice(&rt.device));
-        cudaDeviceProp prop;
-        CUDA_CHECK(cudaGetDeviceProperties(&prop, rt.device));
-        if (prop.major != 10) {
-            throw std::runtime_error("cpmcu_b200: kernels are built for sm_100a only (found sm_" +
-                                     std::to_string(prop.major * 10 + prop.minor) + ")");
-        }
-        rt.num_sms = prop.multiProcessorCount;
-        rt.pdl = (getenv("CPMCU_NO_PDL") == nullptr);
-        CUDA_CHECK(cudaStreamCreate(&rt.stream));
-        CUDA_CHECK(cudaMalloc(&rt.d_error, sizeof(int)));
-        CUDA_CHECK(cudaMemset(rt.d_error, 0, sizeof(int)));
-        CUDA_CHECK(cudaMallocHost(&rt.h_error, sizeof(int)));
-        CUDA_CHECK(cudaMalloc(&rt.d_accept_ticket, sizeof(unsigned)));
-        CUDA_CHECK(cudaMemset(rt.d_accept_ticket, 0, sizeof(unsigned)));
-        ready = true;
+namespace {
+Runtime make_runtime() {
+    Runtime rt;
+    int count = 0;
+    cudaError_t e = cudaGetDeviceCount(&count);
+    if (e != cudaSuccess || count == 0) {
+        throw std::runtime_error("cpmcu_b200: no CUDA device visible; this library has no CPU path");
     }
+    CUDA_CHECK(cudaGetDevice(&rt.device));
+    cudaDeviceProp prop;
+    CUDA_CHECK(cudaGetDeviceProperties(&prop, rt.device));
+    if (prop.major != 10) {
+        throw std::runtime_error("cpmcu_b200: kernels are built for sm_100a only (found sm_" +
+                                 std::to_string(prop.major * 10 + prop.minor) + ")");
+    }
+    rt.num_sms = prop.multiProcessorCount;
+    rt.pdl = (getenv("CPMCU_NO_PDL") == nullptr);
+    CUDA_CHECK(cudaStreamCreate(&rt.stream));
+    CUDA_CHECK(cudaMalloc(&rt.d_error, 2 * sizeof(int)));
+    CUDA_CHECK(cudaMemset(rt.d_error, 0, 2 * sizeof(int)));
+    rt.d_op_error = rt.d_error + 1;
+    CUDA_CHECK(cudaMallocHost(&rt.h_error, 2 * sizeof(int)));
+    CUDA_CHECK(cudaMalloc(&rt.d_accept_ticket, sizeof(unsigned)));
+    CUDA_CHECK(cudaMemset(rt.d_accept_ticket, 0, sizeof(unsigned)));
+    return rt;
+}
+}  // namespace
+
+Runtime& runtime() {
+    static Runtime rt = make_runtime();   // first calls from several threads: one of them, the others wait
     return rt;
 }
 
@@ -133,5 +137,22 @@ CUtensorMap make_tmap_2d_u8(const void* base, uint64_t inner_bytes, uint64_t out
                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw std::runtime_error("cpmcu_b200: cuTensorMapEncodeTiled (u8) failed: " + std::to_string(r));
+    return tm;
+}
+
+CUtensorMap make_tmap_2d_u8_sw128(const void* base, uint64_t inner_bytes, uint64_t outer, uint64_t outer_stride_bytes,
+                                  uint32_t box_inner_bytes, uint32_t box_outer) {
+    CPM_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0, "tensor map base must be 16-byte aligned");
+    CPM_REQUIRE(outer_stride_bytes % 16 == 0 && box_inner_bytes % 16 == 0, "tensor map stride/box must be multiples of 16 bytes");
+    CPM_REQUIRE(box_inner_bytes == 128 && box_outer >= 1 && box_outer <= 256, "tensor map box out of range");
+    CUtensorMap tm;
+    cuuint64_t dims[2] = {inner_bytes, outer};
+    cuuint64_t strides[1] = {outer_stride_bytes};
+    cuuint32_t box[2] = {box_inner_bytes, box_outer};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = encode_fn()(&tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("cpmcu_b200: cuTensorMapEncodeTiled (u8, swizzled) failed: " + std::to_string(r));
     return tm;
 }

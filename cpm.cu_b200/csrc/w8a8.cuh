@@ -1,0 +1,131 @@
+// Linear layers in 8-bit integers: y = (q W^T) * (scale of the token) * (scale of the channel) + bias, with q the rows rounded to
+// integers in [-127, 127] (w8a8_rows.cu), W int8, sums exact in 32-bit integers.  Rows of one token go through w8a8_one_row.cu, more
+// through the tensor cores (gemm_w8a8.cu).
+//
+// All launches here are programmatic, on the caller's stream.  A launch lets its successor start only where the note at its kernel says
+// so; packed weights are the one thing that is fetched before the wait for the predecessor.  That is in order because the kernels
+// that write them (pack_kernel) never let a successor start early, so that they have ended, with their writes in L2, before any later launch
+// begins; the fetches go past the first-level cache.
+#pragma once
+#include "common.cuh"
+
+namespace w8 {
+
+constexpr int TILE_ROWS = 128;        // weight rows of a tile
+constexpr int BLOCK_COLS = 128;       // int8 columns of a block: one 128-byte row
+constexpr int BLOCK_BYTES = TILE_ROWS * BLOCK_COLS;
+constexpr int MAX_COLS = 131072;      // 127 * 128 * MAX_COLS < 2^31
+
+inline int pad_cols(int K) { return (K + BLOCK_COLS - 1) / BLOCK_COLS * BLOCK_COLS; }
+
+// Packed weights: ceil(N / 128) x ceil(K / 128) blocks of 128 rows x 128 bytes, blocks of a tile consecutive along K (one sequential burst of 16 KB
+// for each copy, as for the bf16 weights), zeros beyond N and K; then the fp32 scales of the tiles' rows.  A gate/up pair has 64
+// gate rows and the 64 up rows of the same features in every tile.
+struct Packed {
+    const uint8_t* blocks = nullptr;
+    const float* scales = nullptr;
+    int tiles = 0, kblocks = 0;
+};
+enum Role : int { ROLE_PLAIN = 0, ROLE_GATE = 1, ROLE_UP = 2 };
+size_t packed_bytes(int N, int K, bool gated);
+Packed packed_view(const void* p, int N, int K, bool gated);
+void launch_pack(const int8_t* q, const float* scale, int N, int K, Role role, void* packed, cudaStream_t s);
+
+// What the integers of a row are made of.
+struct RowSource {
+    const bf16* x = nullptr;        // rows of K values, ldx apart; or
+    const float* x32 = nullptr;     // fp32 rows
+    long long ldx = 0;
+    // norm != null: integers of t * norm, t = bf16(x + delta_scale * delta) (delta may be null: t = x), whose scale carries 1 / rms(t)
+    const bf16* norm = nullptr;
+    const bf16* delta = nullptr;    // [rows, K]
+    bf16* total = nullptr;          // [rows, K]: t, where there is a delta
+    float delta_scale = 1.f, eps = 0.f;
+};
+// q [rows, ldq] (zeros from K to pad_cols(K)), scale [rows]; also clears n_clear counters for the product behind it
+void launch_quantize(const RowSource& src, int rows, int K, int8_t* q, long long ldq, int pad_to, float* scale, int* clear, int n_clear, cudaStream_t s);
+
+struct Product {
+    int M = 0, N = 0, K = 0;
+    Packed w;
+    const int8_t* q = nullptr;      // [M, pad_cols(K)]
+    const float* xs = nullptr;      // [M], readable up to the next multiple of 256
+    const bf16* bias = nullptr;
+    bf16* y = nullptr;              // [M, ldy]
+    long long ldy = 0;
+    float* act = nullptr;           // gate/up weights: silu(gate) * up instead of y, fp32, N features, ldy floats apart
+    void* partials = nullptr;
+    int* tickets = nullptr;         // zero
+};
+size_t product_partial_bytes(int M, int N, int K, bool gated);
+int product_tickets(int M, int N, bool gated);
+void launch_product(const Product& p, cudaStream_t s);
+// one row, straight from its source
+void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const bf16* bias, bf16* y, float* act, cudaStream_t s);
+
+// The launchers below belong to streams of the caller's choice: they do not count in the library stream's order of launches.
+template <typename... KArgs, typename... Args>
+void launch(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t s, int cluster, bool programmatic, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    if (programmatic && runtime().pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
+}
+
+// ---------------------------------------------------------------- rounding of a row
+// q = round(127 v / top) to nearest, even at ties, exactly: with both scaled by a power of two so that nothing over- or underflows, an estimate
+// from the reciprocal is at most one off, and the rest 127 v - q top, which is exact in fp32 for v of up to 17 significant bits (bf16
+// values and products of two of them), decides.  fp32 rows round on the same estimate; their ties are those of their fp32 quotients.
+struct RowRound {
+    float c127, top, inv;
+    bool finite;
+    // bits: largest of the magnitudes' bit patterns (infinities and NaN are above all finite ones)
+    __device__ __forceinline__ explicit RowRound(uint32_t bits) {
+        finite = bits < 0x7f800000u;
+        const float v = __uint_as_float(bits);
+        int e = static_cast<int>(bits >> 23) - 127;              // top is in [2^e, 2^(e+1)), or below where it is subnormal
+        e = e < -119 ? -119 : e;
+        const float c = __uint_as_float(static_cast<uint32_t>(127 - (e > 126 ? 126 : e)) << 23);
+        c127 = 127.f * c;
+        top = v * c;
+        const bool some = finite && bits != 0u;
+        inv = some ? 1.f / top : 0.f;
+        if (!some) c127 = 0.f;
+    }
+    __device__ __forceinline__ int operator()(float v) const {
+        const float p = v * c127;
+        float r = rintf(p * inv);
+        const float rest = fmaf(-r, top, p);
+        const float twice = 2.f * fabsf(rest);
+        if (twice > top || (twice == top && (static_cast<int>(r) & 1))) r += copysignf(1.f, rest);
+        return static_cast<int>(r);
+    }
+    // the row's scale: NaN for a row with an infinity or a NaN, so that its outputs are NaN
+    __device__ __forceinline__ static float scale(uint32_t bits, float factor) {
+        return bits < 0x7f800000u ? __uint_as_float(bits) / 127.f * factor : __uint_as_float(0x7fffffffu);
+    }
+};
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
+}
+
+}  // namespace w8

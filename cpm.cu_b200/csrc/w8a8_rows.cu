@@ -1,0 +1,173 @@
+// Rows to 8-bit integers, sm_100a:  q = round(127 v / top), scale = top / 127, with top the largest magnitude of the row, alone or
+// behind a residual sum and an RMS norm; and the packing of 8-bit weights.
+//
+// A norm multiplies a whole row by 1 / rms, which cancels in v / top: the integers are those of t * w, a product of two bf16 values and
+// exact in fp32, and the factor goes into the scale.  So the sum of squares and the largest magnitude are found in the same pass, and the integers
+// do not depend on the order of any sum.
+//
+// Bound: bytes.  One CTA per row, which stays in registers between the pass that finds the maximum and the one that rounds; rows too
+// long or not aligned for that are read twice.  A row with an infinity or a NaN gets the scale NaN and integers 0, a row of zeros the scale 0.
+#include "w8a8_rows.cuh"
+
+namespace w8 {
+namespace {
+
+struct QuantizeArgs {
+    RowSource src;
+    int K, pad_to;
+    int8_t* q;
+    long long ldq;
+    float* scale;
+    int* clear;
+    int n_clear;
+};
+
+// VPT > 0: a thread's VPT vectors of 8 stay in registers; 0: the row is read twice, VEC elements at a time.
+// Lets its successor start behind its own wait: a product may then fetch weights, which are older than this launch's predecessor.
+template <Source SRC, int VPT, int VEC>
+__global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const QuantizeArgs a) {
+    __shared__ uint32_t sh_top[32];
+    __shared__ float sh_sum[32];
+    grid_dep_wait();
+    grid_dep_trigger();
+    const size_t row = blockIdx.x;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < a.n_clear; i += gridDim.x * blockDim.x) a.clear[i] = 0;
+    constexpr int N = VPT > 0 ? VPT : 1;
+    Values<SRC, VEC> row_values[N];
+    float ss = 0.f;
+    uint32_t top = 0u;
+    const int step = blockDim.x * VEC;
+    auto largest = [&](const float (&f)[VEC]) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) top = max(top, magnitude(f[e]));
+    };
+    if constexpr (VPT > 0) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = threadIdx.x * VEC + j * step;
+            if (c < a.K) row_values[j].fetch(a.src, row, a.K, c);
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = threadIdx.x * VEC + j * step;
+            if (c < a.K) {
+                row_values[j].combine(a.src, row, a.K, c, ss, true);
+                largest(row_values[j].v);
+            }
+        }
+    } else {
+        for (int c = threadIdx.x * VEC; c < a.K; c += step) {
+            row_values[0].fetch(a.src, row, a.K, c);
+            row_values[0].combine(a.src, row, a.K, c, ss, true);
+            largest(row_values[0].v);
+        }
+    }
+    top = block_max(top, sh_top);
+    float factor = 1.f;
+    if constexpr (SRC == SRC_NORM || SRC == SRC_ADD_NORM) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
+    const RowRound round(top);
+    int8_t* q = a.q + row * a.ldq;
+    if constexpr (VPT > 0) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int c = threadIdx.x * VEC + j * step;
+            if (c < a.K) store_ints<VEC>(q + c, round, row_values[j].v);
+        }
+    } else {
+        for (int c = threadIdx.x * VEC; c < a.K; c += step) {
+            float unused = 0.f;
+            row_values[0].fetch(a.src, row, a.K, c);
+            row_values[0].combine(a.src, row, a.K, c, unused, false);
+            store_ints<VEC>(q + c, round, row_values[0].v);
+        }
+    }
+    for (int c = a.K + threadIdx.x; c < a.pad_to; c += blockDim.x) q[c] = 0;
+    if (threadIdx.x == 0) a.scale[row] = RowRound::scale(top, factor);
+}
+
+template <Source SRC>
+void run_quantize(const QuantizeArgs& a, int rows, bool vec, cudaStream_t s) {
+    auto go = [&](void (*kernel)(QuantizeArgs), int threads) { launch(kernel, rows, threads, 0, s, 1, true, a); };
+    if (!vec) { go(quantize_kernel<SRC, 0, 1>, 256); return; }
+    // Threads for one vector each up to 256, then up to four vectors each, then up to 512 threads
+    const int vectors = a.K / 8;
+    const int round32 = (vectors + 31) / 32 * 32;
+    if (vectors <= 256) go(quantize_kernel<SRC, 1, 8>, round32);
+    else if (vectors <= 512) go(quantize_kernel<SRC, 2, 8>, 256);
+    else if (vectors <= 2048) go(quantize_kernel<SRC, 4, 8>, vectors <= 1024 ? 256 : 512);
+    else go(quantize_kernel<SRC, 0, 8>, 256);
+}
+
+// one thread per 16 bytes of the packed blocks; R rows of a role per tile
+__global__ void pack_kernel(const int8_t* __restrict__ q, const float* __restrict__ scale, int N, int K, int role, int kblocks, bool vec,
+                            uint8_t* __restrict__ blocks, float* __restrict__ scales, size_t chunks) {
+    const int R = role == ROLE_PLAIN ? TILE_ROWS : TILE_ROWS / 2;
+    const size_t per_row = static_cast<size_t>(kblocks) * (BLOCK_COLS / 16);
+    for (size_t i = static_cast<size_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < chunks; i += static_cast<size_t>(gridDim.x) * blockDim.x) {
+        const int r = static_cast<int>(i / per_row), c = static_cast<int>(i - r * per_row) * 16;
+        const int tile = r / R, slot = r % R + (role == ROLE_UP ? R : 0);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (r < N && c < K) {
+            const int8_t* src = q + static_cast<size_t>(r) * K + c;
+            if (vec) {
+                v = *reinterpret_cast<const uint4*>(src);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    auto at = [&](int k) { return c + k < K ? static_cast<int>(src[k]) : 0; };
+                    w[j] = pack4(at(4 * j), at(4 * j + 1), at(4 * j + 2), at(4 * j + 3));
+                }
+                v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        *reinterpret_cast<uint4*>(blocks + (static_cast<size_t>(tile) * kblocks + c / BLOCK_COLS) * BLOCK_BYTES + slot * BLOCK_COLS + c % BLOCK_COLS) = v;
+        if (c == 0) scales[tile * TILE_ROWS + slot] = r < N ? scale[r] : 0.f;
+    }
+}
+
+int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TILE_ROWS); }
+
+}  // namespace
+
+size_t packed_bytes(int N, int K, bool gated) {
+    const size_t tiles = tiles_of(N, gated);
+    return tiles * (pad_cols(K) / BLOCK_COLS) * BLOCK_BYTES + tiles * TILE_ROWS * sizeof(float);
+}
+
+Packed packed_view(const void* p, int N, int K, bool gated) {
+    Packed w;
+    w.tiles = tiles_of(N, gated);
+    w.kblocks = pad_cols(K) / BLOCK_COLS;
+    w.blocks = static_cast<const uint8_t*>(p);
+    w.scales = reinterpret_cast<const float*>(w.blocks + static_cast<size_t>(w.tiles) * w.kblocks * BLOCK_BYTES);
+    return w;
+}
+
+void launch_pack(const int8_t* q, const float* scale, int N, int K, Role role, void* packed, cudaStream_t s) {
+    const bool gated = role != ROLE_PLAIN;
+    const Packed w = packed_view(packed, N, K, gated);
+    const size_t chunks = static_cast<size_t>(w.tiles) * (gated ? TILE_ROWS / 2 : TILE_ROWS) * w.kblocks * (BLOCK_COLS / 16);
+    const bool vec = K % 16 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+    const size_t want = (chunks + 255) / 256;
+    // not programmatic, and the kernel lets no successor start early (w8a8.cuh)
+    launch(pack_kernel, static_cast<int>(want < 148 * 32 ? want : 148 * 32), 256, 0, s, 1, false, q, scale, N, K, static_cast<int>(role), w.kblocks, vec,
+           const_cast<uint8_t*>(w.blocks), const_cast<float*>(w.scales), chunks);
+}
+
+void launch_quantize(const RowSource& src, int rows, int K, int8_t* q, long long ldq, int pad_to, float* scale, int* clear, int n_clear, cudaStream_t s) {
+    if (rows <= 0) return;
+    QuantizeArgs a;
+    a.src = src;
+    a.K = K; a.pad_to = pad_to;
+    a.q = q; a.ldq = ldq;
+    a.scale = scale;
+    a.clear = clear; a.n_clear = n_clear;
+    const bool vec = rows_in_vectors(src, K) && (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldq % 8 == 0;
+    if (src.x32 != nullptr) run_quantize<SRC_F32>(a, rows, vec, s);
+    else if (src.norm == nullptr) run_quantize<SRC_PLAIN>(a, rows, vec, s);
+    else if (src.delta == nullptr) run_quantize<SRC_NORM>(a, rows, vec, s);
+    else run_quantize<SRC_ADD_NORM>(a, rows, vec, s);
+}
+
+}  // namespace w8
