@@ -114,6 +114,8 @@ _SIGNATURES = {
     "cpmcu_w8a8_workspace_bytes": (ctypes.c_long, [_c_int] * 4),
     "cpmcu_w8a8_linear": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 4 + [_c_longlong] + [_c_int] * 3 + [_c_void_p, _c_longlong, _c_void_p]),
     "cpmcu_w8a8_ffn": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 4 + [_c_longlong] + [_c_int] * 3 + [_c_void_p, _c_longlong, _c_void_p]),
+    "cpmcu_rotary_append": (_c_int, [_c_void_p, _c_longlong] + [_c_int] * 6 + [_c_void_p, _c_float, _c_void_p, _c_void_p, _c_longlong] + [_c_void_p] * 2 +
+                            [_c_int, _c_void_p, _c_void_p]),
     "cpmcu_argmax": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p]),
     "cpmcu_argmax_noalloc": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p]),
     "cpmcu_draft_tree_from_logits": (_c_int, [_c_void_p] + [_c_int] * 4 + [_c_void_p] * 9),

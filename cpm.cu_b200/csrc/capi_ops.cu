@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "../../include/cpmcu_b200.h"
+#include "rotary.cuh"
 #include "w8a8.cuh"
 
 namespace {
@@ -276,6 +277,44 @@ int cpmcu_w8a8_ffn(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, co
         p.tickets = reinterpret_cast<int*>(ws + l.tickets);
         w8::launch_quantize(middle, rows, inter, q, w8::pad_cols(inter), w8::pad_cols(inter), xs, p.tickets, l.n_tickets, s);
         w8::launch_product(p, s);
+        return 0;
+    });
+}
+
+int cpmcu_rotary_append(const void* qkv, long long ld, int rows, int heads, int kv_heads, int dim, int rot_dims, int interleaved, const float* inv_freq,
+                        float factor, const int32_t* pos, void* q, long long ldq, void* k_cache, void* v_cache, int cache_rows, const int32_t* slots,
+                        void* stream) {
+    return guarded([&] {
+        CPM_REQUIRE(rows >= 0 && heads >= 0 && kv_heads >= 0 && heads + kv_heads >= 1 && dim >= 2 && dim % 2 == 0,
+                    "rotary_append: sizes must be positive and head widths even");
+        CPM_REQUIRE(heads <= 65536 && kv_heads <= 65536 && dim <= 4096 && (static_cast<long long>(heads) + 2 * kv_heads) * dim < (1ll << 28), "rotary_append: rows are too wide");
+        CPM_REQUIRE(rot_dims >= 0 && rot_dims <= dim && rot_dims % 2 == 0, "rotary_append: rot_dims is even and at most the head's width");
+        CPM_REQUIRE(rot_dims / 2 <= rotary_max_pairs(), "rotary_append: at most 512 pairs are rotated");
+        if (rows == 0) return 0;
+        const long long kv_dim = static_cast<long long>(kv_heads) * dim, q_cols = static_cast<long long>(heads) * dim, cols = q_cols + 2 * kv_dim;
+        CPM_REQUIRE(qkv != nullptr && pos != nullptr && (rot_dims == 0 || inv_freq != nullptr), "rotary_append: qkv, pos and inv_freq must not be null");
+        CPM_REQUIRE(ld >= cols && (heads == 0 || ldq >= q_cols), "rotary_append: rows overlap: a leading dimension is smaller than the row");
+        CPM_REQUIRE(heads == 0 || q != nullptr, "rotary_append: q must not be null");
+        const Rows in{qkv, rows, cols, ld, 2}, qr{heads > 0 ? q : nullptr, rows, q_cols, ldq, 2};
+        CPM_REQUIRE((q == qkv && (ldq == ld || rows == 1)) || !overlap(in, qr), "rotary_append: q must be the query part of qkv itself, or apart from it");
+        if (kv_heads > 0) {
+            CPM_REQUIRE(k_cache != nullptr && v_cache != nullptr && slots != nullptr && cache_rows >= 0, "rotary_append: caches and slots must not be null");
+            const Rows kr{k_cache, cache_rows, kv_dim, kv_dim, 2}, vr{v_cache, cache_rows, kv_dim, kv_dim, 2};
+            CPM_REQUIRE(!overlap(in, kr) && !overlap(in, vr) && !overlap(qr, kr) && !overlap(qr, vr) && !overlap(kr, vr),
+                        "rotary_append: the caches must not overlap each other, qkv or q");
+        }
+        require_device("rotary_append");
+        RotaryArgs a;
+        a.qkv = static_cast<const bf16*>(qkv);
+        a.ld = ld;
+        a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.half = rot_dims / 2;
+        a.inv_freq = inv_freq; a.factor = factor; a.pos = pos;
+        a.q = static_cast<bf16*>(q);
+        a.ldq = heads > 0 ? ldq : 0;
+        a.k_cache = static_cast<bf16*>(k_cache); a.v_cache = static_cast<bf16*>(v_cache);
+        a.cache_rows = cache_rows; a.slots = slots;
+        a.error = runtime().d_op_error;
+        launch_rotary(a, rows, interleaved != 0, stream_of(stream));
         return 0;
     });
 }

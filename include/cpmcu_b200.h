@@ -507,6 +507,16 @@ int cpmcu_w8a8_linear(const void* x, long long ldx, const cpmcu_w8a8_norm* norm,
 int cpmcu_w8a8_ffn(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, const void* gate_up, const void* down, void* y, long long ldy, int rows,
                    int K, int inter, void* workspace, long long workspace_bytes, void* stream);
 
+/* Rotary positions for rows of fused queries, keys and values, and their append to a cache.  qkv [rows, (heads + 2 kv_heads) * dim] bf16, rows ld
+ * apart.  The first rot_dims elements of every query and key head turn, pair i by pos[row] * inv_freq[i] (angles of 64 bits), with
+ * sines and cosines times `factor`: pairs are (2 i, 2 i + 1) if interleaved, else (i, i + rot_dims / 2).  The rest of a head stays.
+ * q [rows, heads * dim], rows ldq apart (may be qkv itself, ldq = ld); key and value of a row go to row slots[row] of the caches
+ * [cache_rows, kv_heads * dim]: a negative slot stores neither, one that is cache_rows or more is an error (cpmcu_stream_check) that stores
+ * neither; of two equal slots either row's elements may stay.  heads or kv_heads may be 0 (then q, or caches and slots, may be NULL). */
+int cpmcu_rotary_append(const void* qkv, long long ld, int rows, int heads, int kv_heads, int dim, int rot_dims, int interleaved, const float* inv_freq,
+                        float factor, const int32_t* pos, void* q, long long ldq, void* k_cache, void* v_cache, int cache_rows, const int32_t* slots,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

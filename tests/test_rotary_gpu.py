@@ -1,0 +1,116 @@
+"""Rotation of fused q/k/v rows against its definition in 64 bits: both layouts, parts of a head, odd widths and strides, far and negative positions,
+cache slots that are skipped or out of range."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, I32, F64 = torch.bfloat16, torch.int32, torch.float64
+
+
+@pytest.fixture(scope="module")
+def rotary():
+    import cpmcu.rotary as r
+    return r
+
+
+def definition(qkv, heads, kv, dim, inv_freq, pos, rot, interleaved, factor):
+    """(rotated queries and keys, values, allowed error of the rotated)"""
+    x = qkv.double().unflatten(1, (heads + 2 * kv, dim))
+    angle = pos.double()[:, None] * inv_freq.double()
+    f = float(torch.tensor(factor, dtype=torch.float32))
+    cs, sn = torch.cos(angle)[:, None] * f, torch.sin(angle)[:, None] * f
+    out, part = x[:, :heads + kv].clone(), x[:, :heads + kv, :rot]
+    a, b = (part[..., 0::2], part[..., 1::2]) if interleaved else (part[..., :rot // 2], part[..., rot // 2:])
+    new = (a * cs - b * sn, b * cs + a * sn)
+    size = (a.abs() + b.abs()) * abs(f)
+    if interleaved:
+        out[..., 0:rot:2], out[..., 1:rot:2] = new
+        size = size.repeat_interleave(2, -1)
+    else:
+        out[..., :rot // 2], out[..., rot // 2:rot] = new
+        size = torch.cat((size, size), -1)
+    # rounding to bf16; sines and cosines to 2^-20 (a turn's fraction in fp32, its functions, the factor and two more roundings)
+    tol = out.abs() * 2.0 ** -8
+    tol[..., :rot] += size * 2.0 ** -20 + 1e-38
+    tol[..., rot:] = 0
+    return out, x[:, heads + kv:], tol
+
+
+SHAPES = [(32, 2, 128, 128, False), (32, 8, 128, 64, False), (15, 5, 80, 20, True), (4, 4, 80, 20, False), (3, 1, 64, 64, True), (2, 2, 96, 48, False), (1, 1, 2, 2, True),
+          (5, 1, 6, 2, False), (7, 3, 10, 6, True), (8, 8, 256, 256, False), (2, 1, 256, 64, True), (1, 1, 36, 36, False), (2, 2, 1024, 1024, False), (3, 1, 64, 0, False), (40, 1, 72, 72, True)]
+
+
+@pytest.mark.parametrize("heads,kv,dim,rot,interleaved", SHAPES)
+@pytest.mark.parametrize("rows,pad", [(1, 0), (5, 0), (60, 8), (33, 3), (700, 2)])
+def test_rotation(rotary, heads, kv, dim, rot, interleaved, rows, pad):
+    g = torch.Generator("cuda").manual_seed(rows + dim)
+    cols = (heads + 2 * kv) * dim
+    wide = torch.randn(rows, cols + 2 * pad, generator=g, device="cuda").to(BF16)
+    qkv = wide[:, pad:pad + cols]
+    before = wide.clone()
+    inv, _ = rotary.frequencies(max(rot, 2), 10000.0)
+    inv = inv[:rot // 2].cuda()
+    pos = torch.randint(-50, 2_000_000, (rows,), generator=g, device="cuda", dtype=I32)
+    n = rows + 9
+    slots = torch.randperm(n, generator=g, device="cuda")[:rows].to(I32)
+    slots[rows // 2] = -3
+    k, v = torch.randn(2, n, kv * dim, generator=g, device="cuda").to(BF16)
+    k0, v0 = k.clone(), v.clone()
+    q = rotary.append(qkv, heads, kv, dim, inv, pos, k, v, slots, rot_dims=rot, interleaved=interleaved, factor=1.19)
+    want, values, tol = definition(qkv, heads, kv, dim, inv, pos, rot, interleaved, 1.19)
+    got = q.double().unflatten(1, (heads, dim))
+    assert bool(((got - want[:, :heads]).abs() <= tol[:, :heads]).all())
+    kept = slots >= 0
+    at = slots[kept].long()
+    assert bool(((k[at].double().unflatten(1, (kv, dim)) - want[kept][:, heads:]).abs() <= tol[kept][:, heads:]).all())
+    assert torch.equal(v[at].double().unflatten(1, (kv, dim)), values[kept])
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert torch.equal(k[rest], k0[rest]) and torch.equal(v[rest], v0[rest])          # rows that no slot names
+    assert torch.equal(wide.view(torch.int16), before.view(torch.int16))
+    # in place: the queries of qkv themselves
+    again = rotary.append(qkv, heads, kv, dim, inv, pos, k, v, slots, rot_dims=rot, interleaved=interleaved, factor=1.19, out=qkv[:, :heads * dim])
+    assert torch.equal(again, q)
+    assert torch.equal(wide[:, :pad], before[:, :pad]) and torch.equal(wide[:, pad + heads * dim:], before[:, pad + heads * dim:])
+
+
+def test_unrotated_elements_and_infinities_stay_apart(rotary):
+    """An infinity or a NaN reaches its own pair only."""
+    for interleaved in (False, True):
+        qkv = torch.randn(4, 3 * 64, device="cuda").to(BF16)
+        inv = rotary.frequencies(32, 10000.0)[0].cuda()
+        pos = torch.arange(4, dtype=I32, device="cuda")
+        k, v = torch.zeros(2, 4, 64, dtype=BF16, device="cuda")
+        clean = rotary.append(qkv, 1, 1, 64, inv, pos, k, v, pos, rot_dims=32, interleaved=interleaved)
+        bad = qkv.clone()
+        bad[1, 40], bad[2, 5], bad[3, 6] = float("nan"), float("inf"), float("nan")
+        got = rotary.append(bad, 1, 1, 64, inv, pos, k, v, pos, rot_dims=32, interleaved=interleaved)
+        differ = {(int(r), int(c)) for r, c in (got != clean).nonzero()}
+        pairs = {(2, 4), (2, 5), (3, 6), (3, 7)} if interleaved else {(2, 5), (2, 21), (3, 6), (3, 22)}
+        assert differ == pairs | {(1, 40)}
+
+
+def test_slots_beyond_the_cache_are_reported_and_not_written(rotary):
+    import cpmcu.C as C
+    qkv = torch.randn(3, 3 * 64, device="cuda").to(BF16)
+    inv = rotary.frequencies(64, 10000.0)[0].cuda()
+    pos = torch.arange(3, dtype=I32, device="cuda")
+    store = torch.zeros(2, 8, 64, dtype=BF16, device="cuda")
+    k, v = store[0, :4], store[1, :4]
+    rotary.append(qkv, 1, 1, 64, inv, pos, k, v, torch.tensor([4, 1, 2 ** 31 - 1], dtype=I32, device="cuda"))
+    with pytest.raises(RuntimeError, match="error flags 8"):
+        C.call("cpmcu_stream_check", torch.cuda.current_stream().cuda_stream)
+    C.call("cpmcu_stream_check", torch.cuda.current_stream().cuda_stream)      # reported once
+    assert not bool(store[:, 0].any()) and not bool(store[:, 2:].any()) and bool(store[:, 1].any())
+
+
+def test_queries_or_keys_alone(rotary):
+    qkv = torch.randn(6, 4 * 32, device="cuda").to(BF16)
+    inv = rotary.frequencies(32, 10000.0)[0].cuda()
+    pos = torch.arange(6, dtype=I32, device="cuda") * 1000
+    q = rotary.append(qkv, 4, 0, 32, inv, pos)
+    k, v = torch.zeros(2, 6, 64, dtype=BF16, device="cuda")
+    none = rotary.append(qkv, 0, 2, 32, inv, pos, k, v, torch.arange(6, dtype=I32, device="cuda"))
+    assert none.shape == (6, 0)
+    assert torch.equal(k, q[:, :64]) and torch.equal(v, qkv[:, 64:])
+    assert rotary.append(qkv[:0], 4, 0, 32, inv, pos[:0]).shape == (0, 128)
