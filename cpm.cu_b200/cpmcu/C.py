@@ -112,8 +112,10 @@ _SIGNATURES = {
     "cpmcu_w8a8_pack": (_c_int, [_c_void_p] * 2 + [_c_int] * 3 + [_c_void_p] * 2),
     "cpmcu_w8a8_quantize": (_c_int, [_c_void_p, _c_longlong, _c_int, _c_int] + [_c_void_p] * 3),
     "cpmcu_w8a8_workspace_bytes": (ctypes.c_long, [_c_int] * 4),
-    "cpmcu_w8a8_linear": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 4 + [_c_longlong] + [_c_int] * 3 + [_c_void_p, _c_longlong, _c_void_p]),
-    "cpmcu_w8a8_ffn": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 4 + [_c_longlong] + [_c_int] * 3 + [_c_void_p, _c_longlong, _c_void_p]),
+    "cpmcu_w8a8_linear": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 3 + [_c_float, _c_void_p, _c_float] + [_c_void_p] * 2 + [_c_longlong] + [_c_int] * 3 +
+                          [_c_void_p, _c_longlong, _c_void_p]),
+    "cpmcu_w8a8_ffn": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 3 + [_c_float, _c_void_p, _c_float] + [_c_void_p] * 2 + [_c_longlong] + [_c_int] * 3 +
+                          [_c_void_p, _c_longlong, _c_void_p]),
     "cpmcu_rotary_append": (_c_int, [_c_void_p, _c_longlong] + [_c_int] * 6 + [_c_void_p, _c_float, _c_void_p, _c_void_p, _c_longlong] + [_c_void_p] * 2 +
                             [_c_int, _c_void_p, _c_void_p]),
     "cpmcu_argmax": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p]),
@@ -156,13 +158,17 @@ def _check(code):
     return code
 
 
+_functions = {}
+
+
 def call(name, *args):
     """Call an extern "C" entry point by name; negative return codes raise RuntimeError."""
-    fn = getattr(load(), name)
-    res = fn(*args)
-    if fn.restype is _c_int:
-        return _check(res)
-    return res
+    known = _functions.get(name)
+    if known is None:
+        fn = getattr(load(), name)
+        known = _functions[name] = (fn, fn.restype is _c_int)
+    res = known[0](*args)
+    return _check(res) if known[1] and res < 0 else res
 
 
 # ---------------------------------------------------------------- reference names

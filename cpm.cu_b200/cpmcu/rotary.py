@@ -107,7 +107,6 @@ def append(qkv, heads, kv_heads, dim, inv_freq, positions, k_cache=None, v_cache
     _check(qkv, "qkv", _BF16, (rows, (heads + 2 * kv_heads) * dim), rows=True)
     _check(inv_freq, "inv_freq", _F32, (rot // 2,), device)
     _check(positions, "positions", _I32, (rows,), device)
-    cache_rows = 0
     if kv_heads > 0:
         if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 2:
             raise ValueError("k_cache must be a matrix")
@@ -115,11 +114,13 @@ def append(qkv, heads, kv_heads, dim, inv_freq, positions, k_cache=None, v_cache
         _check(k_cache, "k_cache", _BF16, (cache_rows, kv_heads * dim), device)
         _check(v_cache, "v_cache", _BF16, k_cache.shape, device)
         _check(slots, "slots", _I32, (rows,), device)
+        keys = (k_cache.data_ptr(), v_cache.data_ptr(), cache_rows, slots.data_ptr())
+    else:
+        keys = (None, None, 0, None)
     if out is None:
-        out = torch.empty(rows, heads * dim, dtype=_BF16, device=device)
+        out = qkv.new_empty((rows, heads * dim))
     else:
         _check(out, "out", _BF16, (rows, heads * dim), device, rows=True)
-    keys = (k_cache.data_ptr(), v_cache.data_ptr(), cache_rows, slots.data_ptr()) if kv_heads > 0 else (None, None, 0, None)
-    _call("cpmcu_rotary_append", device, qkv.data_ptr(), _ld(qkv), rows, heads, kv_heads, dim, rot, int(interleaved), inv_freq.data_ptr(), factor,
+    _call("cpmcu_rotary_append", device, qkv.data_ptr(), _ld(qkv), rows, heads, kv_heads, dim, rot, interleaved, inv_freq.data_ptr(), factor,
           positions.data_ptr(), out.data_ptr(), _ld(out), *keys)
     return out

@@ -8,41 +8,45 @@ scale each, exact 32-bit sums (formulas at cpmcu_w8a8_norm in include/cpmcu_b200
 
 Calls run on torch's current stream and return without waiting; they can be captured into CUDA graphs.
 """
-import ctypes
+import functools
 
 import torch
 
 from . import C
 
 _BF16, _I8, _F32 = torch.bfloat16, torch.int8, torch.float32
-
-
-class Norm(ctypes.Structure):
-    """cpmcu_w8a8_norm of include/cpmcu_b200.h."""
-    _fields_ = [("weight", ctypes.c_void_p), ("eps", ctypes.c_float), ("delta", ctypes.c_void_p), ("delta_scale", ctypes.c_float),
-                ("total", ctypes.c_void_p)]
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice   # torch.cuda.current_stream(i).cuda_stream, a tenth of its time
 
 
 def _check(t, what, dtype, shape, device=None, rows=False):
     """rows: any distance between the rows; otherwise contiguous."""
+    if type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape and (t.is_cuda if device is None else t.device == device) and t.is_contiguous():
+        return
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what} must be {dtype} of shape {tuple(shape)}" +
                          (f", got {t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else ""))
     if not t.is_cuda or (device is not None and t.device != device):
         raise ValueError(f"{what} must be on {device or 'the GPU'}, got {t.device}")
-    if rows and t.dim() == 2:
-        if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-            raise ValueError(f"{what} must have consecutive elements in rows that do not overlap")
-    elif not t.is_contiguous():
+    if t.is_contiguous():
+        return
+    if not rows or t.dim() != 2:
         raise ValueError(f"{what} must be contiguous")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what} must have consecutive elements in rows that do not overlap")
 
 
 def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
+
+
+def _call(name, device, *args):
+    """The entry point on torch's current stream of `device`."""
+    i = device.index
+    if i == _current_device():
+        C.call(name, *args, _raw_stream(i))
+        return
+    with torch.cuda.device(device):
+        C.call(name, *args, _raw_stream(i))
 
 
 def quantize(x):
@@ -51,8 +55,7 @@ def quantize(x):
         raise ValueError("x must be a matrix")
     _check(x, "x", _BF16, x.shape, rows=True)
     q, scale = torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[0], dtype=_F32, device=x.device)
-    with torch.cuda.device(x.device):
-        C.call("cpmcu_w8a8_quantize", x.data_ptr(), _ld(x), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr(), _stream(x.device))
+    _call("cpmcu_w8a8_quantize", x.device, x.data_ptr(), _ld(x), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -66,9 +69,8 @@ class _Packed:
             raise ValueError(C.load().cpmcu_last_error().decode())
         self.data = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.ptr = self.data.data_ptr()
-        with torch.cuda.device(self.device):
-            for part, (q, scale) in enumerate(parts, start=int(gated)):
-                C.call("cpmcu_w8a8_pack", q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr, _stream(self.device))
+        for part, (q, scale) in enumerate(parts, start=int(gated)):
+            _call("cpmcu_w8a8_pack", self.device, q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr)
 
 
 class PackedLinear(_Packed):
@@ -105,76 +107,82 @@ class PackedGateUp(_Packed):
 
 
 def _rows(x, width, device):
+    """Checks x; (rows, distance of the rows)."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError("x must be a matrix")
-    _check(x, "x", _BF16, (x.shape[0], width), device, rows=True)
+    rows = x.shape[0]
+    if x.dtype is not _BF16 or x.device != device or x.shape[1] != width or not x.is_contiguous():
+        _check(x, "x", _BF16, (rows, width), device, rows=True)
+        return rows, _ld(x)
+    return rows, width
 
 
 def _norm(x, norm_weight, eps, delta, delta_scale):
-    """(argument, total)"""
+    """(arguments, total)"""
     if norm_weight is None:
         if delta is not None:
             raise ValueError("delta needs norm_weight")
-        return None, None
+        return (None, 0.0, None, 1.0, None), None
     _check(norm_weight, "norm_weight", _BF16, x.shape[1:], x.device)
-    total = None
-    if delta is not None:
-        _check(delta, "delta", _BF16, x.shape, x.device)
-        total = torch.empty(x.shape, dtype=_BF16, device=x.device)
-    n = Norm(norm_weight.data_ptr(), eps, None if delta is None else delta.data_ptr(), delta_scale, None if total is None else total.data_ptr())
-    return n, total
+    if delta is None:
+        return (norm_weight.data_ptr(), eps, None, 1.0, None), None
+    _check(delta, "delta", _BF16, x.shape, x.device)
+    total = delta.new_empty(x.shape)
+    return (norm_weight.data_ptr(), eps, delta.data_ptr(), delta_scale, total.data_ptr()), total
 
 
-def _out(out, rows, width, device):
+def _out(out, x, rows, width):
+    """(tensor, distance of its rows)"""
     if out is None:
-        return torch.empty(rows, width, dtype=_BF16, device=device)
-    _check(out, "out", _BF16, (rows, width), device, rows=True)
-    return out
+        return x.new_empty((rows, width)), width
+    _check(out, "out", _BF16, (rows, width), x.device, rows=True)
+    return out, _ld(out)
 
 
-def _workspace(rows, out, width, inter, device):
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows, out, width, inter):
     n = C.load().cpmcu_w8a8_workspace_bytes(rows, out, width, inter)
     if n < 0:
         raise ValueError(C.load().cpmcu_last_error().decode())
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return n
 
 
-def _call(name, device, *args):
-    if device.index == torch.cuda.current_device():
-        C.call(name, *args, _stream(device))
-        return
-    with torch.cuda.device(device):
-        C.call(name, *args, _stream(device))
+def _workspace(x, *sizes):
+    """(tensor that holds it, address, bytes): of torch's allocator, so that calls of several streams and graphs have their own."""
+    n = _workspace_bytes(*sizes)
+    if n == 0:
+        return None, None, 0
+    t = x.new_empty(n // 2)
+    return t, t.data_ptr(), n
 
 
 def linear(x, weight, bias=None, norm_weight=None, eps=1e-5, delta=None, delta_scale=1.0, out=None):
     """y [rows, out] of x [rows, in].  With norm_weight the rows are RMS norms; with delta, of t = x + delta_scale * delta, and (y, t) is
     returned.  bias [out] bf16.  x (and out) may be rows of a wider matrix."""
-    _rows(x, weight.width, weight.device)
-    if not isinstance(weight, PackedLinear):
+    if type(weight) is not PackedLinear:
         raise ValueError("weight must be a PackedLinear")
+    width, n = weight.width, weight.out
+    rows, ldx = _rows(x, width, weight.device)
     if bias is not None:
-        _check(bias, "bias", _BF16, (weight.out,), x.device)
-    rows = x.shape[0]
-    y = _out(out, rows, weight.out, x.device)
+        _check(bias, "bias", _BF16, (n,), x.device)
+        bias = bias.data_ptr()
     norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
-    ws = _workspace(rows, weight.out, weight.width, 0, x.device)
-    _call("cpmcu_w8a8_linear", x.device, x.data_ptr(), _ld(x), None if norm is None else ctypes.addressof(norm), weight.ptr,
-          None if bias is None else bias.data_ptr(), y.data_ptr(), _ld(y), rows, weight.out, weight.width, ws.data_ptr(), ws.numel())
+    y, ldy = _out(out, x, rows, n)
+    keep, ws, size = _workspace(x, rows, n, width, 0)
+    _call("cpmcu_w8a8_linear", weight.device, x.data_ptr(), ldx, weight.ptr, bias, *norm, y.data_ptr(), ldy, rows, n, width, ws, size)
     return y if total is None else (y, total)
 
 
 def gated_ffn(x, gate_up, down, norm_weight=None, eps=1e-5, delta=None, delta_scale=1.0, out=None):
     """down(silu(gate(x)) * up(x)) of x [rows, in]; norm_weight, delta and out as for linear."""
-    if not isinstance(gate_up, PackedGateUp) or not isinstance(down, PackedLinear):
+    if type(gate_up) is not PackedGateUp or type(down) is not PackedLinear:
         raise ValueError("gate_up must be a PackedGateUp and down a PackedLinear")
-    if (down.width, down.out) != (gate_up.out, gate_up.width) or down.device != gate_up.device:
-        raise ValueError(f"down must be [{gate_up.width}, {gate_up.out}] on {gate_up.device}")
-    _rows(x, gate_up.width, gate_up.device)
-    rows, width, inter = x.shape[0], gate_up.width, gate_up.out
-    y = _out(out, rows, width, x.device)
+    width, inter = gate_up.width, gate_up.out
+    if down.width != inter or down.out != width or down.device != gate_up.device:
+        raise ValueError(f"down must be [{width}, {inter}] on {gate_up.device}")
+    rows, ldx = _rows(x, width, gate_up.device)
     norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
-    ws = _workspace(rows, width, width, inter, x.device)
-    _call("cpmcu_w8a8_ffn", x.device, x.data_ptr(), _ld(x), None if norm is None else ctypes.addressof(norm), gate_up.ptr, down.ptr, y.data_ptr(),
-          _ld(y), rows, width, inter, ws.data_ptr(), ws.numel())
+    y, ldy = _out(out, x, rows, width)
+    keep, ws, size = _workspace(x, rows, width, width, inter)
+    _call("cpmcu_w8a8_ffn", gate_up.device, x.data_ptr(), ldx, gate_up.ptr, down.ptr, *norm, y.data_ptr(), ldy, rows, width, inter, ws, size)
     return y if total is None else (y, total)

@@ -22,6 +22,11 @@ auto guarded(F&& f) -> decltype(f()) {
     }
 }
 
+// The message is put together only where it is needed.
+void require(bool ok, const char* what, const char* msg) {
+    if (!ok) throw std::invalid_argument(std::string("cpmcu_b200: ") + what + ": " + msg);
+}
+
 uintptr_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 // Rows of `cols` elements of `size` bytes, `ld` elements apart.
@@ -57,13 +62,10 @@ void require_device(const char* what) {
 cudaStream_t stream_of(void* s) { return static_cast<cudaStream_t>(s); }
 
 void require_sizes(const char* what, int rows, int N, int K) {
-    const std::string name = std::string("cpmcu_b200: ") + what;
-    if (rows < 0 || N < 1 || K < 1) throw std::invalid_argument(name + ": sizes must be positive");
-    if (K > w8::MAX_COLS) throw std::invalid_argument(name + ": sums of more than 131072 products do not fit 32 bits");
-    const long long tiles = (N + 63) / 64;
-    if (tiles * (w8::pad_cols(K) / w8::BLOCK_COLS) > (1ll << 23) || ((static_cast<long long>(rows) + 15) / 16) * tiles > (1ll << 30)) {
-        throw std::invalid_argument(name + ": too many tiles");
-    }
+    require(rows >= 0 && N >= 1 && K >= 1, what, "sizes must be positive");
+    require(K <= w8::MAX_COLS, what, "sums of more than 131072 products do not fit 32 bits");
+    const long long tiles = (static_cast<long long>(N) + 63) / 64;
+    require(tiles * (w8::pad_cols(K) / w8::BLOCK_COLS) <= (1ll << 23) && ((static_cast<long long>(rows) + 15) / 16) * tiles <= (1ll << 30), what, "too many tiles");
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -87,7 +89,7 @@ Layout layout_of(int rows, int N, int K, int inter) {
         l.xs = take(align256(rows) * sizeof(float));
         // the down projection's, or the only product's
         const int k_last = inter > 0 ? inter : K;
-        l.n_tickets = w8::product_tickets(rows, N, false);
+        l.n_tickets = w8::product_tickets(rows, N, k_last, false);
         l.tickets = take(l.n_tickets * sizeof(int));
         l.partials = take(w8::product_partial_bytes(rows, N, k_last, false));
     }
@@ -95,45 +97,41 @@ Layout layout_of(int rows, int N, int K, int inter) {
     return l;
 }
 
-w8::RowSource source_of(const char* what, const void* x, long long ldx, const cpmcu_w8a8_norm* norm, int rows, int K, const void* y, long long ldy, int out) {
-    const std::string name = std::string("cpmcu_b200: ") + what;
-    auto require = [&](bool ok, const char* msg) { if (!ok) throw std::invalid_argument(name + ": " + msg); };
-    require(x != nullptr && y != nullptr, "x and y must not be null");
-    require(ldx >= K && ldy >= out, "rows overlap: a leading dimension is smaller than the row");
-    require(ldy < (1ll << 31), "the leading dimension of y does not fit 32 bits");
+w8::RowSource source_of(const char* what, const void* x, long long ldx, const void* norm, float eps, const void* delta, float delta_scale, void* total,
+                        int rows, int K, const void* y, long long ldy, int out) {
+    require(x != nullptr && y != nullptr, what, "x and y must not be null");
+    require(ldx >= K && ldy >= out, what, "rows overlap: a leading dimension is smaller than the row");
+    require(ldy < (1ll << 31), what, "the leading dimension of y does not fit 32 bits");
+    require(norm != nullptr || delta == nullptr, what, "a delta needs the norm's weights");
+    require((delta == nullptr) == (total == nullptr), what, "delta and total come together");
     w8::RowSource s;
     s.x = static_cast<const bf16*>(x);
     s.ldx = ldx;
     const Rows xr{x, rows, K, ldx, 2}, yr{y, rows, out, ldy, 2};
-    require(!overlap(xr, yr), "y must not overlap x");
+    require(!overlap(xr, yr), what, "y must not overlap x");
     if (norm != nullptr) {
-        require(norm->weight != nullptr, "a norm needs its weights");
-        require((norm->delta == nullptr) == (norm->total == nullptr), "delta and total come together");
-        s.norm = static_cast<const bf16*>(norm->weight);
-        s.eps = norm->eps;
-        s.delta = static_cast<const bf16*>(norm->delta);
-        s.total = static_cast<bf16*>(norm->total);
-        s.delta_scale = norm->delta_scale;
-        const Rows dr{norm->delta, rows, K, K, 2}, tr{norm->total, rows, K, K, 2}, wr{norm->weight, 1, K, K, 2};
-        require(!overlap(tr, xr) && !overlap(tr, dr) && !overlap(tr, yr) && !overlap(tr, wr), "total must not overlap x, delta, y or the weights");
-        require(!overlap(yr, dr) && !overlap(yr, wr), "y must not overlap delta or the weights");
+        s.norm = static_cast<const bf16*>(norm);
+        s.eps = eps;
+        s.delta = static_cast<const bf16*>(delta);
+        s.total = static_cast<bf16*>(total);
+        s.delta_scale = delta_scale;
+        const Rows dr{delta, rows, K, K, 2}, tr{total, rows, K, K, 2}, wr{norm, 1, K, K, 2};
+        require(!overlap(tr, xr) && !overlap(tr, dr) && !overlap(tr, yr) && !overlap(tr, wr), what, "total must not overlap x, delta, y or the weights");
+        require(!overlap(yr, dr) && !overlap(yr, wr), what, "y must not overlap delta or the weights");
     }
     return s;
 }
 
 void require_workspace(const char* what, void* ws, long long bytes, const Layout& l) {
     if (l.total == 0) return;
-    const std::string name = std::string("cpmcu_b200: ") + what;
     if (ws == nullptr || bytes < 0 || static_cast<size_t>(bytes) < l.total) {
-        throw std::invalid_argument(name + ": the workspace needs " + std::to_string(l.total) + " bytes");
+        throw std::invalid_argument(std::string("cpmcu_b200: ") + what + ": the workspace needs " + std::to_string(l.total) + " bytes");
     }
-    if ((addr(ws) & 255) != 0) throw std::invalid_argument(name + ": the workspace must be 256-byte aligned");
+    require((addr(ws) & 255) == 0, what, "the workspace must be 256-byte aligned");
 }
 
 void require_packed(const char* what, const void* packed) {
-    if (packed == nullptr || (addr(packed) & 255) != 0) {
-        throw std::invalid_argument(std::string("cpmcu_b200: ") + what + ": packed weights must be 256-byte aligned");
-    }
+    require(packed != nullptr && (addr(packed) & 255) == 0, what, "packed weights must be 256-byte aligned");
 }
 
 }  // namespace
@@ -202,13 +200,13 @@ long cpmcu_w8a8_workspace_bytes(int rows, int N, int K, int inter) {
     });
 }
 
-int cpmcu_w8a8_linear(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, const void* packed, const void* bias, void* y, long long ldy,
-                      int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream) {
+int cpmcu_w8a8_linear(const void* x, long long ldx, const void* packed, const void* bias, const void* norm, float eps, const void* delta,
+                      float delta_scale, void* total, void* y, long long ldy, int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream) {
     return guarded([&] {
         require_sizes("w8a8_linear", rows, N, K);
         if (rows == 0) return 0;
         require_packed("w8a8_linear", packed);
-        const w8::RowSource src = source_of("w8a8_linear", x, ldx, norm, rows, K, y, ldy, N);
+        const w8::RowSource src = source_of("w8a8_linear", x, ldx, norm, eps, delta, delta_scale, total, rows, K, y, ldy, N);
         const Layout l = layout_of(rows, N, K, 0);
         require_workspace("w8a8_linear", workspace, workspace_bytes, l);
         require_device("w8a8_linear");
@@ -235,15 +233,15 @@ int cpmcu_w8a8_linear(const void* x, long long ldx, const cpmcu_w8a8_norm* norm,
     });
 }
 
-int cpmcu_w8a8_ffn(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, const void* gate_up, const void* down, void* y, long long ldy, int rows,
-                   int K, int inter, void* workspace, long long workspace_bytes, void* stream) {
+int cpmcu_w8a8_ffn(const void* x, long long ldx, const void* gate_up, const void* down, const void* norm, float eps, const void* delta,
+                   float delta_scale, void* total, void* y, long long ldy, int rows, int K, int inter, void* workspace, long long workspace_bytes, void* stream) {
     return guarded([&] {
         require_sizes("w8a8_ffn", rows, inter, K);
         require_sizes("w8a8_ffn", rows, K, inter);
         if (rows == 0) return 0;
         require_packed("w8a8_ffn", gate_up);
         require_packed("w8a8_ffn", down);
-        const w8::RowSource src = source_of("w8a8_ffn", x, ldx, norm, rows, K, y, ldy, K);
+        const w8::RowSource src = source_of("w8a8_ffn", x, ldx, norm, eps, delta, delta_scale, total, rows, K, y, ldy, K);
         const Layout l = layout_of(rows, K, K, inter);
         require_workspace("w8a8_ffn", workspace, workspace_bytes, l);
         require_device("w8a8_ffn");

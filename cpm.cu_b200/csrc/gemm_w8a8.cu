@@ -3,10 +3,11 @@
 //
 // Operand mapping as for the bf16 products (gemm_umma.cu): weights are the A operand (128 rows of a tile), token rows the B operand, the
 // accumulator is Y^T.  A k-block is 128 integers, one 128-byte swizzle row, so a stage has the bytes of a bf16 stage and twice the products.
-//   M <= 64, and few tiles        clusters of 2 to 4 CTAs that cut a tile's k-blocks evenly and sum it in distributed shared memory
-//   M <= 256                      single CTAs, the line of all (tile, k-block) units cut evenly (stream-K)
-//   M > 256, tiles in twos        pairs of CTAs on tiles of 256 x 256 (tcgen05 cta_group::2): half of the operand bytes per product; whole
-//                                 tiles in waves, only those of the last wave are cut
+//   M <= 64, and few tiles   clusters of 2 to 4 CTAs that cut a tile's k-blocks evenly and sum it in distributed shared memory
+//   M <= 64                  single CTAs on whole tiles, or the line of all (tile, k-block) units cut evenly (stream-K)
+//   M > 64                   token tiles of 64, 128 or 256 on single CTAs, or pairs of CTAs on tiles of 256 x 256 (tcgen05 cta_group::2: half of the
+//                            operand bytes per product), whichever division divide() expects to end first; whole tiles in waves, and only those
+//                            of the last wave are cut
 // Bound: the weights' bytes from HBM up to some 300 rows, the tensor pipe (and, with warm passes, the power cap) beyond.
 //
 // Cut tiles: each piece but the last counted one leaves its int32 sums in a workspace slot, the one counted last adds them to its own.  Integer
@@ -133,7 +134,7 @@ __device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act
 #pragma unroll
         for (int c = 0; c < HB; ++c) {
             const float other = in[c * 32 + lane];
-            const float v = silu_f32(gates ? mine[c] : other) * (gates ? other : mine[c]);
+            const float v = silu_fast(gates ? mine[c] : other) * (gates ? other : mine[c]);
             if (first + c < m_cnt && n0 + lane < N) dst[c * ld] = v;
         }
         ptx::named_bar_sync(pair_bar, 64);   // the partner may write `in` again
@@ -558,7 +559,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
             ptx::named_bar_sync(1, 128);
             const int f = row & 63, n = tile * 64 + f;
             for (int t = row >> 6; t < cnt; t += 2) {
-                if (n < a.N) a.act[static_cast<long long>(t0 + t) * a.ldy + n] = silu_f32(meet[t * TILE_ROWS + f]) * meet[t * TILE_ROWS + 64 + f];
+                if (n < a.N) a.act[static_cast<long long>(t0 + t) * a.ldy + n] = silu_fast(meet[t * TILE_ROWS + f]) * meet[t * TILE_ROWS + 64 + f];
             }
         }
     }
@@ -576,20 +577,24 @@ CUtensorMap map_rows(const void* base, long long rows, long long cols, int box_r
     return make_tmap_2d_u8_sw128(base, cols, rows, cols, BLOCK_COLS, box_rows);
 }
 
-// A kernel's shared memory limit; harmless when two threads set it at once
 template <typename... A>
-void allow_smem(void (*kernel)(A...), int bytes) { CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)); }
+bool allow_smem(void (*kernel)(A...), int bytes) {
+    CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return true;
+}
 
 template <int MT, bool PAIR>
 void run(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
     using C = Cfg<MT, PAIR>;
-    allow_smem(product_s8_kernel<MT, PAIR>, C::SMEM_BYTES);
+    static const bool allowed = allow_smem(product_s8_kernel<MT, PAIR>, C::SMEM_BYTES);   // the library runs on one device
+    (void)allowed;
     launch(product_s8_kernel<MT, PAIR>, grid, NUM_THREADS, C::SMEM_BYTES, s, PAIR ? 2 : 1, true, tw, tx, a);
 }
 template <int MT, int CS>
 void run_cluster(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
     using C = ClusterCfg<MT, CS>;
-    allow_smem(product_s8_cluster_kernel<MT, CS>, C::SMEM_BYTES);
+    static const bool allowed = allow_smem(product_s8_cluster_kernel<MT, CS>, C::SMEM_BYTES);
+    (void)allowed;
     launch(product_s8_cluster_kernel<MT, CS>, grid, NUM_THREADS, C::SMEM_BYTES, s, CS, true, tw, tx, a);
 }
 template <int MT>
@@ -633,7 +638,27 @@ Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
             }
         }
     }
-    d.pair = d.m_tiles > 1 && tiles % 2 == 0;
+    if (M > 64) {
+        // Cycles of a k-block, measured in long products (operands from L2 bound the small tiles), and of a tile's way out of tensor memory, of
+        // which a launch shows the last one.
+        struct Kind { int mt; bool pair; int block, out; };
+        static const Kind kinds[] = {{64, false, 480, 1500}, {128, false, 640, 3000}, {256, false, 960, 6000}, {256, true, 640, 6000}};
+        long long best = -1;
+        for (const Kind& k : kinds) {
+            if (k.pair && (tiles % 2 != 0 || M <= 128)) continue;
+            const int m_tiles = ceil_div(M, k.mt);
+            const long long n = static_cast<long long>(k.pair ? tiles / 2 : tiles) * m_tiles, workers = k.pair ? sms / 2 : sms;
+            // blocks of the busiest worker: whole tiles, or even pieces of at least eight blocks
+            const long long blocks = gated || n * kblocks < workers * 8 ? (n + workers - 1) / workers * kblocks : (n * kblocks + workers - 1) / workers;
+            const long long cost = blocks * k.block + k.out;
+            if (best < 0 || cost < best) {
+                best = cost;
+                d.mt = k.mt;
+                d.pair = k.pair;
+                d.m_tiles = m_tiles;
+            }
+        }
+    }
     const int n_tiles = d.pair ? tiles / 2 : tiles, most = d.pair ? sms / 2 : sms;
     const long long all = static_cast<long long>(n_tiles) * d.m_tiles;
     if (gated) {
@@ -670,8 +695,10 @@ size_t product_partial_bytes(int M, int N, int K, bool gated) {
     const Division d = divide(M, tiles_of(N, gated), pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms);
     return d.cluster > 0 ? 0 : static_cast<size_t>(d.workers) * (d.pair ? 2 : 1) * 2 * d.mt * TILE_ROWS * sizeof(int);
 }
-int product_tickets(int M, int N, bool gated) {
-    return gated || M <= 1 ? 0 : tiles_of(N, gated) * ceil_div(M, linear_pick_mt(M));
+int product_tickets(int M, int N, int K, bool gated) {
+    if (gated || M <= 1) return 0;
+    const int tiles = tiles_of(N, gated);
+    return tiles * divide(M, tiles, pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms).m_tiles;
 }
 
 void launch_product(const Product& p, cudaStream_t s) {
@@ -703,7 +730,10 @@ void launch_product(const Product& p, cudaStream_t s) {
         else run_cluster<64>(d.cluster, tw, tx, a, grid, s);
         return;
     }
-    if (d.pair) { run<256, true>(tw, tx, a, 2 * d.workers, s); return; }
+    if (d.pair) {
+        run<256, true>(tw, tx, a, 2 * d.workers, s);
+        return;
+    }
     switch (d.mt) {
         case 16: run<16, false>(tw, tx, a, d.workers, s); break;
         case 32: run<32, false>(tw, tx, a, d.workers, s); break;

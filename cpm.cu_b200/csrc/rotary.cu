@@ -4,7 +4,7 @@
 // Rotated keys, and values as they are, go to the row's cache slot.
 //
 // The angle is a 64-bit product, reduced to a fraction of a turn before it becomes fp32: at position 10^6 an fp32 product is off by 0.03
-// radians.  One CTA per row: its first loads are in flight while some threads make the row's `half` sines and cosines.
+// radians.  One CTA per row: its loads are in flight while some threads make the row's `half` sines and cosines.
 //
 // Bound: every element in and out once.
 #include "row_ops.cuh"
@@ -93,16 +93,25 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     const int all = a.heads + a.kv_heads;
     auto target = [&](int h, int c) { return h < a.heads ? q + h * a.dim + c : k + (h - a.heads) * a.dim + c; };
 
-    int i = threadIdx.x;
+    // the first pieces of each kind are in flight before the table is made
+    constexpr int AHEAD = 2;
     const int items = all * turned;
-    Piece<VEC, INTERLEAVED, WIDE> piece;
-    int h = 0, c = 0;
-    auto fetch = [&]() {
+    Piece<VEC, INTERLEAVED, WIDE> piece[AHEAD];
+    const bf16* v = row + all * a.dim;
+    Elems<VEC, WIDE> value;
+    const int v0 = threadIdx.x * VEC;
+    auto place = [&](int i, int& h, int& c) {
         h = i / turned;
         c = (i - h * turned) * VEC;
-        piece.load(row + h * a.dim + c, a.half);
     };
-    if (i < items) fetch();
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        int h, c;
+        place(i, h, c);
+        if (i < items) piece[j].load(row + h * a.dim + c, a.half);
+    }
+    if (keep && v0 < kv_dim) value.load(v + v0);
     const double p = a.pos[r];
     for (int t = threadIdx.x; t < a.half; t += blockDim.x) {
         const double turns = p * static_cast<double>(a.inv_freq[t]) * 0.15915494309189533577;
@@ -110,12 +119,25 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
         sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
         table[t] = make_float2(cs * a.factor, sn * a.factor);
     }
+    bf16* v_row = a.v_cache + slot * kv_dim;
+    if (keep && v0 < kv_dim) value.store(v_row + v0);
     __syncthreads();
-    while (i < items) {
-        piece.rotate(c, a.half, table);
-        if (h < a.heads || keep) piece.store(target(h, c), a.half);
-        i += blockDim.x;
-        if (i < items) fetch();
+    auto finish = [&](Piece<VEC, INTERLEAVED, WIDE>& e, int h, int c) {
+        e.rotate(c, a.half, table);
+        if (h < a.heads || keep) e.store(target(h, c), a.half);
+    };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        int h, c;
+        place(i, h, c);
+        if (i < items) finish(piece[j], h, c);
+    }
+    for (int i = threadIdx.x + AHEAD * blockDim.x; i < items; i += blockDim.x) {
+        int h, c;
+        place(i, h, c);
+        piece[0].load(row + h * a.dim + c, a.half);
+        finish(piece[0], h, c);
     }
     // what no rotation reaches: the rest of the heads, and the values
     for (int j = threadIdx.x; j < all * copied; j += blockDim.x) {
@@ -125,12 +147,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
         if (hh < a.heads || keep) e.store(target(hh, cc));
     }
     if (keep) {
-        const bf16* v = row + all * a.dim;
-        bf16* dst = a.v_cache + slot * kv_dim;
-        for (int j = threadIdx.x * VEC; j < kv_dim; j += blockDim.x * VEC) {
-            Elems<VEC, WIDE> e;
-            e.load(v + j);
-            e.store(dst + j);
+        for (int j = v0 + blockDim.x * VEC; j < kv_dim; j += blockDim.x * VEC) {
+            value.load(v + j);
+            value.store(v_row + j);
         }
     }
 }

@@ -58,7 +58,7 @@ struct Product {
     int* tickets = nullptr;         // zero
 };
 size_t product_partial_bytes(int M, int N, int K, bool gated);
-int product_tickets(int M, int N, bool gated);
+int product_tickets(int M, int N, int K, bool gated);
 void launch_product(const Product& p, cudaStream_t s);
 // one row, straight from its source
 void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const bf16* bias, bf16* y, float* act, cudaStream_t s);
@@ -86,46 +86,6 @@ void launch(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStre
     cfg.attrs = attr;
     cfg.numAttrs = n;
     CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
-}
-
-// ---------------------------------------------------------------- rounding of a row
-// q = round(127 v / top) to nearest, even at ties, exactly: with both scaled by a power of two so that nothing over- or underflows, an estimate
-// from the reciprocal is at most one off, and the rest 127 v - q top, which is exact in fp32 for v of up to 17 significant bits (bf16
-// values and products of two of them), decides.  fp32 rows round on the same estimate; their ties are those of their fp32 quotients.
-struct RowRound {
-    float c127, top, inv;
-    bool finite;
-    // bits: largest of the magnitudes' bit patterns (infinities and NaN are above all finite ones)
-    __device__ __forceinline__ explicit RowRound(uint32_t bits) {
-        finite = bits < 0x7f800000u;
-        const float v = __uint_as_float(bits);
-        int e = static_cast<int>(bits >> 23) - 127;              // top is in [2^e, 2^(e+1)), or below where it is subnormal
-        e = e < -119 ? -119 : e;
-        const float c = __uint_as_float(static_cast<uint32_t>(127 - (e > 126 ? 126 : e)) << 23);
-        c127 = 127.f * c;
-        top = v * c;
-        const bool some = finite && bits != 0u;
-        inv = some ? 1.f / top : 0.f;
-        if (!some) c127 = 0.f;
-    }
-    __device__ __forceinline__ int operator()(float v) const {
-        const float p = v * c127;
-        float r = rintf(p * inv);
-        const float rest = fmaf(-r, top, p);
-        const float twice = 2.f * fabsf(rest);
-        if (twice > top || (twice == top && (static_cast<int>(r) & 1))) r += copysignf(1.f, rest);
-        return static_cast<int>(r);
-    }
-    // the row's scale: NaN for a row with an infinity or a NaN, so that its outputs are NaN
-    __device__ __forceinline__ static float scale(uint32_t bits, float factor) {
-        return bits < 0x7f800000u ? __uint_as_float(bits) / 127.f * factor : __uint_as_float(0x7fffffffu);
-    }
-};
-
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
 }
 
 }  // namespace w8

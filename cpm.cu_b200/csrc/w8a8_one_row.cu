@@ -1,37 +1,35 @@
 // One row of an 8-bit linear layer, sm_100a:  y[N] = (q . W_n) * scale * scale_n + bias_n, with q made of the row inside the launch (w8a8_rows.cuh).
 //
-// Bound: the weights' bytes from HBM.  One CTA of 32 warps per SM makes the integers of the row once, in shared memory; the weights of a warp's
-// first batch, eight 16-byte loads a lane, are on their way meanwhile: 128 KB per SM, so that a product of up to 19 MB is in flight
-// as a whole before its integers are there.  Eight lanes read 128 consecutive bytes of one weight row, a warp four rows (512 bytes) per
-// k-block; S warps share the k-blocks of a group of rows and meet in shared memory, S chosen so that the groups divide evenly among the SMs.
-// dp4a sums four products: 4 of them per 16 bytes, far below what the lanes can do at the HBM rate.
+// Bound: the weights' bytes from HBM.  One CTA of 16 warps per SM makes the integers of the row once, in shared memory.  Weights come through
+// asynchronous 16-byte copies into slots of shared memory that one lane writes and reads (no barriers): 80 KB per SM are in flight, the first of
+// them before the wait for the predecessor and while the integers are made, and no registers hold them, so that the next launch's CTAs fit
+// beside this one's and its weights are on their way before this one ends.  Eight lanes read 128 consecutive bytes of one weight row, a
+// warp four rows (512 bytes) per k-block; S warps share the k-blocks of a group of rows and meet in shared memory, S chosen so
+// that the groups divide evenly among the SMs.  dp4a sums four products: 4 of them per 16 bytes, far below what the lanes can do at
+// the HBM rate.
 #include <algorithm>
 
+#include "ptx.cuh"
 #include "w8a8_rows.cuh"
 
 namespace w8 {
 namespace {
 
-constexpr int WARPS = 32, THREADS = WARPS * 32;
-constexpr int BATCH = 8;                              // 16-byte loads per lane in flight
-constexpr int MAX_STAGE_BYTES = 200 * 1024;
+constexpr int WARPS = 16, THREADS = WARPS * 32;
+constexpr int SLOTS = 10;                             // 16-byte copies per lane in flight
+constexpr int RING_BYTES = SLOTS * THREADS * 16;
+constexpr int KEEP = 4;                               // vectors of 8 that a thread keeps of the row
+constexpr int MAX_SMEM = RING_BYTES + MAX_COLS;
 
 struct OneRowArgs {
     RowSource src;
     Packed w;
     int N, K, share, units, rounds;   // share: warps per group of rows; units: groups of 4 (gated: 4 + 4) rows
-    int staged;                       // the row's fp32 values fit beside its integers
     const bf16* bias;
     bf16* y;
     float* act;
 };
 
-// past the first-level cache, and kept in its place: before the wait (w8a8.cuh)
-__device__ __forceinline__ uint4 load_weights(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-    return v;
-}
 __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
     acc = __dp4a(static_cast<int>(a.x), static_cast<int>(b.x), acc);
     acc = __dp4a(static_cast<int>(a.y), static_cast<int>(b.y), acc);
@@ -41,88 +39,125 @@ __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
 
 // Lets its successor start behind its own wait, so that the successor's weights are older than this launch's predecessor.
 template <Source SRC, int VEC, bool GATED>
-__global__ void __launch_bounds__(THREADS, 1) one_row_s8_kernel(const OneRowArgs a) {
+__global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs a) {
     constexpr int SETS = GATED ? 2 : 1;               // gate and up rows of the same features
-    constexpr int KB = BATCH / SETS;                  // k-blocks per batch
+    constexpr int DEPTH = SLOTS / SETS;               // steps in flight
     constexpr int TILE_UNITS = (GATED ? TILE_ROWS / 2 : TILE_ROWS) / 4;
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(16) uint8_t smem[];   // ring, then the integers
     __shared__ uint32_t sh_top[32];
     __shared__ float sh_sum[32];
     __shared__ int part[2][WARPS][4 * SETS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int slots = WARPS / a.share, slot = warp / a.share, ks = warp % a.share;
     const int kblocks = a.w.kblocks;
-    const int batches = ceil_div_dev(ceil_div_dev(kblocks, a.share), KB);
+    uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;
 
-    uint4 wv[KB][SETS];
+    // ---- copies: steps (round, k-block) in the order of their use; a step's place in the ring is its number modulo DEPTH
+    int load_round = 0, load_kb = ks, load_at = 0;
+    const uint8_t* load_from = nullptr;
     auto unit_of = [&](int round) { return (blockIdx.x + round * gridDim.x) * slots + slot; };
-    auto load = [&](int round, int batch) {
-        const int unit = unit_of(round);
-        const uint8_t* base = a.w.blocks + static_cast<size_t>(unit / TILE_UNITS) * kblocks * BLOCK_BYTES +
-                              ((unit % TILE_UNITS) * 4 + (lane >> 3)) * BLOCK_COLS + (lane & 7) * 16;
-#pragma unroll
-        for (int u = 0; u < KB; ++u) {
-            const int kb = ks + a.share * (batch * KB + u);
+    auto seek = [&]() {   // first bytes of this lane in the unit of load_round; null behind the last unit
+        const int unit = unit_of(load_round);
+        load_from = load_round < a.rounds && unit < a.units ? a.w.blocks + static_cast<size_t>(unit / TILE_UNITS) * kblocks * BLOCK_BYTES +
+                                                                  ((unit % TILE_UNITS) * 4 + (lane >> 3)) * BLOCK_COLS + (lane & 7) * 16
+                                                            : nullptr;
+    };
+    auto issue = [&]() {
+        if (load_kb >= kblocks && load_round < a.rounds) {
+            ++load_round;
+            load_kb = ks;
+            seek();
+        }
+        if (load_from != nullptr && load_kb < kblocks) {
 #pragma unroll
             for (int g = 0; g < SETS; ++g) {
-                wv[u][g] = unit < a.units && kb < kblocks ? load_weights(base + static_cast<size_t>(kb) * BLOCK_BYTES + g * (TILE_ROWS / 2) * BLOCK_COLS)
-                                                          : make_uint4(0u, 0u, 0u, 0u);
+                ptx::cp_async16(ring + (load_at * SETS + g) * THREADS, load_from + static_cast<size_t>(load_kb) * BLOCK_BYTES + g * (TILE_ROWS / 2) * BLOCK_COLS, 16);
             }
         }
+        ptx::cp_async_commit();   // empty groups keep the count
+        load_kb += a.share;
+        load_at = load_at + 1 == DEPTH ? 0 : load_at + 1;
     };
-    load(0, 0);
+    seek();
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) issue();
     grid_dep_wait();
     grid_dep_trigger();
 
     // ---- the row's integers
-    int8_t* q = reinterpret_cast<int8_t*>(smem);
-    float* stage = reinterpret_cast<float*>(smem + kblocks * BLOCK_COLS);
+    int8_t* q = reinterpret_cast<int8_t*>(smem + RING_BYTES);
     uint32_t top = 0u;
     float ss = 0.f;
-    for (int c = threadIdx.x * VEC; c < a.K; c += THREADS * VEC) {
+    Values<SRC, VEC> kept[KEEP];
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+        const int c = (threadIdx.x + j * THREADS) * VEC;
+        if (c < a.K) kept[j].fetch(a.src, 0, a.K, c);
+    }
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+        const int c = (threadIdx.x + j * THREADS) * VEC;
+        if (c < a.K) {
+            kept[j].combine(a.src, 0, a.K, c, blockIdx.x == 0);
+            kept[j].measure(a.src, c, top, ss);
+        }
+    }
+    for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {   // of longer rows: read again below
         Values<SRC, VEC> r;
         r.fetch(a.src, 0, a.K, c);
-        r.combine(a.src, 0, a.K, c, ss, blockIdx.x == 0);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) top = max(top, magnitude(r.v[e]));
-        if (a.staged) store_vec<VEC>(stage + c, r.v);
+        r.combine(a.src, 0, a.K, c, blockIdx.x == 0);
+        r.measure(a.src, c, top, ss);
     }
     top = block_max(top, sh_top);
     float factor = 1.f;
-    if constexpr (SRC == SRC_NORM || SRC == SRC_ADD_NORM) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
+    if constexpr (HAS_NORM<SRC>) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
     const RowRound round8(top);
-    for (int c = threadIdx.x * VEC; c < a.K; c += THREADS * VEC) {
-        Values<SRC, VEC> r;
-        if (a.staged) {
-            load_vec<VEC>(stage + c, r.v);
-        } else {
-            float unused = 0.f;
-            r.fetch(a.src, 0, a.K, c);
-            r.combine(a.src, 0, a.K, c, unused, false);
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+        const int c = (threadIdx.x + j * THREADS) * VEC;
+        if (c < a.K) {
+            float v[VEC];
+            kept[j].values(a.src, c, v);
+            store_ints<VEC>(q + c, round8, v);
         }
-        store_ints<VEC>(q + c, round8, r.v);
+    }
+    for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {
+        Values<SRC, VEC> r;
+        float v[VEC];
+        r.fetch(a.src, 0, a.K, c);
+        r.combine(a.src, 0, a.K, c, false);
+        r.values(a.src, c, v);
+        store_ints<VEC>(q + c, round8, v);
     }
     for (int c = a.K + threadIdx.x; c < kblocks * BLOCK_COLS; c += THREADS) q[c] = 0;
     const float scale = RowRound::scale(top, factor);
     __syncthreads();
 
     // ---- products
+    int at = 0;
     for (int round = 0; round < a.rounds; ++round) {
+        const int unit = unit_of(round);
+        const int tile = unit / TILE_UNITS, row = (unit % TILE_UNITS) * 4 + (lane >> 3);
+        const int n = tile * (GATED ? TILE_ROWS / 2 : TILE_ROWS) + row;
+        const bool writes = ks == 0 && (lane & 7) == 0 && unit < a.units && n < a.N;
+        float ws = 0.f, ws_up = 0.f, bias = 0.f;
+        if (writes) {   // here before the sums are
+            ws = __ldcg(a.w.scales + tile * TILE_ROWS + row);
+            if constexpr (GATED) ws_up = __ldcg(a.w.scales + tile * TILE_ROWS + row + TILE_ROWS / 2);
+            else if (a.bias != nullptr) bias = __bfloat162float(a.bias[n]);
+        }
         int acc[SETS];
 #pragma unroll
         for (int g = 0; g < SETS; ++g) acc[g] = 0;
-        for (int batch = 0; batch < batches; ++batch) {
+        for (int kb = ks; kb < kblocks; kb += a.share) {
+            ptx::cp_async_wait<DEPTH - 1>();
+            if (unit < a.units) {
+                const uint4 x = *reinterpret_cast<const uint4*>(q + kb * BLOCK_COLS + (lane & 7) * 16);
 #pragma unroll
-            for (int u = 0; u < KB; ++u) {
-                const int kb = ks + a.share * (batch * KB + u);
-                if (kb < kblocks) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(q + kb * BLOCK_COLS + (lane & 7) * 16);
-#pragma unroll
-                    for (int g = 0; g < SETS; ++g) acc[g] = dot16(wv[u][g], x, acc[g]);
-                }
+                for (int g = 0; g < SETS; ++g) acc[g] = dot16(ring[(at * SETS + g) * THREADS], x, acc[g]);
             }
-            if (batch + 1 < batches) load(round, batch + 1);
-            else if (round + 1 < a.rounds) load(round + 1, 0);
+            at = at + 1 == DEPTH ? 0 : at + 1;
+            issue();
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) {
@@ -134,8 +169,7 @@ __global__ void __launch_bounds__(THREADS, 1) one_row_s8_kernel(const OneRowArgs
 #pragma unroll
                 for (int g = 0; g < SETS; ++g) part[round & 1][warp][g * 4 + (lane >> 3)] = acc[g];
             }
-            // the warps of one group: at most eight groups
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + slot), "r"(a.share * 32) : "memory");
+            ptx::named_bar_sync(1 + slot, a.share * 32);   // the warps of one group: at most eight groups
             if (ks == 0) {
 #pragma unroll
                 for (int g = 0; g < SETS; ++g) {
@@ -147,27 +181,22 @@ __global__ void __launch_bounds__(THREADS, 1) one_row_s8_kernel(const OneRowArgs
                 }
             }
         }
-        const int unit = unit_of(round);
-        if (ks == 0 && (lane & 7) == 0 && unit < a.units) {
-            const int tile = unit / TILE_UNITS, row = (unit % TILE_UNITS) * 4 + (lane >> 3);
-            const int n = tile * (GATED ? TILE_ROWS / 2 : TILE_ROWS) + row;
-            if (n < a.N) {
-                const float* ws = a.w.scales + tile * TILE_ROWS + row;
-                const float v = static_cast<float>(acc[0]) * scale * ws[0];
-                if constexpr (GATED) {
-                    a.act[n] = silu_f32(v) * (static_cast<float>(acc[SETS - 1]) * scale * ws[TILE_ROWS / 2]);
-                } else {
-                    a.y[n] = __float2bfloat16(v + (a.bias != nullptr ? __bfloat162float(a.bias[n]) : 0.f));
-                }
-            }
+        if (writes) {
+            const float v = static_cast<float>(acc[0]) * scale;
+            if constexpr (GATED) a.act[n] = silu_fast(v * ws) * (static_cast<float>(acc[SETS - 1]) * scale * ws_up);
+            else a.y[n] = __float2bfloat16(fmaf(v, ws, bias));
         }
     }
+    ptx::cp_async_wait<0>();
 }
 
 template <Source SRC, int VEC, bool GATED>
 void run(const OneRowArgs& a, int grid, size_t smem, cudaStream_t s) {
-    // the attribute belongs to the function on this device; setting it again costs a fraction of a launch and needs no flag that threads share
-    CUDA_CHECK(cudaFuncSetAttribute(one_row_s8_kernel<SRC, VEC, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_STAGE_BYTES));
+    static const bool allowed = [] {   // the library runs on one device
+        CUDA_CHECK(cudaFuncSetAttribute(one_row_s8_kernel<SRC, VEC, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM));
+        return true;
+    }();
+    (void)allowed;
     launch(one_row_s8_kernel<SRC, VEC, GATED>, grid, THREADS, smem, s, 1, true, a);
 }
 template <Source SRC, bool GATED>
@@ -186,13 +215,12 @@ void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const b
     a.N = N; a.K = K;
     a.bias = bias; a.y = y; a.act = act;
     a.units = w.tiles * (gated ? 16 : 32);
-    // Warps per group: the fewest rounds times batches, the fewest warps of those (a shared group costs a barrier a round)
-    const int sms = runtime().num_sms, per_batch = gated ? BATCH / 2 : BATCH;
+    // Warps per group: the fewest steps of the busiest warp, with half a step for each round's meeting
+    const int sms = runtime().num_sms;
     long long best = -1;
-    for (int share = 1; share <= WARPS; share *= (share == 1 ? 4 : 2)) {
-        const int slots = WARPS / share;
-        const int rounds = ceil_div(ceil_div(a.units, slots), sms);
-        const long long cost = static_cast<long long>(rounds) * ceil_div(ceil_div(w.kblocks, share), per_batch);
+    for (int share = 1; share <= WARPS; share *= 2) {
+        const int rounds = ceil_div(ceil_div(a.units, WARPS / share), sms);
+        const long long cost = static_cast<long long>(rounds) * (2 * ceil_div(w.kblocks, share) + (share > 1 ? 1 : 0));
         if (best < 0 || cost < best) {
             best = cost;
             a.share = share;
@@ -200,9 +228,7 @@ void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const b
         }
     }
     const int grid = std::min(sms, ceil_div(a.units, WARPS / a.share));
-    const size_t ints = static_cast<size_t>(w.kblocks) * BLOCK_COLS, floats = (static_cast<size_t>(K) + 7) / 8 * 32;
-    a.staged = ints + floats <= static_cast<size_t>(MAX_STAGE_BYTES);
-    const size_t smem = ints + (a.staged ? floats : 0);
+    const size_t smem = RING_BYTES + static_cast<size_t>(w.kblocks) * BLOCK_COLS;
     const bool vec = rows_in_vectors(src, K);
     if (src.x32 != nullptr) run<SRC_F32, false>(a, grid, smem, vec, s);
     else if (src.norm == nullptr) gated ? run<SRC_PLAIN, true>(a, grid, smem, vec, s) : run<SRC_PLAIN, false>(a, grid, smem, vec, s);

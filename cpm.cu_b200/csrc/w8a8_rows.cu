@@ -32,53 +32,53 @@ __global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const Qua
     grid_dep_trigger();
     const size_t row = blockIdx.x;
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < a.n_clear; i += gridDim.x * blockDim.x) a.clear[i] = 0;
-    constexpr int N = VPT > 0 ? VPT : 1;
-    Values<SRC, VEC> row_values[N];
+    Values<SRC, VEC> kept[VPT > 0 ? VPT : 1];
     float ss = 0.f;
     uint32_t top = 0u;
     const int step = blockDim.x * VEC;
-    auto largest = [&](const float (&f)[VEC]) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) top = max(top, magnitude(f[e]));
-    };
     if constexpr (VPT > 0) {
+        // every load of the row is in flight before the first sum is stored
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int c = threadIdx.x * VEC + j * step;
-            if (c < a.K) row_values[j].fetch(a.src, row, a.K, c);
+            if (c < a.K) kept[j].fetch(a.src, row, a.K, c);
         }
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int c = threadIdx.x * VEC + j * step;
             if (c < a.K) {
-                row_values[j].combine(a.src, row, a.K, c, ss, true);
-                largest(row_values[j].v);
+                kept[j].combine(a.src, row, a.K, c, true);
+                kept[j].measure(a.src, c, top, ss);
             }
         }
     } else {
         for (int c = threadIdx.x * VEC; c < a.K; c += step) {
-            row_values[0].fetch(a.src, row, a.K, c);
-            row_values[0].combine(a.src, row, a.K, c, ss, true);
-            largest(row_values[0].v);
+            kept[0].fetch(a.src, row, a.K, c);
+            kept[0].combine(a.src, row, a.K, c, true);
+            kept[0].measure(a.src, c, top, ss);
         }
     }
     top = block_max(top, sh_top);
     float factor = 1.f;
-    if constexpr (SRC == SRC_NORM || SRC == SRC_ADD_NORM) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
+    if constexpr (HAS_NORM<SRC>) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
     const RowRound round(top);
     int8_t* q = a.q + row * a.ldq;
+    auto finish = [&](const Values<SRC, VEC>& r, int c) {
+        float v[VEC];
+        r.values(a.src, c, v);
+        store_ints<VEC>(q + c, round, v);
+    };
     if constexpr (VPT > 0) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int c = threadIdx.x * VEC + j * step;
-            if (c < a.K) store_ints<VEC>(q + c, round, row_values[j].v);
+            if (c < a.K) finish(kept[j], c);
         }
     } else {
         for (int c = threadIdx.x * VEC; c < a.K; c += step) {
-            float unused = 0.f;
-            row_values[0].fetch(a.src, row, a.K, c);
-            row_values[0].combine(a.src, row, a.K, c, unused, false);
-            store_ints<VEC>(q + c, round, row_values[0].v);
+            kept[0].fetch(a.src, row, a.K, c);
+            kept[0].combine(a.src, row, a.K, c, false);
+            finish(kept[0], c);
         }
     }
     for (int c = a.K + threadIdx.x; c < a.pad_to; c += blockDim.x) q[c] = 0;

@@ -1,5 +1,7 @@
-// What the kernels that round rows to 8-bit integers share: a row's values, and maxima and sums over a CTA.
+// What the kernels that round rows to 8-bit integers share: a row's values, the rounding, and maxima and sums over a CTA.
 #pragma once
+#include <type_traits>
+
 #include "row_ops.cuh"
 #include "w8a8.cuh"
 
@@ -7,35 +9,23 @@ namespace w8 {
 namespace {
 
 enum Source { SRC_PLAIN, SRC_NORM, SRC_ADD_NORM, SRC_F32 };
+template <Source S>
+constexpr bool HAS_NORM = S == SRC_NORM || S == SRC_ADD_NORM;
 
-// VEC elements of a row from column c on.  fetch() loads them, combine() makes of them what is rounded; apart, so that a thread's loads are
-// all in flight before the first residual sum is stored.
-template <Source SRC, int VEC>
-struct Values {
-    float v[VEC], d[SRC == SRC_ADD_NORM ? VEC : 1], w[SRC == SRC_NORM || SRC == SRC_ADD_NORM ? VEC : 1];
-    __device__ __forceinline__ void fetch(const RowSource& s, size_t row, int K, int c) {
-        if constexpr (SRC == SRC_F32) load_vec<VEC>(s.x32 + row * s.ldx + c, v);
-        else load_vec<VEC>(s.x + row * s.ldx + c, v);
-        if constexpr (SRC == SRC_ADD_NORM) load_vec<VEC>(s.delta + row * K + c, d);
-        if constexpr (SRC == SRC_NORM || SRC == SRC_ADD_NORM) load_vec<VEC>(s.norm + c, w);
-    }
-    // ss += the squares that a norm needs; `write`: stores the residual sum
-    __device__ __forceinline__ void combine(const RowSource& s, size_t row, int K, int c, float& ss, bool write) {
-        if constexpr (SRC == SRC_ADD_NORM) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = __bfloat162float(__float2bfloat16(fmaf(d[e], s.delta_scale, v[e])));
-            if (write) store_vec<VEC>(s.total + row * K + c, v);
-        }
-        if constexpr (SRC == SRC_NORM || SRC == SRC_ADD_NORM) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                ss = fmaf(v[e], v[e], ss);
-                v[e] *= w[e];
-            }
-        }
-    }
-};
+// whether 16-byte accesses fit the source
+inline bool rows_in_vectors(const RowSource& s, int K) {
+    auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+    return K % 8 == 0 && s.ldx % 8 == 0 && ((bits(s.x) | bits(s.x32) | bits(s.norm) | bits(s.delta) | bits(s.total)) & 15) == 0;
+}
 
+// ---------------------------------------------------------------- the largest magnitude
+// NaN, where there is one, stays
+__device__ __forceinline__ float max_magnitude(float top, float v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
+    return r;
+}
+// as a bit pattern: infinities and NaN are above all finite magnitudes
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* sh) {
     v = __reduce_max_sync(0xffffffffu, v);
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
@@ -51,23 +41,139 @@ __device__ __forceinline__ float block_total(float v, float* sh) {
     return warp_sum((threadIdx.x & 31) < (blockDim.x >> 5) ? sh[threadIdx.x & 31] : 0.f);
 }
 
+// ---------------------------------------------------------------- rounding
+// q = round(127 v / top) to nearest, even at ties, exactly.  v * k, k = 127 / top rounded, is off by less than 127 * 2^-23 from 127 v / top, so that
+// its nearest integer is the one, unless it lies within NEAR of the middle between two; a vector with such a value is rounded again by exact().
+// There v and top are scaled by a power of two so that nothing over- or underflows, an estimate is at most one off, and the rest
+// 127 v - q top, which fp32 holds exactly for v of up to 17 significant bits (bf16 values and products of two of them), decides.  (Rows of
+// fp32 values round the middle as their fp32 rests have it.)
+struct RowRound {
+    float k, c127, top, inv;
+    bool finite, plain;   // plain: k is exact enough; not for rows of tiny values
+    static constexpr float MAGIC = 12582912.f;       // 1.5 * 2^23: v + MAGIC has round(v) in its low byte
+    static constexpr float NEAR = 0.49996f;
+    __device__ __forceinline__ explicit RowRound(uint32_t bits) {
+        finite = bits < 0x7f800000u;
+        plain = finite && bits >= 0x10000000u;                   // 2^-95
+        const float v = __uint_as_float(bits);
+        k = plain ? 127.f / v : 0.f;
+        int e = static_cast<int>(bits >> 23) - 127;              // v is in [2^e, 2^(e+1)), or below where it is subnormal
+        e = e < -119 ? -119 : e;
+        const float c = __uint_as_float(static_cast<uint32_t>(127 - (e > 126 ? 126 : e)) << 23);
+        const bool some = finite && bits != 0u;
+        c127 = some ? 127.f * c : 0.f;
+        top = v * c;
+        inv = some ? 1.f / top : 0.f;
+    }
+    __device__ __forceinline__ int exact(float v) const {
+        const float p = v * c127;
+        float r = rintf(p * inv);
+        const float rest = fmaf(-r, top, p);
+        const float twice = 2.f * fabsf(rest);
+        if (twice > top || (twice == top && (static_cast<int>(r) & 1))) r += copysignf(1.f, rest);
+        return static_cast<int>(r);
+    }
+    // four values to four bytes; near: largest distance from an integer so far
+    __device__ __forceinline__ uint32_t four(const float* v, float& near) const {
+        uint32_t y[4];
+        const f32x2 kk = pair(k, k), magic = pair(MAGIC, MAGIC), minus = pair(-1.f, -1.f);
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const f32x2 x = pair(v[i], v[i + 1]);
+            const f32x2 sum = fma2(x, kk, magic);
+            const float2 off = unpair(fma2(x, kk, fma2(sum, minus, magic)));   // v k - round(v k)
+            near = fmaxf(near, fmaxf(fabsf(off.x), fabsf(off.y)));
+            const float2 f = unpair(sum);
+            y[i] = __float_as_uint(f.x);
+            y[i + 1] = __float_as_uint(f.y);
+        }
+        return __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
+    }
+    // the row's scale: NaN for a row with an infinity or a NaN, so that its outputs are NaN
+    __device__ __forceinline__ static float scale(uint32_t bits, float factor) {
+        return bits < 0x7f800000u ? __uint_as_float(bits) / 127.f * factor : __uint_as_float(0x7fffffffu);
+    }
+};
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
+}
+
 template <int VEC>
 __device__ __forceinline__ void store_ints(int8_t* q, const RowRound& round, const float (&v)[VEC]) {
     if constexpr (VEC == 8) {
         uint2 w = make_uint2(0u, 0u);
-        if (round.finite) w = make_uint2(pack4(round(v[0]), round(v[1]), round(v[2]), round(v[3])), pack4(round(v[4]), round(v[5]), round(v[6]), round(v[7])));
+        float near = 0.f;
+        if (round.plain) w = make_uint2(round.four(v, near), round.four(v + 4, near));
+        if (round.finite && (near > RowRound::NEAR || !round.plain)) {
+            w = make_uint2(pack4(round.exact(v[0]), round.exact(v[1]), round.exact(v[2]), round.exact(v[3])),
+                           pack4(round.exact(v[4]), round.exact(v[5]), round.exact(v[6]), round.exact(v[7])));
+        }
         *reinterpret_cast<uint2*>(q) = w;
     } else {
-        *q = static_cast<int8_t>(round.finite ? round(v[0]) : 0);
+        *q = static_cast<int8_t>(round.finite ? round.exact(v[0]) : 0);
     }
 }
 
-// whether 16-byte accesses fit the source
-inline bool rows_in_vectors(const RowSource& s, int K) {
-    auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
-    return K % 8 == 0 && s.ldx % 8 == 0 && ((bits(s.x) | bits(s.x32) | bits(s.norm) | bits(s.delta) | bits(s.total)) & 15) == 0;
-}
-__device__ __forceinline__ int ceil_div_dev(int a, int b) { return (a + b - 1) / b; }
+// ---------------------------------------------------------------- VEC consecutive elements of a row
+// kept as they came (t: bf16 pairs, or fp32), because a row waits for its maximum in registers
+template <Source SRC, int VEC>
+struct Values {
+    using T = typename std::conditional<SRC == SRC_F32, float, bf16>::type;
+    struct alignas(VEC == 8 ? 16 : sizeof(T)) Block { T e[VEC]; };
+    Block t, d;
+    __device__ __forceinline__ static const T* base(const RowSource& s) {
+        if constexpr (SRC == SRC_F32) return s.x32;
+        else return s.x;
+    }
+    __device__ __forceinline__ void fetch(const RowSource& s, size_t row, int K, int c) {
+        t = *reinterpret_cast<const Block*>(base(s) + row * s.ldx + c);
+        if constexpr (SRC == SRC_ADD_NORM) d = *reinterpret_cast<const Block*>(s.delta + row * K + c);
+    }
+    // the residual sum, in place of x; `write`: stores it
+    __device__ __forceinline__ void combine(const RowSource& s, size_t row, int K, int c, bool write) {
+        if constexpr (SRC == SRC_ADD_NORM) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) t.e[e] = __float2bfloat16(fmaf(__bfloat162float(d.e[e]), s.delta_scale, __bfloat162float(t.e[e])));
+            if (write) *reinterpret_cast<Block*>(s.total + row * K + c) = t;
+        }
+    }
+    // what is rounded
+    __device__ __forceinline__ void values(const RowSource& s, int c, float (&v)[VEC]) const {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = to_float(t.e[e]);
+        if constexpr (HAS_NORM<SRC>) {
+            float w[VEC];
+            load_vec<VEC>(s.norm + c, w);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] *= w[e];
+        }
+    }
+    // the largest magnitude of values(), and the squares that a norm needs
+    __device__ __forceinline__ void measure(const RowSource& s, int c, uint32_t& top, float& ss) const {
+        if constexpr (SRC == SRC_PLAIN && VEC == 8) {   // two magnitudes at a time, as 16-bit patterns
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(t.e);
+            uint32_t m = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            top = max(top, max(m << 16, m & 0xffff0000u));
+        } else {
+            float v[VEC];
+            values(s, c, v);
+            float m = 0.f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m = max_magnitude(m, v[e]);
+            top = max(top, __float_as_uint(m));
+            if constexpr (HAS_NORM<SRC>) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float f = to_float(t.e[e]);
+                    ss = fmaf(f, f, ss);
+                }
+            }
+        }
+    }
+};
 
 }  // namespace
 }  // namespace w8

@@ -477,21 +477,14 @@ int cpmcu_accept_fixup(int tree_size, int32_t* pred, const int32_t* gt, const in
 int cpmcu_stream_check(void* stream);
 
 /* Linear layers in 8-bit integers (weights and activations).
- *   v = x, or v = t * weight with t = bf16(x + delta_scale * delta) and the factor f = 1 / sqrt(mean(t^2) + eps)   (f = 1 without a norm)
+ *   v = x, or with norm [K] (bf16, may be NULL) v = t * norm, the factor f = 1 / sqrt(mean(t^2) + eps)   (f = 1 without a norm)
+ *   t = x, or with delta [rows, K] (bf16, may be NULL) t = bf16(x + delta_scale * delta), which goes to total [rows, K], apart from x
  *   q = round(127 v / max|v|) (to even at ties),  s = max|v| / 127 * f            one scale for each row
  *   y[m][n] = (sum over k of q[m][k] W[n][k]) * s[m] * S[n] + bias[n]             exact sums, rounded once, to bf16
  * A row with an infinity or a NaN gives NaN, a row of zeros the bias.  K <= 131072 (sums of 32 bits).
  *
  * Packed weights are written once, by cpmcu_w8a8_pack, and are read before the launch waits for its predecessor in the stream: write them with that
  * call or with a copy, and not by a kernel of your own that lets its successor start early. */
-typedef struct {
-    const void* weight;   /* [K] bf16 */
-    float eps;
-    const void* delta;    /* [rows, K] bf16, or NULL */
-    float delta_scale;
-    void* total;          /* [rows, K] bf16: receives t; given with a delta, and apart from x */
-} cpmcu_w8a8_norm;
-
 /* Bytes of packed weights [N, K] (gated: of N gate rows and N up rows), 256-byte aligned. */
 long cpmcu_w8a8_packed_bytes(int N, int K, int gated);
 /* q [N, K] int8 row-major, scale [N] fp32.  part 0: a matrix of its own; 1 and 2: the gate and the up rows of one gated buffer. */
@@ -500,12 +493,12 @@ int cpmcu_w8a8_pack(const void* q, const float* scale, int N, int K, int part, v
 int cpmcu_w8a8_quantize(const void* x, long long ldx, int rows, int K, void* q, float* scale, void* stream);
 /* Bytes of the workspace of a linear layer (inter 0), or of a feed-forward block (N = K = its width); 256-byte aligned. */
 long cpmcu_w8a8_workspace_bytes(int rows, int N, int K, int inter);
-/* y [rows, N], rows ldy apart; x [rows, K], rows ldx apart; bias [N] bf16 or NULL; norm or NULL (HOST struct). */
-int cpmcu_w8a8_linear(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, const void* packed, const void* bias, void* y, long long ldy,
-                      int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream);
+/* y [rows, N], rows ldy apart; x [rows, K], rows ldx apart; bias [N] bf16 or NULL. */
+int cpmcu_w8a8_linear(const void* x, long long ldx, const void* packed, const void* bias, const void* norm, float eps, const void* delta,
+                      float delta_scale, void* total, void* y, long long ldy, int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream);
 /* y = down(silu(gate(v)) * up(v)), all three as above; the activations in between are fp32 until they become 8-bit integers. */
-int cpmcu_w8a8_ffn(const void* x, long long ldx, const cpmcu_w8a8_norm* norm, const void* gate_up, const void* down, void* y, long long ldy, int rows,
-                   int K, int inter, void* workspace, long long workspace_bytes, void* stream);
+int cpmcu_w8a8_ffn(const void* x, long long ldx, const void* gate_up, const void* down, const void* norm, float eps, const void* delta,
+                   float delta_scale, void* total, void* y, long long ldy, int rows, int K, int inter, void* workspace, long long workspace_bytes, void* stream);
 
 /* Rotary positions for rows of fused queries, keys and values, and their append to a cache.  qkv [rows, (heads + 2 kv_heads) * dim] bf16, rows ld
  * apart.  The first rot_dims elements of every query and key head turn, pair i by pos[row] * inv_freq[i] (angles of 64 bits), with
