@@ -25,7 +25,12 @@ namespace w8 {
 namespace {
 
 constexpr int UMMA_K = 32;
-constexpr int NUM_THREADS = 192;   // warp 0 TMA, warp 1 MMA + TMEM, warps 2-5 epilogue
+// Warp 0 TMA, warp 1 MMA + TMEM, then the epilogue.  Two warps for each quarter of the tensor memory's lanes take turns with the tokens: one alone on
+// its scheduler waits for its own instructions most of the time, and a gate/up tile of 256 tokens took 27000 cycles beside 16400 of products at K = 4096.
+constexpr int EPI_WARPS = 8;
+constexpr int NUM_THREADS = 64 + EPI_WARPS * 32;
+constexpr int CLUSTER_THREADS = 192;   // of the cluster kernel, whose epilogue is short
+constexpr int XCH_BYTES = EPI_WARPS * gemm::EPI_WARP_BYTES;
 constexpr int CTRL_BYTES = 256;
 
 struct ProductArgs {
@@ -78,8 +83,8 @@ struct Cfg {
     static constexpr int STAGE_BYTES = BLOCK_BYTES + X_ROWS * BLOCK_COLS;
     static constexpr int STAGES = PAIR ? 6 : (MT <= 16) ? 10 : (MT <= 32) ? 9 : (MT <= 64) ? 8 : (MT <= 128) ? 6 : 4;
     static constexpr int TMEM_COLS = 2 * MT;
-    static constexpr int SCALE_BYTES = 4 * MT * 4;              // per epilogue warp the token scales of its tile
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CTRL_BYTES + gemm::EPI_XCH_BYTES + SCALE_BYTES + 1024;
+    static constexpr int SCALE_BYTES = EPI_WARPS * MT * 4;      // per epilogue warp the token scales of its tile
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CTRL_BYTES + XCH_BYTES + SCALE_BYTES + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
@@ -105,52 +110,60 @@ __device__ __forceinline__ void store16(bf16* y, long long ldy, int N, long long
 }
 
 // silu(gate) * up of a whole tile: lanes 0-63 hold the gate sums of 64 features, 64-127 the up sums of the same ones.  Warps q and q + 2 hand
-// each other half of the tokens of a batch, scaled, so that all four compute.  fp32: what is rounded next is the row of 8-bit integers.
+// each other the sums of half of the tokens of a batch, so that both compute.  fp32: what is rounded next is the row of 8-bit integers.
 template <int MT>
-__device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act, long long ld, int N, long long row0, int n0, const float* xs, float ws,
-                                          float* xch, int q, int lane) {
+__device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act, long long ld, int N, long long row0, int n0, const float* xs, float ws_gate,
+                                          float ws_up, float* xch, int q, int half, int lane) {
     constexpr int HB = MT >= 32 ? 16 : 8;
-    float* out = xch + q * (gemm::EPI_WARP_BYTES / 4);
-    const float* in = xch + (q ^ 2) * (gemm::EPI_WARP_BYTES / 4);
-    const int pair_bar = 2 + (q & 1);
+    int* out = reinterpret_cast<int*>(xch) + (half * 4 + q) * (gemm::EPI_WARP_BYTES / 4) + lane;
+    const int* in = reinterpret_cast<const int*>(xch) + (half * 4 + (q ^ 2)) * (gemm::EPI_WARP_BYTES / 4) + lane;
+    const int pair_bar = 2 + half * 2 + (q & 1);
     const bool gates = q < 2;
+    const bool column = n0 + lane < N;
 #pragma unroll 1
-    for (int c0 = 0; c0 < m_cnt; c0 += 2 * HB) {   // uniform across the CTA
+    for (int c0 = half * 2 * HB; c0 < m_cnt; c0 += 4 * HB) {   // uniform across the warps of a half
         uint32_t r[2 * HB];
         ptx::tmem_ld16(t_addr + c0, r);
         if constexpr (HB == 16) ptx::tmem_ld16(t_addr + c0 + 16, r + 16);
         ptx::tmem_wait_ld();
-        float mine[HB];
         // gate warps keep the first half of the tokens, up warps the second
 #pragma unroll
-        for (int c = 0; c < HB; ++c) {
-            const float lo = static_cast<float>(static_cast<int>(r[c])) * xs[c0 + c] * ws, hi = static_cast<float>(static_cast<int>(r[HB + c])) * xs[c0 + HB + c] * ws;
-            out[c * 32 + lane] = gates ? hi : lo;
-            mine[c] = gates ? lo : hi;
-        }
+        for (int c = 0; c < HB; ++c) out[c * 32] = static_cast<int>(gates ? r[HB + c] : r[c]);
         ptx::named_bar_sync(pair_bar, 64);
         const int first = c0 + (gates ? 0 : HB);
-        float* dst = act + (row0 + first) * ld + n0 + lane;
+        float v[HB];
 #pragma unroll
-        for (int c = 0; c < HB; ++c) {
-            const float other = in[c * 32 + lane];
-            const float v = silu_fast(gates ? mine[c] : other) * (gates ? other : mine[c]);
-            if (first + c < m_cnt && n0 + lane < N) dst[c * ld] = v;
+        for (int c = 0; c < HB; c += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(xs + first + c);
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int mine = static_cast<int>(gates ? r[c + e] : r[HB + c + e]), other = in[(c + e) * 32];
+                const float g = static_cast<float>(gates ? mine : other) * s[e] * ws_gate, u = static_cast<float>(gates ? other : mine) * s[e] * ws_up;
+                v[c + e] = silu_fast(g) * u;
+            }
+        }
+        float* dst = act + (row0 + first) * ld + n0 + lane;
+        if (column) {
+#pragma unroll
+            for (int c = 0; c < HB; ++c, dst += ld) {
+                if (first + c < m_cnt) *dst = v[c];
+            }
         }
         ptx::named_bar_sync(pair_bar, 64);   // the partner may write `in` again
     }
 }
 
-// The 128 epilogue threads of one CTA walk the segments of `it`; rank: of a pair's CTA, which has 128 of the tile's 256 weight rows.
+// The epilogue threads of one CTA walk the segments of `it`; rank: of a pair's CTA, which has 128 of the tile's 256 weight rows.
 template <int MT, bool PAIR>
 __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint32_t tmem_base, uint64_t* acc_full, uint64_t* acc_empty,
                                          volatile int* abort_flag, volatile int* s_last, int warp, int lane, int epi_tid, int g, int G, float* xch,
                                          float* scales, int rank) {
     constexpr int CSZ = PAIR ? 2 : 1;
     const gemm::LinearArgs& w = a.sched;
-    const int q = warp & 3, row = q * 32 + lane;
-    uint8_t* buf = reinterpret_cast<uint8_t*>(xch) + q * gemm::EPI_WARP_BYTES;
-    float* xs = scales + q * MT;
+    const int q = warp & 3, row = q * 32 + lane, half = (warp - 2) >> 2;   // batches of tokens alternate between the halves
+    uint8_t* buf = reinterpret_cast<uint8_t*>(xch) + (half * 4 + q) * gemm::EPI_WARP_BYTES;
+    float* xs = scales + (half * 4 + q) * MT;
     const bool vec = a.act == nullptr && ((reinterpret_cast<uintptr_t>(a.y) | (static_cast<uintptr_t>(a.ldy) * 2) | (static_cast<uintptr_t>(a.N) * 2)) & 15) == 0;
     const int gt = w.tail_grid > 0 ? w.tail_grid : G;
     int acc = 0;
@@ -164,7 +177,8 @@ __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint3
         const int m_cnt = min(w.M - m_base, MT);
         // scales of the tokens and of this feature, while the sums are being made
         for (int t = lane; t < MT; t += 32) xs[t] = t < m_cnt ? a.xs[m_base + t] : 0.f;
-        const float ws = a.ws[n_tile * TILE_ROWS + row];
+        const float ws = a.ws[n_tile * TILE_ROWS + (a.act == nullptr ? row : row & 63)];             // gate/up tiles: of the gate
+        const float ws_up = a.act == nullptr ? 0.f : a.ws[n_tile * TILE_ROWS + 64 + (row & 63)];
         __syncwarp();
         if (!ptx::mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag)) break;
         ptx::tc_fence_after();
@@ -179,11 +193,11 @@ __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint3
             pieces = gemm::unit_owner(u0 + w.kblocks - 1, w.total_units, gt) - first + 1;
         }
         if (a.act != nullptr) {
-            gate_tile<MT>(t_addr, m_cnt, a.act, a.ldy, a.N, m_base, n_tile * 64 + (q & 1) * 32, xs, ws, xch, q, lane);
+            gate_tile<MT>(t_addr, m_cnt, a.act, a.ldy, a.N, m_base, n_tile * 64 + (q & 1) * 32, xs, ws, ws_up, xch, q, half, lane);
         } else if (whole) {
             const float bias = a.bias != nullptr && n0 + lane < a.N ? __bfloat162float(a.bias[n0 + lane]) : 0.f;
 #pragma unroll 1
-            for (int c0 = 0; c0 < m_cnt; c0 += 16) {
+            for (int c0 = half * 16; c0 < m_cnt; c0 += 32) {
                 int r[16];
                 float v[16];
                 load16(t_addr + c0, r);
@@ -193,7 +207,7 @@ __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint3
             }
         } else {
 #pragma unroll 1
-            for (int c0 = 0; c0 < m_cnt; c0 += 16) {
+            for (int c0 = half * 16; c0 < m_cnt; c0 += 32) {
                 int r[16];
                 load16(t_addr + c0, r);
                 ptx::tmem_wait_ld();
@@ -211,16 +225,16 @@ __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint3
 
         if (!whole) {
             __threadfence();   // this thread's sums are visible before the count
-            ptx::named_bar_sync(1, 128);
+            ptx::named_bar_sync(1, EPI_WARPS * 32);
             if (epi_tid == 0) *s_last = atomicAdd(&a.tickets[tile * CSZ + rank], 1) == pieces - 1;
-            ptx::named_bar_sync(1, 128);
+            ptx::named_bar_sync(1, EPI_WARPS * 32);
             const bool last = *s_last != 0;
-            ptx::named_bar_sync(1, 128);   // everyone has read s_last before it can change
+            ptx::named_bar_sync(1, EPI_WARPS * 32);   // everyone has read s_last before it can change
             if (last) {
                 __threadfence();
                 const float bias = a.bias != nullptr && n0 + lane < a.N ? __bfloat162float(a.bias[n0 + lane]) : 0.f;
 #pragma unroll 1
-                for (int c0 = 0; c0 < m_cnt; c0 += 16) {
+                for (int c0 = half * 16; c0 < m_cnt; c0 += 32) {
                     int sum[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) sum[c] = 0;
@@ -266,7 +280,7 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* s_last = abort_flag + 1;
     float* xch = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + CTRL_BYTES);
-    float* scales = xch + gemm::EPI_XCH_BYTES / 4;
+    float* scales = xch + XCH_BYTES / 4;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? static_cast<int>(ptx::cluster_ctarank()) : 0;
@@ -281,7 +295,7 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         }
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(&acc_full[s], 1);
-            ptx::mbar_init(&acc_empty[s], CSZ * 128);
+            ptx::mbar_init(&acc_empty[s], CSZ * EPI_WARPS * 32);
         }
         *abort_flag = 0;
         *s_last = 0;
@@ -418,7 +432,7 @@ struct ClusterCfg {
 };
 
 template <int MT, int CS>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(CLUSTER_THREADS, 1)
 product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const ProductArgs a) {
     using C = ClusterCfg<MT, CS>;
     extern __shared__ uint8_t smem_raw[];
@@ -595,7 +609,7 @@ void run_cluster(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs
     using C = ClusterCfg<MT, CS>;
     static const bool allowed = allow_smem(product_s8_cluster_kernel<MT, CS>, C::SMEM_BYTES);
     (void)allowed;
-    launch(product_s8_cluster_kernel<MT, CS>, grid, NUM_THREADS, C::SMEM_BYTES, s, CS, true, tw, tx, a);
+    launch(product_s8_cluster_kernel<MT, CS>, grid, CLUSTER_THREADS, C::SMEM_BYTES, s, CS, true, tw, tx, a);
 }
 template <int MT>
 void run_cluster(int cs, const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
@@ -607,7 +621,7 @@ template <int MT, int CS>
 int capacity_of() {
     static const int n = [] {
         allow_smem(product_s8_cluster_kernel<MT, CS>, ClusterCfg<MT, CS>::SMEM_BYTES);
-        return max_active_clusters(product_s8_cluster_kernel<MT, CS>, dim3(NUM_THREADS), ClusterCfg<MT, CS>::SMEM_BYTES, CS);
+        return max_active_clusters(product_s8_cluster_kernel<MT, CS>, dim3(CLUSTER_THREADS), ClusterCfg<MT, CS>::SMEM_BYTES, CS);
     }();
     return n;
 }

@@ -1,7 +1,7 @@
 // One row of an 8-bit linear layer, sm_100a:  y[N] = (q . W_n) * scale * scale_n + bias_n, with q made of the row inside the launch (w8a8_rows.cuh).
 //
 // Bound: the weights' bytes from HBM.  One CTA of 16 warps per SM makes the integers of the row once, in shared memory.  Weights come through
-// asynchronous 16-byte copies into slots of shared memory that one lane writes and reads (no barriers): 80 KB per SM are in flight, the first of
+// asynchronous 16-byte copies into slots of shared memory that one lane writes and reads (no barriers): 96 KB per SM are in flight, the first of
 // them before the wait for the predecessor and while the integers are made, and no registers hold them, so that the next launch's CTAs fit
 // beside this one's and its weights are on their way before this one ends.  Eight lanes read 128 consecutive bytes of one weight row, a
 // warp four rows (512 bytes) per k-block; S warps share the k-blocks of a group of rows and meet in shared memory, S chosen so
@@ -16,15 +16,16 @@ namespace w8 {
 namespace {
 
 constexpr int WARPS = 16, THREADS = WARPS * 32;
-constexpr int SLOTS = 10;                             // 16-byte copies per lane in flight
+constexpr int SLOTS = 12;                             // 16-byte copies per lane in flight
+constexpr int STEP = 2;                               // k-blocks per step
 constexpr int RING_BYTES = SLOTS * THREADS * 16;
-constexpr int KEEP = 4;                               // vectors of 8 that a thread keeps of the row
-constexpr int MAX_SMEM = RING_BYTES + MAX_COLS;
+constexpr int MAX_SMEM = RING_BYTES + MAX_COLS + STEP * BLOCK_COLS;
 
 struct OneRowArgs {
     RowSource src;
     Packed w;
     int N, K, share, units, rounds;   // share: warps per group of rows; units: groups of 4 (gated: 4 + 4) rows
+    int steps;                        // of a warp in a round
     const bf16* bias;
     bf16* y;
     float* act;
@@ -41,7 +42,8 @@ __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
 template <Source SRC, int VEC, bool GATED>
 __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs a) {
     constexpr int SETS = GATED ? 2 : 1;               // gate and up rows of the same features
-    constexpr int DEPTH = SLOTS / SETS;               // steps in flight
+    constexpr int PER_STEP = STEP * SETS, DEPTH = SLOTS / PER_STEP;   // copies of a lane; steps in flight
+    constexpr int KEEP = HAS_NORM<SRC> ? 2 : 4;       // vectors that a thread keeps of the row
     constexpr int TILE_UNITS = (GATED ? TILE_ROWS / 2 : TILE_ROWS) / 4;
     extern __shared__ __align__(16) uint8_t smem[];   // ring, then the integers
     __shared__ uint32_t sh_top[32];
@@ -52,34 +54,39 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
     const int kblocks = a.w.kblocks;
     uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;
 
-    // ---- copies: steps (round, k-block) in the order of their use; a step's place in the ring is its number modulo DEPTH
-    int load_round = 0, load_kb = ks, load_at = 0;
-    const uint8_t* load_from = nullptr;
+    // ---- copies: steps in the order of their use.  Every warp has the same number of them in every round; what a step has no weights for is zeros.
     auto unit_of = [&](int round) { return (blockIdx.x + round * gridDim.x) * slots + slot; };
-    auto seek = [&]() {   // first bytes of this lane in the unit of load_round; null behind the last unit
+    const size_t stride = static_cast<size_t>(a.share) * STEP * BLOCK_BYTES;
+    int load_round = 0, load_step = 0, load_at = 0, load_kb = 0;
+    const uint8_t* load_from = a.w.blocks;
+    auto seek = [&]() {
         const int unit = unit_of(load_round);
-        load_from = load_round < a.rounds && unit < a.units ? a.w.blocks + static_cast<size_t>(unit / TILE_UNITS) * kblocks * BLOCK_BYTES +
-                                                                  ((unit % TILE_UNITS) * 4 + (lane >> 3)) * BLOCK_COLS + (lane & 7) * 16
-                                                            : nullptr;
+        const bool there = load_round < a.rounds && unit < a.units;
+        load_kb = there ? ks * STEP : kblocks;
+        load_from = a.w.blocks;
+        if (there) load_from += (static_cast<size_t>(unit / TILE_UNITS) * kblocks + load_kb) * BLOCK_BYTES + ((unit % TILE_UNITS) * 4 + (lane >> 3)) * BLOCK_COLS + (lane & 7) * 16;
     };
     auto issue = [&]() {
-        if (load_kb >= kblocks && load_round < a.rounds) {
-            ++load_round;
-            load_kb = ks;
-            seek();
-        }
-        if (load_from != nullptr && load_kb < kblocks) {
+#pragma unroll
+        for (int u = 0; u < STEP; ++u) {
+            const int bytes = load_kb + u < kblocks ? 16 : 0;   // 0: nothing is read
 #pragma unroll
             for (int g = 0; g < SETS; ++g) {
-                ptx::cp_async16(ring + (load_at * SETS + g) * THREADS, load_from + static_cast<size_t>(load_kb) * BLOCK_BYTES + g * (TILE_ROWS / 2) * BLOCK_COLS, 16);
+                ptx::cp_async16(ring + (load_at * PER_STEP + u * SETS + g) * THREADS, load_from + u * BLOCK_BYTES + g * (TILE_ROWS / 2) * BLOCK_COLS, bytes);
             }
         }
-        ptx::cp_async_commit();   // empty groups keep the count
-        load_kb += a.share;
+        ptx::cp_async_commit();
+        load_kb += a.share * STEP;
+        load_from += stride;
         load_at = load_at + 1 == DEPTH ? 0 : load_at + 1;
+        if (++load_step == a.steps) {
+            load_step = 0;
+            ++load_round;
+            seek();
+        }
     };
     seek();
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < DEPTH; ++i) issue();
     grid_dep_wait();
     grid_dep_trigger();
@@ -99,14 +106,14 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
         const int c = (threadIdx.x + j * THREADS) * VEC;
         if (c < a.K) {
             kept[j].combine(a.src, 0, a.K, c, blockIdx.x == 0);
-            kept[j].measure(a.src, c, top, ss);
+            kept[j].measure(top, ss);
         }
     }
     for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {   // of longer rows: read again below
         Values<SRC, VEC> r;
         r.fetch(a.src, 0, a.K, c);
         r.combine(a.src, 0, a.K, c, blockIdx.x == 0);
-        r.measure(a.src, c, top, ss);
+        r.measure(top, ss);
     }
     top = block_max(top, sh_top);
     float factor = 1.f;
@@ -117,7 +124,7 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
         const int c = (threadIdx.x + j * THREADS) * VEC;
         if (c < a.K) {
             float v[VEC];
-            kept[j].values(a.src, c, v);
+            kept[j].values(v);
             store_ints<VEC>(q + c, round8, v);
         }
     }
@@ -126,10 +133,10 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
         float v[VEC];
         r.fetch(a.src, 0, a.K, c);
         r.combine(a.src, 0, a.K, c, false);
-        r.values(a.src, c, v);
+        r.values(v);
         store_ints<VEC>(q + c, round8, v);
     }
-    for (int c = a.K + threadIdx.x; c < kblocks * BLOCK_COLS; c += THREADS) q[c] = 0;
+    for (int c = a.K + threadIdx.x; c < (kblocks + STEP - 1) / STEP * STEP * BLOCK_COLS; c += THREADS) q[c] = 0;
     const float scale = RowRound::scale(top, factor);
     __syncthreads();
 
@@ -149,13 +156,20 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
         int acc[SETS];
 #pragma unroll
         for (int g = 0; g < SETS; ++g) acc[g] = 0;
-        for (int kb = ks; kb < kblocks; kb += a.share) {
+        const int8_t* x_at = q + ks * STEP * BLOCK_COLS + (lane & 7) * 16;
+#pragma unroll 1
+        for (int step = 0; step < a.steps; ++step) {
             ptx::cp_async_wait<DEPTH - 1>();
-            if (unit < a.units) {
-                const uint4 x = *reinterpret_cast<const uint4*>(q + kb * BLOCK_COLS + (lane & 7) * 16);
+            // steps behind the last k-block have zeros for weights; what they find for x does not matter, but has to be there
+            const bool inside = (step * a.share + ks) * STEP < kblocks;
+            uint4 x[STEP], wv[PER_STEP];
 #pragma unroll
-                for (int g = 0; g < SETS; ++g) acc[g] = dot16(ring[(at * SETS + g) * THREADS], x, acc[g]);
-            }
+            for (int u = 0; u < STEP; ++u) x[u] = *reinterpret_cast<const uint4*>((inside ? x_at : q) + u * BLOCK_COLS);
+#pragma unroll
+            for (int i = 0; i < PER_STEP; ++i) wv[i] = ring[(at * PER_STEP + i) * THREADS];
+#pragma unroll
+            for (int i = 0; i < PER_STEP; ++i) acc[i % SETS] = dot16(wv[i], x[i / SETS], acc[i % SETS]);
+            x_at += a.share * STEP * BLOCK_COLS;
             at = at + 1 == DEPTH ? 0 : at + 1;
             issue();
         }
@@ -215,20 +229,21 @@ void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const b
     a.N = N; a.K = K;
     a.bias = bias; a.y = y; a.act = act;
     a.units = w.tiles * (gated ? 16 : 32);
-    // Warps per group: the fewest steps of the busiest warp, with half a step for each round's meeting
-    const int sms = runtime().num_sms;
+    // Warps per group: the fewest steps of a warp, with half a step for each round's meeting
+    const int sms = runtime().num_sms, pairs = ceil_div(w.kblocks, STEP);
     long long best = -1;
     for (int share = 1; share <= WARPS; share *= 2) {
-        const int rounds = ceil_div(ceil_div(a.units, WARPS / share), sms);
-        const long long cost = static_cast<long long>(rounds) * (2 * ceil_div(w.kblocks, share) + (share > 1 ? 1 : 0));
+        const int rounds = ceil_div(ceil_div(a.units, WARPS / share), sms), steps = ceil_div(pairs, share);
+        const long long cost = static_cast<long long>(rounds) * (2 * steps + (share > 1 ? 1 : 0));
         if (best < 0 || cost < best) {
             best = cost;
             a.share = share;
             a.rounds = rounds;
+            a.steps = steps;
         }
     }
     const int grid = std::min(sms, ceil_div(a.units, WARPS / a.share));
-    const size_t smem = RING_BYTES + static_cast<size_t>(w.kblocks) * BLOCK_COLS;
+    const size_t smem = RING_BYTES + static_cast<size_t>(pairs) * STEP * BLOCK_COLS;
     const bool vec = rows_in_vectors(src, K);
     if (src.x32 != nullptr) run<SRC_F32, false>(a, grid, smem, vec, s);
     else if (src.norm == nullptr) gated ? run<SRC_PLAIN, true>(a, grid, smem, vec, s) : run<SRC_PLAIN, false>(a, grid, smem, vec, s);

@@ -48,14 +48,14 @@ __global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const Qua
             const int c = threadIdx.x * VEC + j * step;
             if (c < a.K) {
                 kept[j].combine(a.src, row, a.K, c, true);
-                kept[j].measure(a.src, c, top, ss);
+                kept[j].measure(top, ss);
             }
         }
     } else {
         for (int c = threadIdx.x * VEC; c < a.K; c += step) {
             kept[0].fetch(a.src, row, a.K, c);
             kept[0].combine(a.src, row, a.K, c, true);
-            kept[0].measure(a.src, c, top, ss);
+            kept[0].measure(top, ss);
         }
     }
     top = block_max(top, sh_top);
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const Qua
     int8_t* q = a.q + row * a.ldq;
     auto finish = [&](const Values<SRC, VEC>& r, int c) {
         float v[VEC];
-        r.values(a.src, c, v);
+        r.values(v);
         store_ints<VEC>(q + c, round, v);
     };
     if constexpr (VPT > 0) {

@@ -121,7 +121,7 @@ template <Source SRC, int VEC>
 struct Values {
     using T = typename std::conditional<SRC == SRC_F32, float, bf16>::type;
     struct alignas(VEC == 8 ? 16 : sizeof(T)) Block { T e[VEC]; };
-    Block t, d;
+    Block t, d, w;
     __device__ __forceinline__ static const T* base(const RowSource& s) {
         if constexpr (SRC == SRC_F32) return s.x32;
         else return s.x;
@@ -129,6 +129,7 @@ struct Values {
     __device__ __forceinline__ void fetch(const RowSource& s, size_t row, int K, int c) {
         t = *reinterpret_cast<const Block*>(base(s) + row * s.ldx + c);
         if constexpr (SRC == SRC_ADD_NORM) d = *reinterpret_cast<const Block*>(s.delta + row * K + c);
+        if constexpr (HAS_NORM<SRC>) w = *reinterpret_cast<const Block*>(s.norm + c);
     }
     // the residual sum, in place of x; `write`: stores it
     __device__ __forceinline__ void combine(const RowSource& s, size_t row, int K, int c, bool write) {
@@ -139,18 +140,15 @@ struct Values {
         }
     }
     // what is rounded
-    __device__ __forceinline__ void values(const RowSource& s, int c, float (&v)[VEC]) const {
+    __device__ __forceinline__ void values(float (&v)[VEC]) const {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = to_float(t.e[e]);
-        if constexpr (HAS_NORM<SRC>) {
-            float w[VEC];
-            load_vec<VEC>(s.norm + c, w);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] *= w[e];
+        for (int e = 0; e < VEC; ++e) {
+            v[e] = to_float(t.e[e]);
+            if constexpr (HAS_NORM<SRC>) v[e] *= to_float(w.e[e]);
         }
     }
     // the largest magnitude of values(), and the squares that a norm needs
-    __device__ __forceinline__ void measure(const RowSource& s, int c, uint32_t& top, float& ss) const {
+    __device__ __forceinline__ void measure(uint32_t& top, float& ss) const {
         if constexpr (SRC == SRC_PLAIN && VEC == 8) {   // two magnitudes at a time, as 16-bit patterns
             const uint32_t* w = reinterpret_cast<const uint32_t*>(t.e);
             uint32_t m = 0u;
@@ -159,7 +157,7 @@ struct Values {
             top = max(top, max(m << 16, m & 0xffff0000u));
         } else {
             float v[VEC];
-            values(s, c, v);
+            values(v);
             float m = 0.f;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) m = max_magnitude(m, v[e]);
