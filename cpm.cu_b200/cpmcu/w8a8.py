@@ -42,11 +42,10 @@ def _ld(t):
 def _call(name, device, *args):
     """The entry point on torch's current stream of `device`."""
     i = device.index
-    if i == _current_device():
-        C.call(name, *args, _raw_stream(i))
-        return
-    with torch.cuda.device(device):
-        C.call(name, *args, _raw_stream(i))
+    if i != _current_device():
+        with torch.cuda.device(device):
+            return C.call(name, *args, _raw_stream(i))
+    C.call(name, *args, _raw_stream(i))
 
 
 def quantize(x):
@@ -127,7 +126,7 @@ def _norm(x, norm_weight, eps, delta, delta_scale):
     if delta is None:
         return (norm_weight.data_ptr(), eps, None, 1.0, None), None
     _check(delta, "delta", _BF16, x.shape, x.device)
-    total = delta.new_empty(x.shape)
+    total = torch.empty_like(delta)
     return (norm_weight.data_ptr(), eps, delta.data_ptr(), delta_scale, total.data_ptr()), total
 
 

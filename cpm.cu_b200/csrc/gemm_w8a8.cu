@@ -418,17 +418,18 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     if (threadIdx.x == 0 && *abort_flag) atomicOr(a.error, ERR_GEMM_TIMEOUT);
 }
 
-// A tile per cluster: CTA `rank` of CS has k-blocks [rank * kblocks / CS, (rank + 1) * kblocks / CS).  When every CTA's products are done (a cluster
-// barrier), the operand rings are idle in all of them and take the sums: each CTA sends each peer that peer's share of the tokens straight from
-// tensor memory, a second barrier, and every CTA adds and stores its own share.  All threads reach both barriers whatever the bounded waits
-// before returned.
+// A tile per cluster: CTA `rank` of CS has k-blocks [rank * kblocks / CS, (rank + 1) * kblocks / CS).  Each CTA sends each peer that peer's share of the tokens
+// straight from tensor memory into a buffer beside the operand ring; one cluster barrier, and every CTA adds and stores its own share.  A first barrier only
+// says that every CTA has started: arrived at on entry, waited for before the first write to a peer.  All threads reach both barriers whatever
+// the bounded waits before returned.
 template <int MT, int CS>
 struct ClusterCfg {
     static constexpr int STAGE_BYTES = Cfg<MT, false>::STAGE_BYTES;
     static constexpr int STAGES = Cfg<MT, false>::STAGES;
     static constexpr int TPR = MT / CS + (MT % CS != 0);            // tokens summed and stored by each rank
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CTRL_BYTES + 1024;
-    static_assert(CS * TPR * TILE_ROWS * 4 <= STAGES * STAGE_BYTES, "sums must fit the ring");
+    static constexpr int RED_BYTES = CS * TPR * TILE_ROWS * 4;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + RED_BYTES + CTRL_BYTES + 1024;
+    static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
 
 template <int MT, int CS>
@@ -437,8 +438,8 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
     using C = ClusterCfg<MT, CS>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    int* red = reinterpret_cast<int*>(smem);   // [source][token][row], over the ring
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+    int* red = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE_BYTES);   // [source][token][row]: peers write here, nothing else does
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES + C::RED_BYTES);
     uint64_t* empty = full + C::STAGES;
     uint64_t* acc_full = empty + C::STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 2);
@@ -449,6 +450,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
     const int tile = blockIdx.x / CS, kblocks = a.sched.kblocks;
     const int kb_begin = kblocks * rank / CS, kpc = kblocks * (rank + 1) / CS - kb_begin;
     grid_dep_trigger();
+    ptx::cluster_arrive_relaxed();   // "this CTA runs"
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -494,7 +496,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
                 ptx::tma_load_2d(dst + BLOCK_BYTES, &tm_x, &full[stage], (kb_begin + i) * BLOCK_COLS, 0);
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }
-            if (!ok) {   // copies already in flight land before peers write over the ring
+            if (!ok) {   // copies already in flight land before the CTA retires
                 const long long t0 = clock64();
                 while (clock64() - t0 < 2000000LL) {}
             }
@@ -518,11 +520,11 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
             if (ok) ptx::umma_commit(acc_full);
         }
     } else {
-        summed = ptx::mbar_wait_warp(acc_full, 0, abort_flag);   // every product has read its operands
+        summed = ptx::mbar_wait_warp(acc_full, 0, abort_flag);
         ptx::tc_fence_after();
     }
     __syncwarp();
-    ptx::cluster_sync();   // all CTAs' products are done: the rings may be written by peers
+    ptx::cluster_wait();   // every CTA has started: its shared memory may be written
 
     const int m_cnt = min(a.sched.M, MT);
     const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);

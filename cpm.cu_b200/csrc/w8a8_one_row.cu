@@ -17,9 +17,9 @@ namespace {
 
 constexpr int WARPS = 16, THREADS = WARPS * 32;
 constexpr int SLOTS = 12;                             // 16-byte copies per lane in flight
-constexpr int STEP = 2;                               // k-blocks per step
+constexpr int MAX_STEP = 2;                           // k-blocks per step: 2, of gate/up pairs 1
 constexpr int RING_BYTES = SLOTS * THREADS * 16;
-constexpr int MAX_SMEM = RING_BYTES + MAX_COLS + STEP * BLOCK_COLS;
+constexpr int MAX_SMEM = RING_BYTES + MAX_COLS + MAX_STEP * BLOCK_COLS;
 
 struct OneRowArgs {
     RowSource src;
@@ -42,7 +42,7 @@ __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
 template <Source SRC, int VEC, bool GATED>
 __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs a) {
     constexpr int SETS = GATED ? 2 : 1;               // gate and up rows of the same features
-    constexpr int PER_STEP = STEP * SETS, DEPTH = SLOTS / PER_STEP;   // copies of a lane; steps in flight
+    constexpr int STEP = MAX_STEP / SETS, PER_STEP = STEP * SETS, DEPTH = SLOTS / PER_STEP;   // copies of a lane; steps in flight
     constexpr int KEEP = HAS_NORM<SRC> ? 2 : 4;       // vectors that a thread keeps of the row
     constexpr int TILE_UNITS = (GATED ? TILE_ROWS / 2 : TILE_ROWS) / 4;
     extern __shared__ __align__(16) uint8_t smem[];   // ring, then the integers
@@ -230,10 +230,10 @@ void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const b
     a.bias = bias; a.y = y; a.act = act;
     a.units = w.tiles * (gated ? 16 : 32);
     // Warps per group: the fewest steps of a warp, with half a step for each round's meeting
-    const int sms = runtime().num_sms, pairs = ceil_div(w.kblocks, STEP);
+    const int sms = runtime().num_sms, step_blocks = gated ? 1 : MAX_STEP, all_steps = ceil_div(w.kblocks, step_blocks);
     long long best = -1;
     for (int share = 1; share <= WARPS; share *= 2) {
-        const int rounds = ceil_div(ceil_div(a.units, WARPS / share), sms), steps = ceil_div(pairs, share);
+        const int rounds = ceil_div(ceil_div(a.units, WARPS / share), sms), steps = ceil_div(all_steps, share);
         const long long cost = static_cast<long long>(rounds) * (2 * steps + (share > 1 ? 1 : 0));
         if (best < 0 || cost < best) {
             best = cost;
@@ -243,7 +243,7 @@ void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const b
         }
     }
     const int grid = std::min(sms, ceil_div(a.units, WARPS / a.share));
-    const size_t smem = RING_BYTES + static_cast<size_t>(pairs) * STEP * BLOCK_COLS;
+    const size_t smem = RING_BYTES + static_cast<size_t>(all_steps) * step_blocks * BLOCK_COLS;
     const bool vec = rows_in_vectors(src, K);
     if (src.x32 != nullptr) run<SRC_F32, false>(a, grid, smem, vec, s);
     else if (src.norm == nullptr) gated ? run<SRC_PLAIN, true>(a, grid, smem, vec, s) : run<SRC_PLAIN, false>(a, grid, smem, vec, s);
