@@ -121,6 +121,6 @@ def append(qkv, heads, kv_heads, dim, inv_freq, positions, k_cache=None, v_cache
         out = qkv.new_empty((rows, heads * dim))
     else:
         _check(out, "out", _BF16, (rows, heads * dim), device, rows=True)
-    _call("cpmcu_rotary_append", device, qkv.data_ptr(), _ld(qkv), rows, heads, kv_heads, dim, rot, interleaved, inv_freq.data_ptr(), factor,
+    _call("cpmcu_rotary_append", qkv.get_device(), qkv.data_ptr(), _ld(qkv), rows, heads, kv_heads, dim, rot, interleaved, inv_freq.data_ptr(), factor,
           positions.data_ptr(), out.data_ptr(), _ld(out), *keys)
     return out

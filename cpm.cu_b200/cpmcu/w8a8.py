@@ -39,13 +39,12 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
 
 
-def _call(name, device, *args):
-    """The entry point on torch's current stream of `device`."""
-    i = device.index
-    if i != _current_device():
-        with torch.cuda.device(device):
-            return C.call(name, *args, _raw_stream(i))
-    C.call(name, *args, _raw_stream(i))
+def _call(name, index, *args):
+    """The entry point on torch's current stream of GPU `index`."""
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return C.call(name, *args, _raw_stream(index))
+    C.call(name, *args, _raw_stream(index))
 
 
 def quantize(x):
@@ -54,7 +53,7 @@ def quantize(x):
         raise ValueError("x must be a matrix")
     _check(x, "x", _BF16, x.shape, rows=True)
     q, scale = torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[0], dtype=_F32, device=x.device)
-    _call("cpmcu_w8a8_quantize", x.device, x.data_ptr(), _ld(x), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr())
+    _call("cpmcu_w8a8_quantize", x.get_device(), x.data_ptr(), _ld(x), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -63,13 +62,14 @@ class _Packed:
         if out < 1 or width < 1:
             raise ValueError("weights must not be empty")
         self.out, self.width, self.device = out, width, parts[0][0].device
+        self.index = parts[0][0].get_device()
         n = C.load().cpmcu_w8a8_packed_bytes(out, width, int(gated))
         if n < 0:
             raise ValueError(C.load().cpmcu_last_error().decode())
         self.data = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.ptr = self.data.data_ptr()
         for part, (q, scale) in enumerate(parts, start=int(gated)):
-            _call("cpmcu_w8a8_pack", self.device, q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr)
+            _call("cpmcu_w8a8_pack", self.index, q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr)
 
 
 class PackedLinear(_Packed):
@@ -105,15 +105,16 @@ class PackedGateUp(_Packed):
         return cls(*quantize(gate), *quantize(up))
 
 
-def _rows(x, width, device):
+def _rows(x, weight):
     """Checks x; (rows, distance of the rows)."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 2:
-        raise ValueError("x must be a matrix")
-    rows = x.shape[0]
-    if x.dtype is not _BF16 or x.device != device or x.shape[1] != width or not x.is_contiguous():
-        _check(x, "x", _BF16, (rows, width), device, rows=True)
-        return rows, _ld(x)
-    return rows, width
+    try:
+        rows, width = x.shape
+    except (AttributeError, ValueError):
+        raise ValueError("x must be a matrix") from None
+    if x.dtype is _BF16 and width == weight.width and x.get_device() == weight.index and x.is_contiguous():
+        return rows, width
+    _check(x, "x", _BF16, (rows, weight.width), weight.device, rows=True)
+    return rows, _ld(x)
 
 
 def _norm(x, norm_weight, eps, delta, delta_scale):
@@ -121,13 +122,16 @@ def _norm(x, norm_weight, eps, delta, delta_scale):
     if norm_weight is None:
         if delta is not None:
             raise ValueError("delta needs norm_weight")
-        return (None, 0.0, None, 1.0, None), None
+        return _NO_NORM, None
     _check(norm_weight, "norm_weight", _BF16, x.shape[1:], x.device)
     if delta is None:
         return (norm_weight.data_ptr(), eps, None, 1.0, None), None
     _check(delta, "delta", _BF16, x.shape, x.device)
     total = torch.empty_like(delta)
     return (norm_weight.data_ptr(), eps, delta.data_ptr(), delta_scale, total.data_ptr()), total
+
+
+_NO_NORM = (None, 0.0, None, 1.0, None)
 
 
 def _out(out, x, rows, width):
@@ -160,15 +164,15 @@ def linear(x, weight, bias=None, norm_weight=None, eps=1e-5, delta=None, delta_s
     returned.  bias [out] bf16.  x (and out) may be rows of a wider matrix."""
     if type(weight) is not PackedLinear:
         raise ValueError("weight must be a PackedLinear")
+    rows, ldx = _rows(x, weight)
     width, n = weight.width, weight.out
-    rows, ldx = _rows(x, width, weight.device)
     if bias is not None:
-        _check(bias, "bias", _BF16, (n,), x.device)
+        _check(bias, "bias", _BF16, (n,), weight.device)
         bias = bias.data_ptr()
     norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
     y, ldy = _out(out, x, rows, n)
     keep, ws, size = _workspace(x, rows, n, width, 0)
-    _call("cpmcu_w8a8_linear", weight.device, x.data_ptr(), ldx, weight.ptr, bias, *norm, y.data_ptr(), ldy, rows, n, width, ws, size)
+    _call("cpmcu_w8a8_linear", weight.index, x.data_ptr(), ldx, weight.ptr, bias, *norm, y.data_ptr(), ldy, rows, n, width, ws, size)
     return y if total is None else (y, total)
 
 
@@ -177,11 +181,11 @@ def gated_ffn(x, gate_up, down, norm_weight=None, eps=1e-5, delta=None, delta_sc
     if type(gate_up) is not PackedGateUp or type(down) is not PackedLinear:
         raise ValueError("gate_up must be a PackedGateUp and down a PackedLinear")
     width, inter = gate_up.width, gate_up.out
-    if down.width != inter or down.out != width or down.device != gate_up.device:
+    if down.width != inter or down.out != width or down.index != gate_up.index:
         raise ValueError(f"down must be [{width}, {inter}] on {gate_up.device}")
-    rows, ldx = _rows(x, width, gate_up.device)
+    rows, ldx = _rows(x, gate_up)
     norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
     y, ldy = _out(out, x, rows, width)
     keep, ws, size = _workspace(x, rows, width, width, inter)
-    _call("cpmcu_w8a8_ffn", gate_up.device, x.data_ptr(), ldx, gate_up.ptr, down.ptr, *norm, y.data_ptr(), ldy, rows, width, inter, ws, size)
+    _call("cpmcu_w8a8_ffn", gate_up.index, x.data_ptr(), ldx, gate_up.ptr, down.ptr, *norm, y.data_ptr(), ldy, rows, width, inter, ws, size)
     return y if total is None else (y, total)

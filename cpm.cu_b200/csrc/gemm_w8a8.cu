@@ -444,6 +444,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
     uint64_t* acc_full = empty + C::STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    __shared__ float xs[C::TPR];   // scales of this CTA's tokens
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(ptx::cluster_ctarank());
@@ -475,6 +476,8 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
 
     const int q = warp & 3, row = q * 32 + lane;
     bool summed = false;   // epilogue threads: this CTA's sums are in tensor memory
+    const int m_cnt = min(a.sched.M, MT), t0 = rank * C::TPR, cnt = min(m_cnt - t0, C::TPR);   // this CTA's share of the tokens
+    float ws = 0.f, bias = 0.f;
     if (warp == 0) {
         if (lane == 0) {
             const int pre = min(kpc, C::STAGES);
@@ -520,13 +523,16 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
             if (ok) ptx::umma_commit(acc_full);
         }
     } else {
+        // scales while the sums are being made
+        ws = a.ws[tile * TILE_ROWS + row];
+        if (a.act == nullptr && a.bias != nullptr && tile * TILE_ROWS + row < a.N) bias = __bfloat162float(a.bias[tile * TILE_ROWS + row]);
+        if (threadIdx.x - 64 < C::TPR) xs[threadIdx.x - 64] = static_cast<int>(threadIdx.x) - 64 < cnt ? a.xs[t0 + threadIdx.x - 64] : 0.f;
         summed = ptx::mbar_wait_warp(acc_full, 0, abort_flag);
         ptx::tc_fence_after();
     }
     __syncwarp();
     ptx::cluster_wait();   // every CTA has started: its shared memory may be written
 
-    const int m_cnt = min(a.sched.M, MT);
     const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
     if (warp >= 2 && summed) {
         const uint32_t mine = ptx::smem_u32(red + rank * C::TPR * TILE_ROWS + row);
@@ -550,17 +556,14 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
     __syncwarp();
     ptx::cluster_sync();   // this CTA's share has arrived
     if (warp >= 2 && *abort_flag == 0) {
-        const float ws = a.ws[tile * TILE_ROWS + row];
-        const int t0 = rank * C::TPR, cnt = min(m_cnt - t0, C::TPR);
         if (a.act == nullptr) {
             const int n = tile * TILE_ROWS + row;
-            const float bias = a.bias != nullptr && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
 #pragma unroll 4
             for (int t = 0; t < cnt; ++t) {
                 int sum = 0;
 #pragma unroll
                 for (int s = 0; s < CS; ++s) sum += red[(s * C::TPR + t) * TILE_ROWS + row];
-                if (n < a.N) a.y[static_cast<long long>(t0 + t) * a.ldy + n] = __float2bfloat16(fmaf(static_cast<float>(sum) * a.xs[t0 + t], ws, bias));
+                if (n < a.N) a.y[static_cast<long long>(t0 + t) * a.ldy + n] = __float2bfloat16(fmaf(static_cast<float>(sum) * xs[t], ws, bias));
             }
         } else {
             // gate rows 0-63 and up rows 64-127 meet in the first source's place, scaled
@@ -570,7 +573,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
                 int sum = 0;
 #pragma unroll
                 for (int s = 0; s < CS; ++s) sum += red[(s * C::TPR + t) * TILE_ROWS + row];
-                meet[t * TILE_ROWS + row] = static_cast<float>(sum) * a.xs[t0 + t] * ws;
+                meet[t * TILE_ROWS + row] = static_cast<float>(sum) * xs[t] * ws;
             }
             ptx::named_bar_sync(1, 128);
             const int f = row & 63, n = tile * 64 + f;

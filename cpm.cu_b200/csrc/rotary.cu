@@ -69,87 +69,92 @@ struct Piece {
 
 constexpr int MAX_HALF = 512;
 
-template <int VEC, bool INTERLEAVED, bool WIDE>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
-    __shared__ float2 table[MAX_HALF];
-    grid_dep_wait();
-    grid_dep_trigger();
-    const long long r = blockIdx.x;
-    const bf16* row = a.qkv + r * a.ld;
-    bf16* q = a.q + r * a.ldq;
-    const int kv_dim = a.kv_heads * a.dim;
-    long long slot = -1;
-    if (a.kv_heads > 0) {
-        slot = a.slots[r];
-        if (slot >= a.cache_rows) {   // memory stays intact; the host hears of it
-            slot = -1;
-            if (threadIdx.x == 0) atomicOr(a.error, ERR_KV_OVERFLOW);
-        }
-    }
-    const bool keep = slot >= 0;
-    bf16* k = a.k_cache + slot * kv_dim;
+// R rows per CTA.  Each thread's first pieces of all its rows are in flight before the tables are made.
+template <int VEC, bool INTERLEAVED, bool WIDE, int R>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a, int rows) {
+    extern __shared__ float2 table[];   // [R][half]
+    constexpr int AHEAD = 2;
+    const int kv_dim = a.kv_heads * a.dim, all = a.heads + a.kv_heads;
     // pieces of a head that are rotated (interleaved: all of it, the unrotated pairs as they are), and that are copied
     const int turned = INTERLEAVED ? a.dim / VEC : a.half / VEC, copied = INTERLEAVED ? 0 : (a.dim - 2 * a.half) / VEC;
-    const int all = a.heads + a.kv_heads;
-    auto target = [&](int h, int c) { return h < a.heads ? q + h * a.dim + c : k + (h - a.heads) * a.dim + c; };
-
-    // the first pieces of each kind are in flight before the table is made
-    constexpr int AHEAD = 2;
     const int items = all * turned;
-    Piece<VEC, INTERLEAVED, WIDE> piece[AHEAD];
-    const bf16* v = row + all * a.dim;
-    Elems<VEC, WIDE> value;
     const int v0 = threadIdx.x * VEC;
-    auto place = [&](int i, int& h, int& c) {
-        h = i / turned;
-        c = (i - h * turned) * VEC;
-    };
+    const long long r0 = static_cast<long long>(blockIdx.x) * R;
+    // where this thread's first pieces lie in a row
+    int head[AHEAD], first[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
         const int i = threadIdx.x + j * blockDim.x;
-        int h, c;
-        place(i, h, c);
-        if (i < items) piece[j].load(row + h * a.dim + c, a.half);
+        head[j] = turned > 0 ? i / turned : 0;
+        first[j] = turned > 0 ? (i - head[j] * turned) * VEC : 0;
     }
-    if (keep && v0 < kv_dim) value.load(v + v0);
-    const double p = a.pos[r];
-    for (int t = threadIdx.x; t < a.half; t += blockDim.x) {
-        const double turns = p * static_cast<double>(a.inv_freq[t]) * 0.15915494309189533577;
-        float sn, cs;
-        sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-        table[t] = make_float2(cs * a.factor, sn * a.factor);
+    grid_dep_wait();
+    grid_dep_trigger();
+    auto row_at = [&](int r) { return a.qkv + (r0 + r) * a.ld; };
+    Piece<VEC, INTERLEAVED, WIDE> piece[R][AHEAD];
+    Elems<VEC, WIDE> value[R];
+    int32_t slot[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        slot[r] = a.kv_heads > 0 && r0 + r < rows ? a.slots[r0 + r] : -1;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (threadIdx.x + j * blockDim.x < items && r0 + r < rows) piece[r][j].load(row_at(r) + head[j] * a.dim + first[j], a.half);
+        }
+        if (v0 < kv_dim && r0 + r < rows) value[r].load(row_at(r) + all * a.dim + v0);
     }
-    bf16* v_row = a.v_cache + slot * kv_dim;
-    if (keep && v0 < kv_dim) value.store(v_row + v0);
+    for (int t = threadIdx.x; t < R * a.half; t += blockDim.x) {
+        const int r = R > 1 ? t / a.half : 0, i = t - r * a.half;
+        if (r0 + r < rows) {
+            const double turns = static_cast<double>(a.pos[r0 + r]) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;
+            float sn, cs;
+            sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+            table[t] = make_float2(cs * a.factor, sn * a.factor);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (slot[r] >= a.cache_rows) {   // memory stays intact; the host hears of it
+            slot[r] = -1;
+            if (threadIdx.x == 0) atomicOr(a.error, ERR_KV_OVERFLOW);
+        }
+        if (slot[r] >= 0 && v0 < kv_dim) value[r].store(a.v_cache + static_cast<long long>(slot[r]) * kv_dim + v0);
+    }
     __syncthreads();
-    auto finish = [&](Piece<VEC, INTERLEAVED, WIDE>& e, int h, int c) {
-        e.rotate(c, a.half, table);
-        if (h < a.heads || keep) e.store(target(h, c), a.half);
-    };
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-        const int i = threadIdx.x + j * blockDim.x;
-        int h, c;
-        place(i, h, c);
-        if (i < items) finish(piece[j], h, c);
-    }
-    for (int i = threadIdx.x + AHEAD * blockDim.x; i < items; i += blockDim.x) {
-        int h, c;
-        place(i, h, c);
-        piece[0].load(row + h * a.dim + c, a.half);
-        finish(piece[0], h, c);
-    }
-    // what no rotation reaches: the rest of the heads, and the values
-    for (int j = threadIdx.x; j < all * copied; j += blockDim.x) {
-        const int hh = j / copied, cc = 2 * a.half + (j - hh * copied) * VEC;
-        Elems<VEC, WIDE> e;
-        e.load(row + hh * a.dim + cc);
-        if (hh < a.heads || keep) e.store(target(hh, cc));
-    }
-    if (keep) {
-        for (int j = v0 + blockDim.x * VEC; j < kv_dim; j += blockDim.x * VEC) {
-            value.load(v + j);
-            value.store(v_row + j);
+    for (int r = 0; r < R; ++r) {
+        if (r0 + r >= rows) break;
+        const bf16* row = row_at(r);
+        bf16* q = a.q + (r0 + r) * a.ldq;
+        const bool keep = slot[r] >= 0;
+        bf16* k = a.k_cache + static_cast<long long>(slot[r]) * kv_dim;
+        auto target = [&](int h, int c) { return h < a.heads ? q + h * a.dim + c : k + (h - a.heads) * a.dim + c; };
+        auto finish = [&](Piece<VEC, INTERLEAVED, WIDE>& e, int h, int c) {
+            e.rotate(c, a.half, table + r * a.half);
+            if (h < a.heads || keep) e.store(target(h, c), a.half);
+        };
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (threadIdx.x + j * blockDim.x < items) finish(piece[r][j], head[j], first[j]);
+        }
+        for (int i = threadIdx.x + AHEAD * blockDim.x; i < items; i += blockDim.x) {
+            const int h = i / turned, c = (i - h * turned) * VEC;
+            piece[r][0].load(row + h * a.dim + c, a.half);
+            finish(piece[r][0], h, c);
+        }
+        // what no rotation reaches: the rest of the heads, and the values
+        for (int j = threadIdx.x; j < all * copied; j += blockDim.x) {
+            const int h = j / copied, c = 2 * a.half + (j - h * copied) * VEC;
+            Elems<VEC, WIDE> e;
+            e.load(row + h * a.dim + c);
+            if (h < a.heads || keep) e.store(target(h, c));
+        }
+        if (keep) {
+            bf16* v_row = a.v_cache + static_cast<long long>(slot[r]) * kv_dim;
+            for (int j = v0 + blockDim.x * VEC; j < kv_dim; j += blockDim.x * VEC) {
+                value[r].load(row + all * a.dim + j);
+                value[r].store(v_row + j);
+            }
         }
     }
 }
@@ -170,27 +175,33 @@ void launch_rotary(const RotaryArgs& a, int rows, bool interleaved, cudaStream_t
     const bool wide = fits(vec);
     const int pieces = (a.heads + 2 * a.kv_heads) * a.dim / vec;
     const int threads = pieces >= 256 ? 256 : (pieces + 31) / 32 * 32;
-    auto go = [&](auto kernel) {
+    const int sms = runtime().num_sms;
+    // two rows per CTA once there are several CTAs for every SM: their loads and tables overlap (TWO_ROWS figures at the top)
+    const bool two = rows >= 8 * sms;
+    auto go = [&](auto kernel, int per_cta) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(rows);
+        cfg.gridDim = dim3(ceil_div(rows, per_cta));
         cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = static_cast<size_t>(per_cta) * a.half * sizeof(float2);
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = runtime().pdl ? 1 : 0;
-        CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, a));
+        CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, a, rows));
     };
     if (interleaved) {
-        if (vec == 8) go(rotary_kernel<8, true, true>);
-        else if (vec == 4) go(rotary_kernel<4, true, true>);
-        else if (wide) go(rotary_kernel<2, true, true>);
-        else go(rotary_kernel<2, true, false>);
+        if (vec == 8 && two) go(rotary_kernel<8, true, true, 2>, 2);
+        else if (vec == 8) go(rotary_kernel<8, true, true, 1>, 1);
+        else if (vec == 4) go(rotary_kernel<4, true, true, 1>, 1);
+        else if (wide) go(rotary_kernel<2, true, true, 1>, 1);
+        else go(rotary_kernel<2, true, false, 1>, 1);
     } else {
-        if (vec == 8) go(rotary_kernel<8, false, true>);
-        else if (vec == 4) go(rotary_kernel<4, false, true>);
-        else if (vec == 2) go(rotary_kernel<2, false, true>);
-        else go(rotary_kernel<1, false, false>);
+        if (vec == 8 && two) go(rotary_kernel<8, false, true, 2>, 2);
+        else if (vec == 8) go(rotary_kernel<8, false, true, 1>, 1);
+        else if (vec == 4) go(rotary_kernel<4, false, true, 1>, 1);
+        else if (vec == 2) go(rotary_kernel<2, false, true, 1>, 1);
+        else go(rotary_kernel<1, false, false, 1>, 1);
     }
 }

@@ -85,6 +85,8 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
             seek();
         }
     };
+    // the row's lines first: behind the weights' they would be late
+    if (static_cast<int>(threadIdx.x) * VEC < a.K && threadIdx.x % 8 == 0) Values<SRC, VEC>::ask(a.src, 0, a.K, threadIdx.x * VEC);
     seek();
 #pragma unroll 1
     for (int i = 0; i < DEPTH; ++i) issue();
@@ -105,15 +107,13 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
     for (int j = 0; j < KEEP; ++j) {
         const int c = (threadIdx.x + j * THREADS) * VEC;
         if (c < a.K) {
-            kept[j].combine(a.src, 0, a.K, c, blockIdx.x == 0);
-            kept[j].measure(top, ss);
+            kept[j].combine(a.src, 0, a.K, c, blockIdx.x == 0, top, ss);
         }
     }
     for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {   // of longer rows: read again below
         Values<SRC, VEC> r;
         r.fetch(a.src, 0, a.K, c);
-        r.combine(a.src, 0, a.K, c, blockIdx.x == 0);
-        r.measure(top, ss);
+        r.combine(a.src, 0, a.K, c, blockIdx.x == 0, top, ss);
     }
     top = block_max(top, sh_top);
     float factor = 1.f;
@@ -130,9 +130,10 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
     }
     for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {
         Values<SRC, VEC> r;
-        float v[VEC];
+        float v[VEC], squares = 0.f;
+        uint32_t known = 0u;
         r.fetch(a.src, 0, a.K, c);
-        r.combine(a.src, 0, a.K, c, false);
+        r.combine(a.src, 0, a.K, c, false, known, squares);
         r.values(v);
         store_ints<VEC>(q + c, round8, v);
     }

@@ -28,9 +28,10 @@ template <Source SRC, int VPT, int VEC>
 __global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const QuantizeArgs a) {
     __shared__ uint32_t sh_top[32];
     __shared__ float sh_sum[32];
+    const size_t row = blockIdx.x;
+    if (static_cast<int>(threadIdx.x) * VEC < a.K && threadIdx.x % 8 == 0) Values<SRC, VEC>::ask(a.src, row, a.K, threadIdx.x * VEC);
     grid_dep_wait();
     grid_dep_trigger();
-    const size_t row = blockIdx.x;
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < a.n_clear; i += gridDim.x * blockDim.x) a.clear[i] = 0;
     Values<SRC, VEC> kept[VPT > 0 ? VPT : 1];
     float ss = 0.f;
@@ -47,15 +48,13 @@ __global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const Qua
         for (int j = 0; j < VPT; ++j) {
             const int c = threadIdx.x * VEC + j * step;
             if (c < a.K) {
-                kept[j].combine(a.src, row, a.K, c, true);
-                kept[j].measure(top, ss);
+                kept[j].combine(a.src, row, a.K, c, true, top, ss);
             }
         }
     } else {
         for (int c = threadIdx.x * VEC; c < a.K; c += step) {
             kept[0].fetch(a.src, row, a.K, c);
-            kept[0].combine(a.src, row, a.K, c, true);
-            kept[0].measure(top, ss);
+            kept[0].combine(a.src, row, a.K, c, true, top, ss);
         }
     }
     top = block_max(top, sh_top);
@@ -77,7 +76,9 @@ __global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const Qua
     } else {
         for (int c = threadIdx.x * VEC; c < a.K; c += step) {
             kept[0].fetch(a.src, row, a.K, c);
-            kept[0].combine(a.src, row, a.K, c, false);
+            uint32_t known = 0u;
+            float squares = 0.f;
+            kept[0].combine(a.src, row, a.K, c, false, known, squares);
             finish(kept[0], c);
         }
     }

@@ -116,59 +116,62 @@ __device__ __forceinline__ void store_ints(int8_t* q, const RowRound& round, con
 }
 
 // ---------------------------------------------------------------- VEC consecutive elements of a row
-// kept as they came (t: bf16 pairs, or fp32), because a row waits for its maximum in registers
+// fetch() loads them, combine() makes the residual sum, the largest magnitude and the squares of it, values() gives what is rounded.  A row waits for its
+// maximum in registers: as it came (bf16, fp32), or as the products with the norm's weights (fp32, in the registers of x and the weights).
 template <Source SRC, int VEC>
 struct Values {
     using T = typename std::conditional<SRC == SRC_F32, float, bf16>::type;
     struct alignas(VEC == 8 ? 16 : sizeof(T)) Block { T e[VEC]; };
     Block t, d, w;
+    float p[VEC];
     __device__ __forceinline__ static const T* base(const RowSource& s) {
         if constexpr (SRC == SRC_F32) return s.x32;
         else return s.x;
+    }
+    // asks for the lines ahead of the wait for the predecessor: into L2 only, where later writes find them
+    __device__ __forceinline__ static void ask(const RowSource& s, size_t row, int K, int c) {
+        prefetch_l2(base(s) + row * s.ldx + c);
+        if constexpr (SRC == SRC_ADD_NORM) prefetch_l2(s.delta + row * K + c);
+        if constexpr (HAS_NORM<SRC>) prefetch_l2(s.norm + c);
     }
     __device__ __forceinline__ void fetch(const RowSource& s, size_t row, int K, int c) {
         t = *reinterpret_cast<const Block*>(base(s) + row * s.ldx + c);
         if constexpr (SRC == SRC_ADD_NORM) d = *reinterpret_cast<const Block*>(s.delta + row * K + c);
         if constexpr (HAS_NORM<SRC>) w = *reinterpret_cast<const Block*>(s.norm + c);
     }
-    // the residual sum, in place of x; `write`: stores it
-    __device__ __forceinline__ void combine(const RowSource& s, size_t row, int K, int c, bool write) {
+    // `write`: stores the residual sum
+    __device__ __forceinline__ void combine(const RowSource& s, size_t row, int K, int c, bool write, uint32_t& top, float& ss) {
         if constexpr (SRC == SRC_ADD_NORM) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) t.e[e] = __float2bfloat16(fmaf(__bfloat162float(d.e[e]), s.delta_scale, __bfloat162float(t.e[e])));
             if (write) *reinterpret_cast<Block*>(s.total + row * K + c) = t;
         }
+        if constexpr (SRC == SRC_PLAIN && VEC == 8) {   // two magnitudes at a time, as 16-bit patterns
+            const uint32_t* pairs = reinterpret_cast<const uint32_t*>(t.e);
+            uint32_t m = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = __vmaxu2(m, pairs[i] & 0x7fff7fffu);
+            top = max(top, max(m << 16, m & 0xffff0000u));
+        } else {
+            float m = 0.f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float v = to_float(t.e[e]);
+                if constexpr (HAS_NORM<SRC>) {
+                    ss = fmaf(v, v, ss);
+                    v *= to_float(w.e[e]);
+                    p[e] = v;
+                }
+                m = max_magnitude(m, v);
+            }
+            top = max(top, __float_as_uint(m));
+        }
     }
-    // what is rounded
     __device__ __forceinline__ void values(float (&v)[VEC]) const {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            v[e] = to_float(t.e[e]);
-            if constexpr (HAS_NORM<SRC>) v[e] *= to_float(w.e[e]);
-        }
-    }
-    // the largest magnitude of values(), and the squares that a norm needs
-    __device__ __forceinline__ void measure(uint32_t& top, float& ss) const {
-        if constexpr (SRC == SRC_PLAIN && VEC == 8) {   // two magnitudes at a time, as 16-bit patterns
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(t.e);
-            uint32_t m = 0u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-            top = max(top, max(m << 16, m & 0xffff0000u));
-        } else {
-            float v[VEC];
-            values(v);
-            float m = 0.f;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) m = max_magnitude(m, v[e]);
-            top = max(top, __float_as_uint(m));
-            if constexpr (HAS_NORM<SRC>) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float f = to_float(t.e[e]);
-                    ss = fmaf(f, f, ss);
-                }
-            }
+            if constexpr (HAS_NORM<SRC>) v[e] = p[e];
+            else v[e] = to_float(t.e[e]);
         }
     }
 };
