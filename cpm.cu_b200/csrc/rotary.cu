@@ -7,6 +7,9 @@
 // radians.  One CTA per row: its loads are in flight while some threads make the row's `half` sines and cosines.
 //
 // Bound: every element in and out once.
+#include <algorithm>
+
+#include "ptx.cuh"
 #include "row_ops.cuh"
 #include "rotary.cuh"
 
@@ -40,7 +43,29 @@ __device__ __forceinline__ void turn(bf16& a, bf16& b, float cs, float sn) {
     b = __float2bfloat16(fmaf(y, cs, x * sn));
 }
 
-// A piece of a row: with PAIRED halves VEC elements and their partners `half` further on, or VEC elements that lie together.
+// Sines and cosines of a row: `padded` cosines, then the sines.
+__host__ __device__ constexpr int padded(int half) { return (half + 7) / 8 * 8; }
+// turns per position of a frequency
+__device__ __forceinline__ double turns_of(float inv_freq) { return static_cast<double>(inv_freq) * 0.15915494309189533577; }
+__device__ __forceinline__ void fill(float* table, int i, int half, int32_t pos, double per_pos, float factor) {
+    const double turns = static_cast<double>(pos) * per_pos;
+    float sn, cs;
+    sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+    table[i] = cs * factor;
+    table[padded(half) + i] = sn * factor;
+}
+template <int N>
+__device__ __forceinline__ void take(const float* p, float (&f)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(p + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = p[i];
+    }
+}
+
+// A piece of a row: VEC elements and their partners `half` further on, or (interleaved) VEC elements that lie together.
 template <int VEC, bool INTERLEAVED, bool WIDE>
 struct Piece {
     Elems<VEC, WIDE> lo, hi;
@@ -48,17 +73,21 @@ struct Piece {
         lo.load(p);
         if constexpr (!INTERLEAVED) hi.load(p + half);
     }
-    // c: first element in the head
-    __device__ __forceinline__ void rotate(int c, int half, const float2* table) {
-        if constexpr (INTERLEAVED) {
+    // c: first element in the head, a multiple of VEC
+    __device__ __forceinline__ void rotate(int c, int half, const float* table) {
+        constexpr int N = INTERLEAVED ? (VEC + 1) / 2 : VEC;   // pairs
+        const int first = INTERLEAVED ? c >> 1 : c;
+        alignas(16) float cs[N], sn[N];
+        if (INTERLEAVED && first >= half) return;
+        take<N>(table + first, cs);
+        take<N>(table + padded(half) + first, sn);
 #pragma unroll
-            for (int j = 0; j < VEC; j += 2) {
-                const int i = (c + j) >> 1;
-                if (i < half) turn(lo.e[j], lo.e[(j + 1) % VEC], table[i].x, table[i].y);
+        for (int j = 0; j < N; ++j) {
+            if constexpr (INTERLEAVED) {
+                if (first + j < half) turn(lo.e[2 * j], lo.e[(2 * j + 1) % VEC], cs[j], sn[j]);
+            } else {
+                turn(lo.e[j], hi.e[j], cs[j], sn[j]);
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) turn(lo.e[j], hi.e[j], table[c + j].x, table[c + j].y);
         }
     }
     __device__ __forceinline__ void store(bf16* p, int half) const {
@@ -69,93 +98,219 @@ struct Piece {
 
 constexpr int MAX_HALF = 512;
 
-// R rows per CTA.  Each thread's first pieces of all its rows are in flight before the tables are made.
-template <int VEC, bool INTERLEAVED, bool WIDE, int R>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a, int rows) {
-    extern __shared__ float2 table[];   // [R][half]
+// One CTA per row: what has few rows, and what does not lie in 16-byte pieces.  A thread's first pieces are in flight before the table is made.
+template <int VEC, bool INTERLEAVED, bool WIDE>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+    __shared__ __align__(16) float table[2 * padded(MAX_HALF)];
     constexpr int AHEAD = 2;
     const int kv_dim = a.kv_heads * a.dim, all = a.heads + a.kv_heads;
     // pieces of a head that are rotated (interleaved: all of it, the unrotated pairs as they are), and that are copied
     const int turned = INTERLEAVED ? a.dim / VEC : a.half / VEC, copied = INTERLEAVED ? 0 : (a.dim - 2 * a.half) / VEC;
     const int items = all * turned;
     const int v0 = threadIdx.x * VEC;
-    const long long r0 = static_cast<long long>(blockIdx.x) * R;
-    // where this thread's first pieces lie in a row
-    int head[AHEAD], first[AHEAD];
+    const long long r = blockIdx.x;
+    const bf16* row = a.qkv + r * a.ld;
+    bf16* q = a.q + r * a.ldq;
+    grid_dep_wait();
+    grid_dep_trigger();
+    Piece<VEC, INTERLEAVED, WIDE> piece[AHEAD];
+    Elems<VEC, WIDE> value;
+    auto place = [&](int i, int& h, int& c) {
+        h = i / turned;
+        c = (i - h * turned) * VEC;
+    };
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
         const int i = threadIdx.x + j * blockDim.x;
-        head[j] = turned > 0 ? i / turned : 0;
-        first[j] = turned > 0 ? (i - head[j] * turned) * VEC : 0;
-    }
-    grid_dep_wait();
-    grid_dep_trigger();
-    auto row_at = [&](int r) { return a.qkv + (r0 + r) * a.ld; };
-    Piece<VEC, INTERLEAVED, WIDE> piece[R][AHEAD];
-    Elems<VEC, WIDE> value[R];
-    int32_t slot[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        slot[r] = a.kv_heads > 0 && r0 + r < rows ? a.slots[r0 + r] : -1;
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            if (threadIdx.x + j * blockDim.x < items && r0 + r < rows) piece[r][j].load(row_at(r) + head[j] * a.dim + first[j], a.half);
-        }
-        if (v0 < kv_dim && r0 + r < rows) value[r].load(row_at(r) + all * a.dim + v0);
-    }
-    for (int t = threadIdx.x; t < R * a.half; t += blockDim.x) {
-        const int r = R > 1 ? t / a.half : 0, i = t - r * a.half;
-        if (r0 + r < rows) {
-            const double turns = static_cast<double>(a.pos[r0 + r]) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;
-            float sn, cs;
-            sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-            table[t] = make_float2(cs * a.factor, sn * a.factor);
+        if (i < items) {
+            int h, c;
+            place(i, h, c);
+            piece[j].load(row + h * a.dim + c, a.half);
         }
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (slot[r] >= a.cache_rows) {   // memory stays intact; the host hears of it
-            slot[r] = -1;
-            if (threadIdx.x == 0) atomicOr(a.error, ERR_KV_OVERFLOW);
-        }
-        if (slot[r] >= 0 && v0 < kv_dim) value[r].store(a.v_cache + static_cast<long long>(slot[r]) * kv_dim + v0);
+    if (v0 < kv_dim) value.load(row + all * a.dim + v0);
+    long long slot = a.kv_heads > 0 ? a.slots[r] : -1;
+    const int32_t pos = a.pos[r];
+    for (int t = threadIdx.x; t < a.half; t += blockDim.x) fill(table, t, a.half, pos, turns_of(a.inv_freq[t]), a.factor);
+    if (slot >= a.cache_rows) {   // memory stays intact; the host hears of it
+        slot = -1;
+        if (threadIdx.x == 0) atomicOr(a.error, ERR_KV_OVERFLOW);
     }
+    const bool keep = slot >= 0;
+    bf16 *k_row = a.k_cache + slot * kv_dim, *v_row = a.v_cache + slot * kv_dim;
+    auto target = [&](int h, int c) { return h < a.heads ? q + h * a.dim + c : k_row + (h - a.heads) * a.dim + c; };
+    if (keep && v0 < kv_dim) value.store(v_row + v0);
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (r0 + r >= rows) break;
-        const bf16* row = row_at(r);
-        bf16* q = a.q + (r0 + r) * a.ldq;
-        const bool keep = slot[r] >= 0;
-        bf16* k = a.k_cache + static_cast<long long>(slot[r]) * kv_dim;
-        auto target = [&](int h, int c) { return h < a.heads ? q + h * a.dim + c : k + (h - a.heads) * a.dim + c; };
-        auto finish = [&](Piece<VEC, INTERLEAVED, WIDE>& e, int h, int c) {
-            e.rotate(c, a.half, table + r * a.half);
-            if (h < a.heads || keep) e.store(target(h, c), a.half);
-        };
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            if (threadIdx.x + j * blockDim.x < items) finish(piece[r][j], head[j], first[j]);
-        }
-        for (int i = threadIdx.x + AHEAD * blockDim.x; i < items; i += blockDim.x) {
-            const int h = i / turned, c = (i - h * turned) * VEC;
-            piece[r][0].load(row + h * a.dim + c, a.half);
-            finish(piece[r][0], h, c);
-        }
-        // what no rotation reaches: the rest of the heads, and the values
+    for (int i = threadIdx.x, j = 0; i < items; i += blockDim.x, ++j) {
+        int h, c;
+        place(i, h, c);
+        Piece<VEC, INTERLEAVED, WIDE> e;
+        if (j == 0) e = piece[0];
+        else if (j == 1) e = piece[1];
+        else e.load(row + h * a.dim + c, a.half);
+        e.rotate(c, a.half, table);
+        if (h < a.heads || keep) e.store(target(h, c), a.half);
+    }
+    // what no rotation reaches: the rest of the heads, and the values
+    if constexpr (!INTERLEAVED) {
         for (int j = threadIdx.x; j < all * copied; j += blockDim.x) {
             const int h = j / copied, c = 2 * a.half + (j - h * copied) * VEC;
             Elems<VEC, WIDE> e;
             e.load(row + h * a.dim + c);
             if (h < a.heads || keep) e.store(target(h, c));
         }
-        if (keep) {
-            bf16* v_row = a.v_cache + static_cast<long long>(slot[r]) * kv_dim;
-            for (int j = v0 + blockDim.x * VEC; j < kv_dim; j += blockDim.x * VEC) {
-                value[r].load(row + all * a.dim + j);
-                value[r].store(v_row + j);
+    }
+    if (keep) {
+        for (int j = v0 + blockDim.x * VEC; j < kv_dim; j += blockDim.x * VEC) {
+            value.load(row + all * a.dim + j);
+            value.store(v_row + j);
+        }
+    }
+}
+
+// Many rows: CTAs that stay, each with a ring of groups of rows in shared memory.  Bulk copies bring a group; while the threads turn group i, some of them
+// make the tables of group i + 1, and the copies of the next groups are on their way.  A row alone in a CTA spends a third of its time with loads in
+// flight.
+constexpr int RING_STAGES = 3, RING_GROUP_BYTES = 12 * 1024, RING_MAX_GROUP = 8, RING_MAX_ROW_BYTES = 24 * 1024, RING_CTAS = 4;
+// i / d for i * d < 2^32
+struct Divisor {
+    uint32_t d = 1, m = 0;
+    void set(int v) { d = v; m = v > 1 ? static_cast<uint32_t>(((1ull << 32) + v - 1) / v) : 0u; }
+    __device__ __forceinline__ int operator()(int i) const { return d == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), m)); }
+};
+struct RingArgs {
+    RotaryArgs a;
+    int rows, group, groups, row_bytes;
+    int turned, copied;                       // pieces of 16 rotated elements, and of 8 copied ones, per head
+    Divisor by_items, by_turned, by_copies, by_copied, by_values;
+};
+template <bool INTERLEAVED>
+__global__ void __launch_bounds__(256, RING_CTAS) rotary_ring_kernel(const RingArgs g) {
+    constexpr int VEC = 8;
+    const RotaryArgs& a = g.a;
+    const int G = g.group, pad = 2 * padded(a.half), stage_bytes = G * g.row_bytes;
+    extern __shared__ __align__(128) uint8_t smem[];   // stages of G rows, then two sets of G tables
+    float* tables = reinterpret_cast<float*>(smem + RING_STAGES * stage_bytes);
+    __shared__ uint64_t full[RING_STAGES];
+    __shared__ int slots[2][RING_MAX_GROUP];
+    __shared__ int abort_flag;
+    const int kv_dim = a.kv_heads * a.dim, all = a.heads + a.kv_heads;
+    const int items = all * g.turned, copies = all * g.copied, values = kv_dim / VEC;
+    // a piece is two vectors, this far apart: interleaved pairs lie in the vectors, the others across them
+    const int apart = INTERLEAVED ? a.dim / 2 : a.half;
+    const int n = (g.groups - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1;   // groups of this CTA
+    auto row_of = [&](int i, int r) { return (static_cast<long long>(blockIdx.x) + static_cast<long long>(i) * gridDim.x) * G + r; };
+    auto rows_in = [&](int i) { return static_cast<int>(min(static_cast<long long>(G), g.rows - row_of(i, 0))); };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < RING_STAGES; ++s) ptx::mbar_init(&full[s], 1);
+        abort_flag = 0;
+        ptx::mbar_fence_init();
+    }
+    __syncthreads();
+    grid_dep_wait();
+    grid_dep_trigger();
+    auto fetch = [&](int i, int s) {
+        const int m = rows_in(i);
+        ptx::mbar_arrive_expect_tx(&full[s], m * g.row_bytes);
+        for (int r = 0; r < m; ++r) ptx::bulk_load(smem + s * stage_bytes + r * g.row_bytes, a.qkv + row_of(i, r) * a.ld, g.row_bytes, &full[s]);
+    };
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RING_STAGES && i < n; ++i) fetch(i, i);
+    }
+    // A thread has one pair of one of the rows (or, of wide heads in groups of one, further ones); its frequency stays in a register, and positions
+    // and slots are loaded two groups ahead: a table is arithmetic alone.
+    const int my_row = a.half > 0 ? threadIdx.x / a.half : G, my_pair = a.half > 0 ? threadIdx.x - my_row * a.half : 0;
+    const double mine = my_row < G ? turns_of(a.inv_freq[my_pair]) : 0.0;
+    auto pos_of = [&](int i) { return my_row < G && i < n && my_row < rows_in(i) ? a.pos[row_of(i, my_row)] : 0; };
+    auto slot_of = [&](int i) { return static_cast<int>(threadIdx.x) < G && a.kv_heads > 0 && i < n && static_cast<int>(threadIdx.x) < rows_in(i) ? a.slots[row_of(i, threadIdx.x)] : -1; };
+    auto prepare = [&](int i, int32_t pos, int slot) {
+        float* t = tables + (i & 1) * G * pad;
+        if (my_row < G) fill(t + my_row * pad, my_pair, a.half, pos, mine, a.factor);
+        for (int k = threadIdx.x + blockDim.x; k < a.half; k += blockDim.x) fill(t, k, a.half, pos, turns_of(a.inv_freq[k]), a.factor);
+        if (static_cast<int>(threadIdx.x) < G) {
+            if (slot >= a.cache_rows) {   // memory stays intact; the host hears of it
+                slot = -1;
+                atomicOr(a.error, ERR_KV_OVERFLOW);
+            }
+            slots[i & 1][threadIdx.x] = slot;
+        }
+    };
+    prepare(0, pos_of(0), slot_of(0));
+    int32_t next_pos = pos_of(1);
+    int next_slot = slot_of(1);
+    __syncthreads();
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < n; ++i) {
+        const int32_t pos = next_pos;
+        const int slot = next_slot;
+        next_pos = pos_of(i + 2);
+        next_slot = slot_of(i + 2);
+        if (i + 1 < n) prepare(i + 1, pos, slot);
+        if (!ptx::mbar_wait(&full[stage], phase, &abort_flag)) break;
+        const int m = rows_in(i);
+        const float* table = tables + (i & 1) * G * pad;
+        const bf16* from = reinterpret_cast<const bf16*>(smem + stage * stage_bytes);
+        const int row_elems = g.row_bytes / 2;
+        const long long r0 = row_of(i, 0);
+        auto put = [&](auto& e, int r, int h, int c) {
+            if (h < a.heads) {
+                e(a.q + (r0 + r) * a.ldq + h * a.dim + c);
+            } else {
+                const long long at = slots[i & 1][r];
+                if (at >= 0) e(a.k_cache + at * kv_dim + (h - a.heads) * a.dim + c);
+            }
+        };
+        for (int j = threadIdx.x; j < m * items; j += blockDim.x) {
+            const int r = g.by_items(j), k = j - r * items, h = g.by_turned(k), c = (k - h * g.turned) * VEC;
+            const bf16* at = from + r * row_elems + h * a.dim + c;
+            Piece<VEC, INTERLEAVED, true> e;
+            e.load(at, a.half);
+            if constexpr (INTERLEAVED) {
+                Piece<VEC, true, true> e2;
+                e2.load(at + apart, a.half);
+                e.rotate(c, a.half, table + r * pad);
+                e2.rotate(c + apart, a.half, table + r * pad);
+                auto store = [&](bf16* to) {
+                    e.store(to, a.half);
+                    e2.store(to + apart, a.half);
+                };
+                put(store, r, h, c);
+            } else {
+                e.rotate(c, a.half, table + r * pad);
+                auto store = [&](bf16* to) { e.store(to, a.half); };
+                put(store, r, h, c);
             }
         }
+        // values, and what no rotation reaches, from the other end of the threads
+        const int back = blockDim.x - 1 - threadIdx.x;
+        if constexpr (!INTERLEAVED) {
+            for (int j = back; j < m * copies; j += blockDim.x) {
+                const int r = g.by_copies(j), k = j - r * copies, h = g.by_copied(k), c = 2 * a.half + (k - h * g.copied) * VEC;
+                Elems<VEC, true> e;
+                e.load(from + r * row_elems + h * a.dim + c);
+                auto store = [&](bf16* to) { e.store(to); };
+                put(store, r, h, c);
+            }
+        }
+        for (int j = back; j < m * values; j += blockDim.x) {
+            const int r = g.by_values(j), c = (j - r * values) * VEC;
+            const long long at = slots[i & 1][r];
+            Elems<VEC, true> e;
+            e.load(from + r * row_elems + all * a.dim + c);
+            if (at >= 0) e.store(a.v_cache + at * kv_dim + c);
+        }
+        __syncthreads();   // the group has been read, the next tables are there
+        if (threadIdx.x == 0 && i + RING_STAGES < n) {
+            ptx::fence_proxy_async_smem();
+            fetch(i + RING_STAGES, stage);
+        }
+        if (++stage == RING_STAGES) { stage = 0; phase ^= 1; }
+    }
+    if (abort_flag) {   // copies in flight land before the CTA retires
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+        if (threadIdx.x == 0) atomicOr(a.error, ERR_GEMM_TIMEOUT);
     }
 }
 
@@ -173,35 +328,63 @@ void launch_rotary(const RotaryArgs& a, int rows, bool interleaved, cudaStream_t
     };
     const int vec = fits(8) ? 8 : fits(4) ? 4 : (interleaved || fits(2)) ? 2 : 1;
     const bool wide = fits(vec);
-    const int pieces = (a.heads + 2 * a.kv_heads) * a.dim / vec;
-    const int threads = pieces >= 256 ? 256 : (pieces + 31) / 32 * 32;
-    const int sms = runtime().num_sms;
-    // two rows per CTA once there are several CTAs for every SM: their loads and tables overlap (TWO_ROWS figures at the top)
-    const bool two = rows >= 8 * sms;
-    auto go = [&](auto kernel, int per_cta) {
+    auto go = [&](auto kernel, int grid, int threads, size_t smem, const auto& args) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(ceil_div(rows, per_cta));
+        cfg.gridDim = dim3(grid);
         cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = static_cast<size_t>(per_cta) * a.half * sizeof(float2);
+        cfg.dynamicSmemBytes = smem;
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = runtime().pdl ? 1 : 0;
-        CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, a, rows));
+        CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args));
     };
+    const int pieces = (a.heads + 2 * a.kv_heads) * a.dim / vec;
+    const int sms = runtime().num_sms, row_bytes = (a.heads + 2 * a.kv_heads) * a.dim * 2;
+    // Rings where every SM has eight rows, or three groups of several short rows: 8192 rows of 32 + 2 * 8 heads of 128 35.5 us (one CTA per row 45.0),
+    // of 16 + 2 * 4 interleaved 19.1 (27.5), 2000 rows of 15 + 2 * 5 heads of 80 6.8 (7.3), 8000 rows of 4 + 2 heads of 64 6.3 (9.8); but
+    // 1000 rows of 32 + 2 * 8 heads of 128 7.8 (7.4), 1000 of 12 + 2 * 4 heads of 64 3.8 (3.2).
+    const int group = std::max(1, std::min({RING_GROUP_BYTES / row_bytes, a.half > 0 ? 256 / a.half : RING_MAX_GROUP, RING_MAX_GROUP}));
+    const int groups = ceil_div(rows, group);
+    if (vec == 8 && (!interleaved || a.dim % 16 == 0) && row_bytes <= RING_MAX_ROW_BYTES && groups >= (group > 1 ? 3 : 8) * sms) {
+        RingArgs g;
+        g.a = a;
+        g.rows = rows;
+        g.row_bytes = row_bytes;
+        g.group = group;
+        g.groups = groups;
+        g.turned = interleaved ? a.dim / 16 : a.half / 8;
+        g.copied = interleaved ? 0 : (a.dim - 2 * a.half) / 8;
+        const int all = a.heads + a.kv_heads;
+        g.by_items.set(std::max(1, all * g.turned));
+        g.by_turned.set(std::max(1, g.turned));
+        g.by_copies.set(std::max(1, all * g.copied));
+        g.by_copied.set(std::max(1, g.copied));
+        g.by_values.set(std::max(1, a.kv_heads * a.dim / 8));
+        const int smem = RING_STAGES * g.group * row_bytes + 2 * g.group * 2 * padded(a.half) * static_cast<int>(sizeof(float));
+        static const bool allowed = [] {   // the library runs on one device
+            for (auto* kernel : {rotary_ring_kernel<true>, rotary_ring_kernel<false>}) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
+            return true;
+        }();
+        (void)allowed;
+        const int per_sm = std::max(1, std::min(RING_CTAS, 227 * 1024 / (smem + 1280)));
+        const int grid = std::min(g.groups, per_sm * sms);
+        if (interleaved) go(rotary_ring_kernel<true>, grid, 256, smem, g);
+        else go(rotary_ring_kernel<false>, grid, 256, smem, g);
+        return;
+    }
+    const int threads = pieces >= 256 ? 256 : (pieces + 31) / 32 * 32;
     if (interleaved) {
-        if (vec == 8 && two) go(rotary_kernel<8, true, true, 2>, 2);
-        else if (vec == 8) go(rotary_kernel<8, true, true, 1>, 1);
-        else if (vec == 4) go(rotary_kernel<4, true, true, 1>, 1);
-        else if (wide) go(rotary_kernel<2, true, true, 1>, 1);
-        else go(rotary_kernel<2, true, false, 1>, 1);
+        if (vec == 8) go(rotary_kernel<8, true, true>, rows, threads, 0, a);
+        else if (vec == 4) go(rotary_kernel<4, true, true>, rows, threads, 0, a);
+        else if (wide) go(rotary_kernel<2, true, true>, rows, threads, 0, a);
+        else go(rotary_kernel<2, true, false>, rows, threads, 0, a);
     } else {
-        if (vec == 8 && two) go(rotary_kernel<8, false, true, 2>, 2);
-        else if (vec == 8) go(rotary_kernel<8, false, true, 1>, 1);
-        else if (vec == 4) go(rotary_kernel<4, false, true, 1>, 1);
-        else if (vec == 2) go(rotary_kernel<2, false, true, 1>, 1);
-        else go(rotary_kernel<1, false, false, 1>, 1);
+        if (vec == 8) go(rotary_kernel<8, false, true>, rows, threads, 0, a);
+        else if (vec == 4) go(rotary_kernel<4, false, true>, rows, threads, 0, a);
+        else if (vec == 2) go(rotary_kernel<2, false, true>, rows, threads, 0, a);
+        else go(rotary_kernel<1, false, false>, rows, threads, 0, a);
     }
 }

@@ -1,8 +1,8 @@
 // One row of an 8-bit linear layer, sm_100a:  y[N] = (q . W_n) * scale * scale_n + bias_n, with q made of the row inside the launch (w8a8_rows.cuh).
 //
 // Bound: the weights' bytes from HBM.  One CTA of 16 warps per SM makes the integers of the row once, in shared memory.  Weights come through
-// asynchronous 16-byte copies into slots of shared memory that one lane writes and reads (no barriers): 96 KB per SM are in flight, the first of
-// them before the wait for the predecessor and while the integers are made, and no registers hold them, so that the next launch's CTAs fit
+// asynchronous 16-byte copies into slots of shared memory that one lane writes and reads (no barriers): 96 or 128 KB per SM are in flight, the
+// first of them before the wait for the predecessor and while the integers are made, and no registers hold them, so that the next launch's CTAs fit
 // beside this one's and its weights are on their way before this one ends.  Eight lanes read 128 consecutive bytes of one weight row, a
 // warp four rows (512 bytes) per k-block; S warps share the k-blocks of a group of rows and meet in shared memory, S chosen so
 // that the groups divide evenly among the SMs.  dp4a sums four products: 4 of them per 16 bytes, far below what the lanes can do at
@@ -16,10 +16,15 @@ namespace w8 {
 namespace {
 
 constexpr int WARPS = 16, THREADS = WARPS * 32;
-constexpr int SLOTS = 12;                             // 16-byte copies per lane in flight
 constexpr int MAX_STEP = 2;                           // k-blocks per step: 2, of gate/up pairs 1
-constexpr int RING_BYTES = SLOTS * THREADS * 16;
-constexpr int MAX_SMEM = RING_BYTES + MAX_COLS + MAX_STEP * BLOCK_COLS;
+// 16-byte copies per lane in flight.  Twelve, so that the next launch's CTA fits beside this one's; or, where the SM's share of the weights is more
+// than sixteen hold, sixteen and the SM alone: (1 x 4096 x 4096, 1 x 16384 x 4096, 1 x 4096 x 32768) 4.84, 14.5, 23.1 us with twelve, 5.61, 13.2,
+// 21.5 with sixteen; twenty and more gain nothing.
+template <bool DEEP>
+constexpr int SLOTS = DEEP ? 16 : 12;
+template <bool DEEP>
+constexpr int RING_BYTES = SLOTS<DEEP> * THREADS * 16;
+constexpr int MAX_DYNAMIC_SMEM = 232448 - 2048;       // the static arrays are smaller than that
 
 struct OneRowArgs {
     RowSource src;
@@ -39,10 +44,10 @@ __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
 }
 
 // Lets its successor start behind its own wait, so that the successor's weights are older than this launch's predecessor.
-template <Source SRC, int VEC, bool GATED>
-__global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs a) {
+template <Source SRC, int VEC, bool GATED, bool DEEP>
+__global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const OneRowArgs a) {
     constexpr int SETS = GATED ? 2 : 1;               // gate and up rows of the same features
-    constexpr int STEP = MAX_STEP / SETS, PER_STEP = STEP * SETS, DEPTH = SLOTS / PER_STEP;   // copies of a lane; steps in flight
+    constexpr int STEP = MAX_STEP / SETS, PER_STEP = STEP * SETS, DEPTH = SLOTS<DEEP> / PER_STEP;   // copies of a lane; steps in flight
     constexpr int KEEP = HAS_NORM<SRC> ? 2 : 4;       // vectors that a thread keeps of the row
     constexpr int TILE_UNITS = (GATED ? TILE_ROWS / 2 : TILE_ROWS) / 4;
     extern __shared__ __align__(16) uint8_t smem[];   // ring, then the integers
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
     grid_dep_trigger();
 
     // ---- the row's integers
-    int8_t* q = reinterpret_cast<int8_t*>(smem + RING_BYTES);
+    int8_t* q = reinterpret_cast<int8_t*>(smem + RING_BYTES<DEEP>);
     uint32_t top = 0u;
     float ss = 0.f;
     Values<SRC, VEC> kept[KEEP];
@@ -205,19 +210,20 @@ __global__ void __launch_bounds__(THREADS, 2) one_row_s8_kernel(const OneRowArgs
     ptx::cp_async_wait<0>();
 }
 
-template <Source SRC, int VEC, bool GATED>
-void run(const OneRowArgs& a, int grid, size_t smem, cudaStream_t s) {
+template <Source SRC, int VEC, bool GATED, bool DEEP>
+void run(const OneRowArgs& a, int grid, size_t ints, cudaStream_t s) {
     static const bool allowed = [] {   // the library runs on one device
-        CUDA_CHECK(cudaFuncSetAttribute(one_row_s8_kernel<SRC, VEC, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM));
+        CUDA_CHECK(cudaFuncSetAttribute(one_row_s8_kernel<SRC, VEC, GATED, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_DYNAMIC_SMEM));
         return true;
     }();
     (void)allowed;
-    launch(one_row_s8_kernel<SRC, VEC, GATED>, grid, THREADS, smem, s, 1, true, a);
+    launch(one_row_s8_kernel<SRC, VEC, GATED, DEEP>, grid, THREADS, RING_BYTES<DEEP> + ints, s, 1, true, a);
 }
 template <Source SRC, bool GATED>
-void run(const OneRowArgs& a, int grid, size_t smem, bool vec, cudaStream_t s) {
-    if (vec) run<SRC, 8, GATED>(a, grid, smem, s);
-    else run<SRC, 1, GATED>(a, grid, smem, s);
+void run(const OneRowArgs& a, int grid, size_t ints, bool vec, bool deep, cudaStream_t s) {
+    if (!vec) run<SRC, 1, GATED, false>(a, grid, ints, s);
+    else if (deep) run<SRC, 8, GATED, true>(a, grid, ints, s);
+    else run<SRC, 8, GATED, false>(a, grid, ints, s);
 }
 
 }  // namespace
@@ -244,12 +250,13 @@ void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const b
         }
     }
     const int grid = std::min(sms, ceil_div(a.units, WARPS / a.share));
-    const size_t smem = RING_BYTES + static_cast<size_t>(all_steps) * step_blocks * BLOCK_COLS;
+    const size_t ints = static_cast<size_t>(all_steps) * step_blocks * BLOCK_COLS;
     const bool vec = rows_in_vectors(src, K);
-    if (src.x32 != nullptr) run<SRC_F32, false>(a, grid, smem, vec, s);
-    else if (src.norm == nullptr) gated ? run<SRC_PLAIN, true>(a, grid, smem, vec, s) : run<SRC_PLAIN, false>(a, grid, smem, vec, s);
-    else if (src.delta == nullptr) gated ? run<SRC_NORM, true>(a, grid, smem, vec, s) : run<SRC_NORM, false>(a, grid, smem, vec, s);
-    else gated ? run<SRC_ADD_NORM, true>(a, grid, smem, vec, s) : run<SRC_ADD_NORM, false>(a, grid, smem, vec, s);
+    const bool deep = static_cast<size_t>(w.tiles) * w.kblocks * BLOCK_BYTES > static_cast<size_t>(sms) * RING_BYTES<true> && RING_BYTES<true> + ints <= MAX_DYNAMIC_SMEM;
+    if (src.x32 != nullptr) run<SRC_F32, false>(a, grid, ints, vec, deep, s);
+    else if (src.norm == nullptr) gated ? run<SRC_PLAIN, true>(a, grid, ints, vec, deep, s) : run<SRC_PLAIN, false>(a, grid, ints, vec, deep, s);
+    else if (src.delta == nullptr) gated ? run<SRC_NORM, true>(a, grid, ints, vec, deep, s) : run<SRC_NORM, false>(a, grid, ints, vec, deep, s);
+    else gated ? run<SRC_ADD_NORM, true>(a, grid, ints, vec, deep, s) : run<SRC_ADD_NORM, false>(a, grid, ints, vec, deep, s);
 }
 
 }  // namespace w8
