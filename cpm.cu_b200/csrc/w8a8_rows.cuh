@@ -99,6 +99,14 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
     return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
 }
 
+// Eight values of a vector that has one near a border, or of a row of tiny values.  Out of line: it is rarely run, and a launch begins by fetching its
+// instructions.
+__device__ __noinline__ uint2 exact8(float v0, float v1, float v2, float v3, float v4, float v5, float v6, float v7, float c127, float top, float inv) {
+    RowRound r(0u);
+    r.c127 = c127; r.top = top; r.inv = inv;
+    return make_uint2(pack4(r.exact(v0), r.exact(v1), r.exact(v2), r.exact(v3)), pack4(r.exact(v4), r.exact(v5), r.exact(v6), r.exact(v7)));
+}
+
 template <int VEC>
 __device__ __forceinline__ void store_ints(int8_t* q, const RowRound& round, const float (&v)[VEC]) {
     if constexpr (VEC == 8) {
@@ -106,8 +114,7 @@ __device__ __forceinline__ void store_ints(int8_t* q, const RowRound& round, con
         float near = 0.f;
         if (round.plain) w = make_uint2(round.four(v, near), round.four(v + 4, near));
         if (round.finite && (near > RowRound::NEAR || !round.plain)) {
-            w = make_uint2(pack4(round.exact(v[0]), round.exact(v[1]), round.exact(v[2]), round.exact(v[3])),
-                           pack4(round.exact(v[4]), round.exact(v[5]), round.exact(v[6]), round.exact(v[7])));
+            w = exact8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], round.c127, round.top, round.inv);
         }
         *reinterpret_cast<uint2*>(q) = w;
     } else {
