@@ -104,9 +104,33 @@ __device__ __forceinline__ void load16(uint32_t taddr, int (&r)[16]) {
     ptx::tmem_ld16(taddr, reinterpret_cast<uint32_t*>(r));
 }
 
-// bf16 rows from 16 tokens' values; y rows are ldy apart (64 bits)
+// 16 tokens' values of 32 features to rows of y, ldy apart (64 bits).  A lane has one feature: through `buf` eight features are one 16-byte store, where
+// rows and widths allow that (vec).
 __device__ __forceinline__ void store16(bf16* y, long long ldy, int N, long long y_row, int cnt, int n0, const float (&v)[16], uint8_t* buf, int lane, bool vec) {
-    gemm::store_tokens<16>(y + y_row * ldy, static_cast<int>(ldy), N, 0, cnt, n0, v, buf, lane, vec);
+    bf16* to = y + y_row * ldy;
+    if (vec) {
+        uint16_t* b = reinterpret_cast<uint16_t*>(buf);
+        __syncwarp();   // the buffer's earlier contents have been read
+#pragma unroll
+        for (int c = 0; c < 16; c += 2) {
+            const uint32_t two = two_bf16(v[c], v[c + 1]);
+            b[c * 32 + lane] = static_cast<uint16_t>(two);
+            b[(c + 1) * 32 + lane] = static_cast<uint16_t>(two >> 16);
+        }
+        __syncwarp();
+        const int f = n0 + (lane & 3) * 8;
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+            const int c = k + (lane >> 2);
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + c * 64 + (lane & 3) * 16);
+            if (c < cnt && f < N) *reinterpret_cast<uint4*>(to + c * ldy + f) = w;
+        }
+    } else if (n0 + lane < N) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            if (c < cnt) to[c * ldy + n0 + lane] = __float2bfloat16(v[c]);
+        }
+    }
 }
 
 // silu(gate) * up of a whole tile: lanes 0-63 hold the gate sums of 64 features, 64-127 the up sums of the same ones.  Warps q and q + 2 hand

@@ -18,7 +18,7 @@ namespace {
 // VEC elements as they lie in memory; WIDE: in one access
 template <int VEC, bool WIDE>
 struct Elems {
-    bf16 e[VEC];
+    alignas(VEC > 1 ? 4 : 2) bf16 e[VEC];
     __device__ __forceinline__ void load(const bf16* p) {
         if constexpr (!WIDE) {
 #pragma unroll
@@ -37,6 +37,24 @@ struct Elems {
     }
 };
 
+// Two pairs (a.lo, b.lo), (a.hi, b.hi) of packed values.  Unpacked by shifts and packed by the pair: conversions of single values go through the unit of
+// the special functions, a quarter of the rate.
+__device__ __forceinline__ float low(uint32_t two) { return __uint_as_float(two << 16); }
+__device__ __forceinline__ float high(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
+__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ void turn_two(uint32_t& a, uint32_t& b, const float* cs, const float* sn) {
+    const uint32_t x = a, y = b;
+    a = two_bf16(fmaf(low(x), cs[0], -(low(y) * sn[0])), fmaf(high(x), cs[1], -(high(y) * sn[1])));
+    b = two_bf16(fmaf(low(y), cs[0], low(x) * sn[0]), fmaf(high(y), cs[1], high(x) * sn[1]));
+}
+// One pair (lo, hi)
+__device__ __forceinline__ void turn_within(uint32_t& a, float cs, float sn) {
+    const uint32_t x = a;
+    a = two_bf16(fmaf(low(x), cs, -(high(x) * sn)), fmaf(high(x), cs, low(x) * sn));
+}
 __device__ __forceinline__ void turn(bf16& a, bf16& b, float cs, float sn) {
     const float x = __bfloat162float(a), y = __bfloat162float(b);
     a = __float2bfloat16(fmaf(x, cs, -(y * sn)));
@@ -81,12 +99,17 @@ struct Piece {
         if (INTERLEAVED && first >= half) return;
         take<N>(table + first, cs);
         take<N>(table + padded(half) + first, sn);
+        if constexpr (VEC == 1) {
+            turn(lo.e[0], hi.e[0], cs[0], sn[0]);
+        } else {
+            uint32_t *a = reinterpret_cast<uint32_t*>(lo.e), *b = reinterpret_cast<uint32_t*>(hi.e);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            if constexpr (INTERLEAVED) {
-                if (first + j < half) turn(lo.e[2 * j], lo.e[(2 * j + 1) % VEC], cs[j], sn[j]);
-            } else {
-                turn(lo.e[j], hi.e[j], cs[j], sn[j]);
+            for (int j = 0; j < VEC / 2; ++j) {
+                if constexpr (INTERLEAVED) {
+                    if (first + j < half) turn_within(a[j], cs[j], sn[j]);
+                } else {
+                    turn_two(a[j], b[j], cs + 2 * j, sn + 2 * j);
+                }
             }
         }
     }

@@ -63,6 +63,15 @@ void launch_product(const Product& p, cudaStream_t s);
 // one row, straight from its source
 void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const bf16* bias, bf16* y, float* act, cudaStream_t s);
 
+// bf16 to fp32 and back by the pair: conversions of single values go through the unit of the special functions, a quarter of the rate, and bound a
+// pass over rows.
+__device__ __forceinline__ float low(uint32_t two) { return __uint_as_float(two << 16); }
+__device__ __forceinline__ float high(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
+__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+
 // The launchers below belong to streams of the caller's choice: they do not count in the library stream's order of launches.
 template <typename... KArgs, typename... Args>
 void launch(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t s, int cluster, bool programmatic, Args&&... args) {

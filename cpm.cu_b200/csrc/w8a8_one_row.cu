@@ -123,14 +123,14 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const
     top = block_max(top, sh_top);
     float factor = 1.f;
     if constexpr (HAS_NORM<SRC>) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
-    const RowRound round8(top);
+    const RowRound round8(top, HAS_NORM<SRC>, SRC != SRC_F32);
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
         const int c = (threadIdx.x + j * THREADS) * VEC;
         if (c < a.K) {
             float v[VEC];
             kept[j].values(v);
-            store_ints<VEC>(q + c, round8, v);
+            store_ints<HAS_NORM<SRC>, VEC>(q + c, round8, v);
         }
     }
     for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const
         r.fetch(a.src, 0, a.K, c);
         r.combine(a.src, 0, a.K, c, false, known, squares);
         r.values(v);
-        store_ints<VEC>(q + c, round8, v);
+        store_ints<HAS_NORM<SRC>, VEC>(q + c, round8, v);
     }
     for (int c = a.K + threadIdx.x; c < (kblocks + STEP - 1) / STEP * STEP * BLOCK_COLS; c += THREADS) q[c] = 0;
     const float scale = RowRound::scale(top, factor);

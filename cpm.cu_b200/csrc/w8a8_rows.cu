@@ -25,7 +25,7 @@ struct QuantizeArgs {
 // VPT > 0: a thread's VPT vectors of 8 stay in registers; 0: the row is read twice, VEC elements at a time.
 // Lets its successor start behind its own wait: a product may then fetch weights, which are older than this launch's predecessor.
 template <Source SRC, int VPT, int VEC>
-__global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const QuantizeArgs a) {
+__global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 1024 : VPT == 4 ? 512 : 256) quantize_kernel(const QuantizeArgs a) {
     __shared__ uint32_t sh_top[32];
     __shared__ float sh_sum[32];
     const size_t row = blockIdx.x;
@@ -60,12 +60,12 @@ __global__ void __launch_bounds__(VPT > 0 ? 512 : 256) quantize_kernel(const Qua
     top = block_max(top, sh_top);
     float factor = 1.f;
     if constexpr (HAS_NORM<SRC>) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
-    const RowRound round(top);
+    const RowRound round(top, HAS_NORM<SRC>, SRC != SRC_F32);
     int8_t* q = a.q + row * a.ldq;
     auto finish = [&](const Values<SRC, VEC>& r, int c) {
         float v[VEC];
         r.values(v);
-        store_ints<VEC>(q + c, round, v);
+        store_ints<HAS_NORM<SRC>, VEC>(q + c, round, v);
     };
     if constexpr (VPT > 0) {
 #pragma unroll
@@ -90,12 +90,21 @@ template <Source SRC>
 void run_quantize(const QuantizeArgs& a, int rows, bool vec, cudaStream_t s) {
     auto go = [&](void (*kernel)(QuantizeArgs), int threads) { launch(kernel, rows, threads, 0, s, 1, true, a); };
     if (!vec) { go(quantize_kernel<SRC, 0, 1>, 256); return; }
-    // Threads for one vector each up to 256, then up to four vectors each, then up to 512 threads
-    const int vectors = a.K / 8;
-    const int round32 = (vectors + 31) / 32 * 32;
+    const int vectors = a.K / 8, round32 = (vectors + 31) / 32 * 32;
+    if (rows <= 2 * runtime().num_sms) {
+        // few rows: a row's own time counts, and the fewer vectors a thread has the shorter it is (60 x 16384: 4.2 us with eight on 256 threads, 2.9
+        // with two on 1024)
+        if (vectors <= 1024) go(quantize_kernel<SRC, 1, 8>, round32);
+        else if (vectors <= 2048) go(quantize_kernel<SRC, 2, 8>, 1024);
+        else go(quantize_kernel<SRC, 0, 8>, 256);
+        return;
+    }
+    // many rows: several CTAs beside one another on an SM
     if (vectors <= 256) go(quantize_kernel<SRC, 1, 8>, round32);
     else if (vectors <= 512) go(quantize_kernel<SRC, 2, 8>, 256);
-    else if (vectors <= 2048) go(quantize_kernel<SRC, 4, 8>, vectors <= 1024 ? 256 : 512);
+    else if (vectors <= 1024) go(quantize_kernel<SRC, 4, 8>, 256);
+    else if (vectors <= 2048 && SRC == SRC_PLAIN) go(quantize_kernel<SRC_PLAIN, 8, 8>, 256);
+    else if (vectors <= 2048) go(quantize_kernel<SRC, 4, 8>, 512);
     else go(quantize_kernel<SRC, 0, 8>, 256);
 }
 
@@ -117,7 +126,7 @@ __global__ void pack_kernel(const int8_t* __restrict__ q, const float* __restric
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     auto at = [&](int k) { return c + k < K ? static_cast<int>(src[k]) : 0; };
-                    w[j] = pack4(at(4 * j), at(4 * j + 1), at(4 * j + 2), at(4 * j + 3));
+                    w[j] = RowRound::low_bytes(at(4 * j), at(4 * j + 1), at(4 * j + 2), at(4 * j + 3));
                 }
                 v = make_uint4(w[0], w[1], w[2], w[3]);
             }

@@ -42,21 +42,30 @@ __device__ __forceinline__ float block_total(float v, float* sh) {
 }
 
 // ---------------------------------------------------------------- rounding
-// q = round(127 v / top) to nearest, even at ties, exactly.  v * k, k = 127 / top rounded, is off by less than 127 * 2^-23 from 127 v / top, so that
-// its nearest integer is the one, unless it lies within NEAR of the middle between two; a vector with such a value is rounded again by exact().
-// There v and top are scaled by a power of two so that nothing over- or underflows, an estimate is at most one off, and the rest
-// 127 v - q top, which fp32 holds exactly for v of up to 17 significant bits (bf16 values and products of two of them), decides.  (Rows of
-// fp32 values round the middle as their fp32 rests have it.)
+// q = round(127 v / top) to nearest, even at ties, exactly, for bf16 values and products of two of them.
+// Let v and top be integers m and M times powers of two, m, M < 2^16, and r = 127 v / top.  Where r is not half-way between two integers it is at least
+// r / (254 m) > r 2^-23.98 away from there (the difference is a fraction with that denominator), and v k, k = 127 / top correctly rounded, is off by
+// r 2^-24 at most: one fused multiply-add to a number whose unit is 1 rounds r itself.  Half-way lie (1) |v| = top / 2, r = 63.5, which
+// has to become 64; where k was rounded down it would become 63, so that k is taken one step up (bf16 values: m < 2^8, there is room) or v is made a
+// little larger (products); and (2) values of rows whose M is a multiple of 127.  Those rows, and rows of tiny values, go through exact(): v and top
+// scaled by a power of two so that nothing over- or underflows, an estimate that is at most one off, and the rest 127 v - q top, which fp32 holds
+// exactly, decides.  (fp32 rows round 127 v / top as the fused product has it.)
 struct RowRound {
-    float k, c127, top, inv;
-    bool finite, plain;   // plain: k is exact enough; not for rows of tiny values
+    float k, half, c127, top, inv;
+    bool finite, plain;   // plain: k rounds the row
     static constexpr float MAGIC = 12582912.f;       // 1.5 * 2^23: v + MAGIC has round(v) in its low byte
-    static constexpr float NEAR = 0.49996f;
-    __device__ __forceinline__ explicit RowRound(uint32_t bits) {
+    __device__ __forceinline__ RowRound() {}
+    // bits: of the row's largest magnitude; products: of two bf16 values; ties: half-way values are to become even (not of fp32 rows)
+    __device__ __forceinline__ RowRound(uint32_t bits, bool products, bool ties) {
         finite = bits < 0x7f800000u;
-        plain = finite && bits >= 0x10000000u;                   // 2^-95
         const float v = __uint_as_float(bits);
+        plain = finite && bits >= 0x10000000u && !(ties && ((bits & 0x7fffffu) | 0x800000u) % 127u == 0u);   // 2^-95
         k = plain ? 127.f / v : 0.f;
+        half = __uint_as_float(0x7f800000u);                     // no value's magnitude
+        if (plain && ties && fmaf(k, v, -127.f) < 0.f) {
+            if (products) half = 0.5f * v;
+            else k = __uint_as_float(__float_as_uint(k) + 1u);
+        }
         int e = static_cast<int>(bits >> 23) - 127;              // v is in [2^e, 2^(e+1)), or below where it is subnormal
         e = e < -119 ? -119 : e;
         const float c = __uint_as_float(static_cast<uint32_t>(127 - (e > 126 ? 126 : e)) << 23);
@@ -65,29 +74,34 @@ struct RowRound {
         top = v * c;
         inv = some ? 1.f / top : 0.f;
     }
-    __device__ __forceinline__ int exact(float v) const {
+    // a number whose low byte is the integer
+    __device__ __forceinline__ uint32_t exact(float v) const {
         const float p = v * c127;
-        float r = rintf(p * inv);
-        const float rest = fmaf(-r, top, p);
-        const float twice = 2.f * fabsf(rest);
-        if (twice > top || (twice == top && (static_cast<int>(r) & 1))) r += copysignf(1.f, rest);
-        return static_cast<int>(r);
+        const float y = fmaf(p, inv, MAGIC), r = y - MAGIC;
+        const float rest = fmaf(-r, top, p), twice = 2.f * fabsf(rest);
+        const bool other = twice > top || (twice == top && (__float_as_uint(y) & 1u));
+        return __float_as_uint(other ? y + copysignf(1.f, rest) : y);
     }
-    // four values to four bytes; near: largest distance from an integer so far
-    __device__ __forceinline__ uint32_t four(const float* v, float& near) const {
+    // four values to four bytes
+    __device__ __forceinline__ static uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+    }
+    template <bool PRODUCTS>
+    __device__ __forceinline__ uint32_t four(const float* v) const {
         uint32_t y[4];
-        const f32x2 kk = pair(k, k), magic = pair(MAGIC, MAGIC), minus = pair(-1.f, -1.f);
+        const f32x2 kk = pair(k, k), magic = pair(MAGIC, MAGIC);
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-            const f32x2 x = pair(v[i], v[i + 1]);
-            const f32x2 sum = fma2(x, kk, magic);
-            const float2 off = unpair(fma2(x, kk, fma2(sum, minus, magic)));   // v k - round(v k)
-            near = fmaxf(near, fmaxf(fabsf(off.x), fabsf(off.y)));
-            const float2 f = unpair(sum);
+            float a = v[i], b = v[i + 1];
+            if constexpr (PRODUCTS) {
+                if (fabsf(a) == half) a *= 1.000001f;
+                if (fabsf(b) == half) b *= 1.000001f;
+            }
+            const float2 f = unpair(fma2(pair(a, b), kk, magic));
             y[i] = __float_as_uint(f.x);
             y[i + 1] = __float_as_uint(f.y);
         }
-        return __byte_perm(__byte_perm(y[0], y[1], 0x0040), __byte_perm(y[2], y[3], 0x0040), 0x5410);
+        return low_bytes(y[0], y[1], y[2], y[3]);
     }
     // the row's scale: NaN for a row with an infinity or a NaN, so that its outputs are NaN
     __device__ __forceinline__ static float scale(uint32_t bits, float factor) {
@@ -95,27 +109,20 @@ struct RowRound {
     }
 };
 
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return (a & 0xff) | (b & 0xff) << 8 | (c & 0xff) << 16 | static_cast<uint32_t>(d) << 24;
-}
-
-// Eight values of a vector that has one near a border, or of a row of tiny values.  Out of line: it is rarely run, and a launch begins by fetching its
-// instructions.
+// Out of line: few rows need it, and a launch begins by fetching its instructions.
 __device__ __noinline__ uint2 exact8(float v0, float v1, float v2, float v3, float v4, float v5, float v6, float v7, float c127, float top, float inv) {
-    RowRound r(0u);
+    RowRound r;
     r.c127 = c127; r.top = top; r.inv = inv;
-    return make_uint2(pack4(r.exact(v0), r.exact(v1), r.exact(v2), r.exact(v3)), pack4(r.exact(v4), r.exact(v5), r.exact(v6), r.exact(v7)));
+    return make_uint2(RowRound::low_bytes(r.exact(v0), r.exact(v1), r.exact(v2), r.exact(v3)),
+                      RowRound::low_bytes(r.exact(v4), r.exact(v5), r.exact(v6), r.exact(v7)));
 }
 
-template <int VEC>
+template <bool PRODUCTS, int VEC>
 __device__ __forceinline__ void store_ints(int8_t* q, const RowRound& round, const float (&v)[VEC]) {
     if constexpr (VEC == 8) {
         uint2 w = make_uint2(0u, 0u);
-        float near = 0.f;
-        if (round.plain) w = make_uint2(round.four(v, near), round.four(v + 4, near));
-        if (round.finite && (near > RowRound::NEAR || !round.plain)) {
-            w = exact8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], round.c127, round.top, round.inv);
-        }
+        if (round.plain) w = make_uint2(round.four<PRODUCTS>(v), round.four<PRODUCTS>(v + 4));
+        else if (round.finite) w = exact8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], round.c127, round.top, round.inv);
         *reinterpret_cast<uint2*>(q) = w;
     } else {
         *q = static_cast<int8_t>(round.finite ? round.exact(v[0]) : 0);
@@ -128,7 +135,19 @@ __device__ __forceinline__ void store_ints(int8_t* q, const RowRound& round, con
 template <Source SRC, int VEC>
 struct Values {
     using T = typename std::conditional<SRC == SRC_F32, float, bf16>::type;
-    struct alignas(VEC == 8 ? 16 : sizeof(T)) Block { T e[VEC]; };
+    struct alignas(VEC == 8 ? 16 : sizeof(T)) Block {
+        T e[VEC];
+        __device__ __forceinline__ float at(int i) const {
+            if constexpr (SRC == SRC_F32) {
+                return e[i];
+            } else if constexpr (VEC == 8) {
+                const uint32_t two = reinterpret_cast<const uint32_t*>(e)[i >> 1];
+                return i & 1 ? high(two) : low(two);
+            } else {
+                return __bfloat162float(e[i]);
+            }
+        }
+    };
     Block t, d, w;
     float p[VEC];
     __device__ __forceinline__ static const T* base(const RowSource& s) {
@@ -149,8 +168,14 @@ struct Values {
     // `write`: stores the residual sum
     __device__ __forceinline__ void combine(const RowSource& s, size_t row, int K, int c, bool write, uint32_t& top, float& ss) {
         if constexpr (SRC == SRC_ADD_NORM) {
+            if constexpr (VEC == 8) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) t.e[e] = __float2bfloat16(fmaf(__bfloat162float(d.e[e]), s.delta_scale, __bfloat162float(t.e[e])));
+                for (int i = 0; i < 4; ++i) {
+                    reinterpret_cast<uint32_t*>(t.e)[i] = two_bf16(fmaf(d.at(2 * i), s.delta_scale, t.at(2 * i)), fmaf(d.at(2 * i + 1), s.delta_scale, t.at(2 * i + 1)));
+                }
+            } else {
+                t.e[0] = __float2bfloat16(fmaf(d.at(0), s.delta_scale, t.at(0)));
+            }
             if (write) *reinterpret_cast<Block*>(s.total + row * K + c) = t;
         }
         if constexpr (SRC == SRC_PLAIN && VEC == 8) {   // two magnitudes at a time, as 16-bit patterns
@@ -163,10 +188,10 @@ struct Values {
             float m = 0.f;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                float v = to_float(t.e[e]);
+                float v = t.at(e);
                 if constexpr (HAS_NORM<SRC>) {
                     ss = fmaf(v, v, ss);
-                    v *= to_float(w.e[e]);
+                    v *= w.at(e);
                     p[e] = v;
                 }
                 m = max_magnitude(m, v);
@@ -178,7 +203,7 @@ struct Values {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             if constexpr (HAS_NORM<SRC>) v[e] = p[e];
-            else v[e] = to_float(t.e[e]);
+            else v[e] = t.at(e);
         }
     }
 };
