@@ -681,51 +681,43 @@ Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
             }
         }
     }
-    if (M > 64) {
-        // Cycles of a k-block, measured in long products (operands from L2 bound the small tiles), and of a tile's way out of tensor memory, of
-        // which a launch shows the last one.
-        struct Kind { int mt; bool pair; int block, out; };
-        static const Kind kinds[] = {{64, false, 480, 1500}, {128, false, 640, 3000}, {256, false, 960, 6000}, {256, true, 640, 6000}};
-        long long best = -1;
-        for (const Kind& k : kinds) {
-            if (k.pair && (tiles % 2 != 0 || M <= 128)) continue;
-            const int m_tiles = ceil_div(M, k.mt);
-            const long long n = static_cast<long long>(k.pair ? tiles / 2 : tiles) * m_tiles, workers = k.pair ? sms / 2 : sms;
-            // blocks of the busiest worker: whole tiles, or even pieces of at least eight blocks
-            const long long blocks = gated || n * kblocks < workers * 8 ? (n + workers - 1) / workers * kblocks : (n * kblocks + workers - 1) / workers;
-            const long long cost = blocks * k.block + k.out;
+    // Otherwise the kind of tile, and whether the tiles of the last wave are cut into equal pieces, that is expected to end first.  In cycles, from runs of all
+    // kinds over 23 shapes: a k-block; what a launch shows of a tile's way out of tensor memory (beyond that of 64 tokens); and the sum over a cut
+    // tile's pieces, as far as whole tiles behind it do not hide it.  Rows x columns x outputs, whole tiles of 64, 128, 256 and pairs, and the best cut
+    // one: 300 x 4096 x 4096 22.5, 13.8, 16.0, 16.1 (21.3) us; 1000 x 4096 x 4608 39.7, 23.0, 16.1, 16.7 (27.7); 2048 x 4096 x 4096 67.4, 42.3,
+    // 26.6, 26.6 (39.9); 128 x 16384 x 4096 38.3, 38.6, 44.4, - (26.6).
+    struct Kind { int mt; bool pair; int block, out, sum; };
+    const Kind kinds[] = {{std::min(d.mt, 64), false, 500, 0, 14000}, {128, false, 560, 1100, 20000}, {256, false, 580, 3600, 45000}, {256, true, 540, 6000, 45000}};
+    bool cut = false;
+    long long best = -1;
+    for (const Kind& k : kinds) {
+        if ((k.mt > 64 && M <= 64) || (k.pair && (tiles % 2 != 0 || M <= 128))) continue;
+        const int m_tiles = ceil_div(M, k.mt);
+        const long long n = static_cast<long long>(k.pair ? tiles / 2 : tiles) * m_tiles, workers = k.pair ? sms / 2 : sms, waves = n / workers;
+        for (int c = 0; c <= (gated ? 0 : 1); ++c) {                                 // gate/up tiles: the activation needs complete sums
+            if (c == 1 && (n % workers == 0 || n % workers * kblocks < workers * 4)) continue;   // pieces of four blocks at least
+            long long cost = (c == 0 ? (n + workers - 1) / workers * kblocks : (n * kblocks + workers - 1) / workers) * k.block + k.out;
+            if (c == 1) cost += 6000 + std::max<long long>(0, k.sum - waves * kblocks * k.block);
             if (best < 0 || cost < best) {
                 best = cost;
                 d.mt = k.mt;
                 d.pair = k.pair;
                 d.m_tiles = m_tiles;
+                cut = c == 1;
             }
         }
     }
     const int n_tiles = d.pair ? tiles / 2 : tiles, most = d.pair ? sms / 2 : sms;
     const long long all = static_cast<long long>(n_tiles) * d.m_tiles;
-    if (gated) {
-        // whole tiles only: the activation needs a tile's complete sums
-        d.workers = static_cast<int>(std::min<long long>(all, most));
+    if (!cut) {
+        const long long rounds = (all + most - 1) / most;
+        d.workers = static_cast<int>(std::min<long long>(d.m_tiles == 1 ? (all + rounds - 1) / rounds : most, all));
         d.wave_tiles = static_cast<int>(all);
         d.tail_grid = 1;
         return d;
     }
-    const long long units = all * kblocks;
-    if (d.m_tiles == 1) {
-        // a piece per CTA; whole tiles where those occupy at least three quarters of the SMs for every round
-        const long long rounds = (all + most - 1) / most;
-        if (all >= rounds * most * 3 / 4) {
-            d.workers = static_cast<int>((all + rounds - 1) / rounds);
-            d.wave_tiles = static_cast<int>(all);
-            d.tail_grid = 1;
-        } else {
-            d.workers = static_cast<int>(std::max<long long>(1, std::min<long long>(most, units / 4)));
-        }
-        return d;
-    }
-    d.workers = static_cast<int>(std::max<long long>(1, std::min<long long>(most, units / 4)));
-    gemm::plan_waves(all, kblocks, d.workers, d.wave_tiles, d.tail_grid);
+    d.workers = static_cast<int>(std::max<long long>(1, std::min<long long>(most, all * kblocks / 4)));
+    if (d.m_tiles > 1) gemm::plan_waves(all, kblocks, d.workers, d.wave_tiles, d.tail_grid);
     return d;
 }
 
