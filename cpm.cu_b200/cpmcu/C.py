@@ -158,17 +158,13 @@ def _check(code):
     return code
 
 
-_functions = {}
-
-
 def call(name, *args):
     """Call an extern "C" entry point by name; negative return codes raise RuntimeError."""
-    known = _functions.get(name)
-    if known is None:
-        fn = getattr(load(), name)
-        known = _functions[name] = (fn, fn.restype is _c_int)
-    res = known[0](*args)
-    return _check(res) if known[1] and res < 0 else res
+    fn = getattr(load(), name)
+    res = fn(*args)
+    if fn.restype is _c_int:
+        return _check(res)
+    return res
 
 
 # ---------------------------------------------------------------- reference names
@@ -323,6 +319,11 @@ def profile(on):
     call("cpmcu_profile", int(on), ctypes.cast(ms, _c_void_p), ctypes.cast(cnt, _c_void_p))
     names = ("linear", "attention", "selection", "experts", "routing", "rows", "scan")
     return {n: (ms[i], cnt[i]) for i, n in enumerate(names)}
+
+
+def stream_check(stream=0):
+    """Waits for a stream (a cudaStream_t; 0: the legacy default stream) and raises what the operators of cpmcu.w8a8 and cpmcu.rotary reported."""
+    call("cpmcu_stream_check", stream or None)
 
 
 def last_step_ms():

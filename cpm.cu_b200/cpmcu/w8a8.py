@@ -39,12 +39,21 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
 
 
+_functions = {}
+
+
 def _call(name, index, *args):
     """The entry point on torch's current stream of GPU `index`."""
-    if index != _current_device():
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(C.load(), name)
+    if index == _current_device():
+        code = fn(*args, _raw_stream(index))
+    else:
         with torch.cuda.device(index):
-            return C.call(name, *args, _raw_stream(index))
-    C.call(name, *args, _raw_stream(index))
+            code = fn(*args, _raw_stream(index))
+    if code < 0:
+        raise RuntimeError(C.load().cpmcu_last_error().decode())
 
 
 def quantize(x):
@@ -137,6 +146,8 @@ _NO_NORM = (None, 0.0, None, 1.0, None)
 def _out(out, x, rows, width):
     """(tensor, distance of its rows)"""
     if out is None:
+        if width == x.shape[1] and x.is_contiguous():
+            return torch.empty_like(x), width
         return x.new_empty((rows, width)), width
     _check(out, "out", _BF16, (rows, width), x.device, rows=True)
     return out, _ld(out)

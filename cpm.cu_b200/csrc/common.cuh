@@ -145,6 +145,34 @@ void launch_kernel_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size
     rt.order.launched();
 }
 
+// A launch on a stream of the caller's choice: it does not count in the library stream's order of launches, and several threads may launch at once.
+// programmatic: may start while its predecessor in the stream drains (the kernel waits for it, as all here do).
+template <typename... KArgs, typename... Args>
+void launch_on(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t s, int cluster, bool programmatic, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    Runtime& rt = runtime();
+    if (programmatic && rt.pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
+    __atomic_fetch_add(&rt.launches, 1, __ATOMIC_RELAXED);
+}
+
 // Clusters of `cluster` CTAs of this kernel that the device runs at once (0 when the query fails).  The SMs
 // come in groups that need not be multiples of the cluster size, so this can be fewer than SMs / cluster.
 template <typename... KArgs>

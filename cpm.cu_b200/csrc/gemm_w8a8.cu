@@ -631,14 +631,14 @@ void run(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int
     using C = Cfg<MT, PAIR>;
     static const bool allowed = allow_smem(product_s8_kernel<MT, PAIR>, C::SMEM_BYTES);   // the library runs on one device
     (void)allowed;
-    launch(product_s8_kernel<MT, PAIR>, grid, NUM_THREADS, C::SMEM_BYTES, s, PAIR ? 2 : 1, true, tw, tx, a);
+    launch_on(product_s8_kernel<MT, PAIR>, grid, NUM_THREADS, C::SMEM_BYTES, s, PAIR ? 2 : 1, true, tw, tx, a);
 }
 template <int MT, int CS>
 void run_cluster(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
     using C = ClusterCfg<MT, CS>;
     static const bool allowed = allow_smem(product_s8_cluster_kernel<MT, CS>, C::SMEM_BYTES);
     (void)allowed;
-    launch(product_s8_cluster_kernel<MT, CS>, grid, CLUSTER_THREADS, C::SMEM_BYTES, s, CS, true, tw, tx, a);
+    launch_on(product_s8_cluster_kernel<MT, CS>, grid, CLUSTER_THREADS, C::SMEM_BYTES, s, CS, true, tw, tx, a);
 }
 template <int MT>
 void run_cluster(int cs, const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {

@@ -351,19 +351,7 @@ void launch_rotary(const RotaryArgs& a, int rows, bool interleaved, cudaStream_t
     };
     const int vec = fits(8) ? 8 : fits(4) ? 4 : (interleaved || fits(2)) ? 2 : 1;
     const bool wide = fits(vec);
-    auto go = [&](auto kernel, int grid, int threads, size_t smem, const auto& args) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(grid);
-        cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = s;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = runtime().pdl ? 1 : 0;
-        CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args));
-    };
+    auto go = [&](auto kernel, int grid, int threads, size_t smem, const auto& args) { launch_on(kernel, grid, threads, smem, s, 1, true, args); };
     const int pieces = (a.heads + 2 * a.kv_heads) * a.dim / vec;
     const int sms = runtime().num_sms, row_bytes = (a.heads + 2 * a.kv_heads) * a.dim * 2;
     // Rings where every SM has eight rows, or three groups of several short rows: 8192 rows of 32 + 2 * 8 heads of 128 35.5 us (one CTA per row 45.0),

@@ -14,16 +14,15 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (fn == nullptr) {
+    static const EncodeTiledFn fn = [] {
         void* sym = nullptr;
         cudaDriverEntryPointQueryResult qres;
         CUDA_CHECK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres));
         if (sym == nullptr || qres != cudaDriverEntryPointSuccess) {
             throw std::runtime_error("cpmcu_b200: driver does not export cuTensorMapEncodeTiled");
         }
-        fn = reinterpret_cast<EncodeTiledFn>(sym);
-    }
+        return reinterpret_cast<EncodeTiledFn>(sym);
+    }();
     return fn;
 }
 

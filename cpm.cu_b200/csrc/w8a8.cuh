@@ -72,29 +72,4 @@ __device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// The launchers below belong to streams of the caller's choice: they do not count in the library stream's order of launches.
-template <typename... KArgs, typename... Args>
-void launch(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t s, int cluster, bool programmatic, Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (cluster > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = cluster;
-        attr[n].val.clusterDim.y = 1;
-        attr[n++].val.clusterDim.z = 1;
-    }
-    if (programmatic && runtime().pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
-    CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
-}
-
 }  // namespace w8

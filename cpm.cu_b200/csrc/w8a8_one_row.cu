@@ -217,7 +217,7 @@ void run(const OneRowArgs& a, int grid, size_t ints, cudaStream_t s) {
         return true;
     }();
     (void)allowed;
-    launch(one_row_s8_kernel<SRC, VEC, GATED, DEEP>, grid, THREADS, RING_BYTES<DEEP> + ints, s, 1, true, a);
+    launch_on(one_row_s8_kernel<SRC, VEC, GATED, DEEP>, grid, THREADS, RING_BYTES<DEEP> + ints, s, 1, true, a);
 }
 template <Source SRC, bool GATED>
 void run(const OneRowArgs& a, int grid, size_t ints, bool vec, bool deep, cudaStream_t s) {

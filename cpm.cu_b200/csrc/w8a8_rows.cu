@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 1024 : VPT == 4 ? 512 :
 
 template <Source SRC>
 void run_quantize(const QuantizeArgs& a, int rows, bool vec, cudaStream_t s) {
-    auto go = [&](void (*kernel)(QuantizeArgs), int threads) { launch(kernel, rows, threads, 0, s, 1, true, a); };
+    auto go = [&](void (*kernel)(QuantizeArgs), int threads) { launch_on(kernel, rows, threads, 0, s, 1, true, a); };
     if (!vec) { go(quantize_kernel<SRC, 0, 1>, 256); return; }
     const int vectors = a.K / 8, round32 = (vectors + 31) / 32 * 32;
     if (rows <= 2 * runtime().num_sms) {
@@ -161,7 +161,7 @@ void launch_pack(const int8_t* q, const float* scale, int N, int K, Role role, v
     const bool vec = K % 16 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
     const size_t want = (chunks + 255) / 256;
     // not programmatic, and the kernel lets no successor start early (w8a8.cuh)
-    launch(pack_kernel, static_cast<int>(want < 148 * 32 ? want : 148 * 32), 256, 0, s, 1, false, q, scale, N, K, static_cast<int>(role), w.kblocks, vec,
+    launch_on(pack_kernel, static_cast<int>(want < 148 * 32 ? want : 148 * 32), 256, 0, s, 1, false, q, scale, N, K, static_cast<int>(role), w.kblocks, vec,
            const_cast<uint8_t*>(w.blocks), const_cast<float*>(w.scales), chunks);
 }
 

@@ -114,3 +114,80 @@ def test_queries_or_keys_alone(rotary):
     assert none.shape == (6, 0)
     assert torch.equal(k, q[:, :64]) and torch.equal(v, qkv[:, 64:])
     assert rotary.append(qkv[:0], 4, 0, 32, inv, pos[:0]).shape == (0, 128)
+
+
+def test_many_rows_and_graphs(rotary):
+    """Row counts on both sides of the change to rings of rows, short rows in groups among them; again from a graph, in place."""
+    for heads, kv, dim, rot, interleaved, rows in [(8, 2, 128, 128, False, 1183), (8, 2, 128, 128, False, 1185), (4, 1, 64, 64, True, 3551), (4, 1, 64, 32, False, 3557),
+                                                   (2, 0, 64, 64, False, 20001), (0, 1, 32, 32, True, 9001), (3, 1, 64, 0, False, 9001), (24, 4, 256, 256, False, 1301)]:
+        g = torch.Generator("cuda").manual_seed(rows)
+        qkv = torch.randn(rows, (heads + 2 * kv) * dim, generator=g, device="cuda").to(BF16)
+        inv = rotary.frequencies(max(rot, 2), 500000.0)[0][:rot // 2].cuda()
+        pos = torch.arange(rows, dtype=I32, device="cuda") + 100000
+        slots = torch.randperm(rows, generator=g, device="cuda").to(I32)
+        slots[::7] = -1
+        k, v = torch.zeros(2, rows, kv * dim, dtype=BF16, device="cuda")
+        q = rotary.append(qkv, heads, kv, dim, inv, pos, k, v, slots, rot_dims=rot, interleaved=interleaved)
+        want, values, tol = definition(qkv, heads, kv, dim, inv, pos, rot, interleaved, 1.0)
+        assert bool(((q.double().unflatten(1, (heads, dim)) if heads else want[:, :0]) - want[:, :heads]).abs().le(tol[:, :heads]).all())
+        if kv:
+            at = slots[slots >= 0].long()
+            assert bool(((k[at].double().unflatten(1, (kv, dim)) - want[slots >= 0][:, heads:]).abs() <= tol[slots >= 0][:, heads:]).all())
+            assert torch.equal(v[at].double().unflatten(1, (kv, dim)), values[slots >= 0])
+            rest = torch.ones(rows, dtype=torch.bool, device="cuda")
+            rest[at] = False
+            assert not bool(k[rest].any()) and not bool(v[rest].any())
+        again = qkv.clone()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                rotary.append(again, heads, kv, dim, inv, pos, k, v, slots, rot_dims=rot, interleaved=interleaved, out=again[:, :heads * dim])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again[:, :heads * dim], q) and torch.equal(again[:, heads * dim:], qkv[:, heads * dim:])
+
+
+def test_offsets_beyond_32_bits(rotary):
+    """Cache slots and rows whose elements lie beyond 2^31."""
+    heads, kv, dim, slots_n = 2, 2, 64, 17_000_000
+    k = torch.empty(slots_n, kv * dim, dtype=BF16, device="cuda")
+    v = torch.empty_like(k)
+    rows, ld = 40000, 60000
+    wide = torch.empty(rows, ld, dtype=BF16, device="cuda")
+    qkv = wide[:, 1000:1000 + (heads + 2 * kv) * dim]
+    qkv.copy_(torch.randn(rows, (heads + 2 * kv) * dim, device="cuda"))
+    inv = rotary.frequencies(dim, 10000.0)[0].cuda()
+    pos = torch.arange(rows, dtype=I32, device="cuda")
+    at = torch.arange(slots_n - rows, slots_n, device="cuda")
+    for n in (rows, 200):                    # rings of rows, one CTA per row
+        k[at], v[at] = 0, 0
+        part = qkv[-n:]
+        q = rotary.append(part, heads, kv, dim, inv, pos[-n:], k, v, at[-n:].to(I32))
+        want, values, tol = definition(part, heads, kv, dim, inv, pos[-n:], dim, False, 1.0)
+        assert bool(((q.double().unflatten(1, (heads, dim)) - want[:, :heads]).abs() <= tol[:, :heads]).all())
+        assert bool(((k[at[-n:]].double().unflatten(1, (kv, dim)) - want[:, heads:]).abs() <= tol[:, heads:]).all())
+        assert torch.equal(v[at[-n:]].double().unflatten(1, (kv, dim)), values)
+        if n < rows:
+            assert not bool(k[at[:-n]].any())
+
+
+def test_refusals_on_the_gpu(rotary):
+    qkv = torch.zeros(4, 3 * 64, dtype=BF16, device="cuda")
+    inv, pos = torch.ones(32, device="cuda"), torch.zeros(4, dtype=I32, device="cuda")
+    k, v = torch.zeros(2, 4, 64, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="qkv"):
+        rotary.append(qkv[:, 1:], 1, 1, 64, inv, pos, k, v, pos)
+    with pytest.raises(ValueError, match="inv_freq"):
+        rotary.append(qkv, 1, 1, 64, inv[1:], pos, k, v, pos)
+    with pytest.raises(ValueError, match="positions"):
+        rotary.append(qkv, 1, 1, 64, inv, pos.long(), k, v, pos)
+    with pytest.raises(ValueError, match="v_cache"):
+        rotary.append(qkv, 1, 1, 64, inv, pos, k, v[:3], pos)
+    with pytest.raises(ValueError, match="slots"):
+        rotary.append(qkv, 1, 1, 64, inv, pos, k, v)
+    with pytest.raises(RuntimeError, match="caches must not overlap"):
+        rotary.append(qkv, 1, 1, 64, inv, pos, k, k, pos)
+    with pytest.raises(RuntimeError, match="query part"):
+        rotary.append(qkv, 1, 1, 64, inv, pos, k, v, pos, out=qkv[:, 64:128])

@@ -51,6 +51,26 @@ def test_integers_at_ties_and_edges(w8):
         assert torch.equal(q2[1:], q[1:]) and torch.equal(s2[1:], scale[1:])
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_integers_behind_a_norm(w8, rows):
+    """The identity as weights shows the integers: exactly those of t * weight, half-way values among them (the half of a row's largest magnitude, and
+    rows whose largest has the mantissa 254, which have many)."""
+    width = 512
+    eye = w8.PackedLinear(torch.eye(width, dtype=torch.int8, device="cuda"), torch.ones(width, device="cuda"))
+    g = torch.Generator("cuda").manual_seed(rows)
+    for top, weight in ((254.0, 1.0), (3.0, 1.0), (1.28125, 1.953125), (1.7, 0.6), (254.0, 1.5), (127.0, 2.540625)):
+        x = torch.randint(-127, 128, (rows, width), generator=g, device="cuda") * torch.tensor(top / 127 / 8, device="cuda")
+        x[:, 0], x[:, 1], x[:, 2], x[:, 3] = top, top / 2, -top / 2, -top / 4
+        x = x.to(BF16)
+        w = torch.full((width,), weight, dtype=BF16, device="cuda")
+        w[200:] = (0.5 + torch.rand(width - 200, generator=g, device="cuda")).to(BF16) * weight / 2
+        r, t, _ = ref.ints(x.double() * w.double())
+        y = w8.linear(x, eye, norm_weight=w)
+        f = 1 / torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + float(torch.tensor(1e-5)))
+        assert torch.equal((y.double() / (t / 127 * f)).round(), r), (top, weight)
+        assert bool((w8.linear(x, eye).double() / (x.double().abs().amax(1, keepdim=True) / 127)).round().eq(ref.ints(x.double())[0]).all())
+
+
 SIZES = [(1, 64, 64), (1, 1, 1), (1, 4096, 512), (1, 1000, 333), (1, 16384, 130), (1, 50000, 20), (1, 128, 8192),
          (2, 64, 64), (2, 1, 1), (3, 129, 127), (16, 1024, 4096), (17, 2048, 640), (60, 4096, 384), (64, 512, 20000), (64, 704, 1000),
          (65, 512, 256), (100, 4096, 1024), (128, 256, 4736), (129, 1024, 512), (256, 2048, 300), (257, 512, 512), (300, 1024, 384),
@@ -112,3 +132,203 @@ def test_gated_ffn(w8, rows, width, inter, norm):
         x = total
     want, tol, _ = ref.ffn(x, *gate, *up, *down, **more)
     near(got, want, tol)
+
+
+# ------------------------------------------------------------------------------------------------ rows with nothing, infinities and NaN; strides; types of calls
+@pytest.mark.parametrize("rows", [1, 5, 40, 100, 300])
+def test_rows_of_zeros_infinities_and_nan(w8, rows):
+    x, q, s = ref.make(rows, 512, 300, seed=rows, device="cuda")
+    bias = torch.randn(300, device="cuda").to(BF16)
+    packed = w8.PackedLinear(q, s)
+    gate_up, down = w8.PackedGateUp(q, s, q.flip(0).contiguous(), s), w8.PackedLinear(*ref.make(1, 300, 512, 1, "cuda")[1:])
+    clean, clean_ffn = w8.linear(x, packed, bias=bias), w8.gated_ffn(x, gate_up, down)
+    for value in (0.0, float("inf"), float("-inf"), float("nan")):
+        bad = x.clone()
+        at = rows // 2
+        if value == 0.0:
+            bad[at] = 0
+        else:
+            bad[at, 100] = value
+        rest = torch.arange(rows, device="cuda") != at
+        y, f = w8.linear(bad, packed, bias=bias), w8.gated_ffn(bad, gate_up, down)
+        assert torch.equal(y[rest], clean[rest]) and torch.equal(f[rest], clean_ffn[rest])     # no other row is touched
+        if value == 0.0:
+            assert torch.equal(y[at], bias) and not bool(f[at].any())
+        else:
+            assert bool(torch.isnan(y[at]).all()) and bool(torch.isnan(f[at]).all())
+        g = torch.ones(512, dtype=BF16, device="cuda")
+        for eps in (1e-5, 0.0):
+            n = w8.linear(bad, packed, bias=bias, norm_weight=g, eps=eps)[at]
+            assert torch.equal(n, bias) if value == 0.0 else bool(torch.isnan(n).all())
+
+
+@pytest.mark.parametrize("rows,width,out", [(1, 257, 65), (1, 256, 64), (7, 257, 129), (33, 264, 200), (300, 130, 131)])
+def test_views_of_wider_matrices(w8, rows, width, out):
+    wide, q, s = ref.make(rows, width + 13, out, seed=2, device="cuda")
+    q = q[:, :width].contiguous()
+    for left in (0, 5, 8):
+        x = wide[:, left:left + width]
+        held = torch.full((rows + 2, out + 11), 7.0, dtype=BF16, device="cuda")
+        y = w8.linear(x, w8.PackedLinear(q, s), out=held[1:1 + rows, 3:3 + out])
+        want, tol, _ = ref.linear(x, q, s)
+        near(y, want, tol)
+        edge = torch.ones_like(held, dtype=torch.bool)
+        edge[1:1 + rows, 3:3 + out] = False
+        assert bool((held[edge] == 7).all())                    # what lies around the outputs
+    # input and output columns of one matrix
+    both = torch.cat((wide[:, :width], torch.zeros(rows, out, dtype=BF16, device="cuda")), 1)
+    y = w8.linear(both[:, :width], w8.PackedLinear(q, s), out=both[:, width:])
+    assert torch.equal(y, w8.linear(wide[:, :width], w8.PackedLinear(q, s)))
+
+
+def test_empty_batches(w8):
+    _, q, s = ref.make(1, 64, 32, device="cuda")
+    x = torch.empty(0, 64, dtype=BF16, device="cuda")
+    assert w8.linear(x, w8.PackedLinear(q, s)).shape == (0, 32)
+    y, t = w8.linear(x, w8.PackedLinear(q, s), norm_weight=torch.ones(64, dtype=BF16, device="cuda"), delta=x)
+    assert y.shape == (0, 32) and t.shape == (0, 64)
+    _, d, ds = ref.make(1, 32, 64, device="cuda")
+    assert w8.gated_ffn(x, w8.PackedGateUp(q, s, q, s), w8.PackedLinear(d, ds)).shape == (0, 64)
+    assert w8.quantize(x)[0].shape == (0, 64)
+
+
+def test_weights_from_bf16(w8):
+    w = torch.randn(200, 333, device="cuda").to(BF16)
+    q, s = w8.quantize(w)
+    x, _, _ = ref.make(9, 333, 1, device="cuda")
+    assert torch.equal(w8.linear(x, w8.PackedLinear.from_bf16(w)), w8.linear(x, w8.PackedLinear(q, s)))
+    assert float(((q * s[:, None]).double() - w.double()).abs().max()) <= float(s.max()) * 0.5001
+
+
+@pytest.mark.parametrize("rows", [1, 2, 60, 129, 600])
+def test_calls_repeat_to_the_bit_and_replay_in_graphs(w8, rows):
+    width, out = 2048, 1152
+    x, q, s = ref.make(rows, width, out, seed=rows, device="cuda")
+    packed = w8.PackedLinear(q, s)
+    norm = {"norm_weight": torch.linspace(0.5, 2, width, device="cuda").to(BF16), "delta": x.flip(0).contiguous()}
+    _, gate, up, down = make_ffn(1, width, 704, 4)
+    gate_up, down = w8.PackedGateUp(*gate, *up), w8.PackedLinear(*down)
+
+    def calls():
+        y, t = w8.linear(x, packed, **norm)
+        return y, t, w8.gated_ffn(x, gate_up, down)
+    first = calls()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(calls(), first))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            kept = calls()
+    x.copy_(x.roll(1, 1))                  # new values in the captured input
+    norm["delta"].copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(kept, calls()))
+
+
+def test_calls_on_several_streams_at_once(w8):
+    """Products that fill the device, cut tiles among them, beside one another: each waits for none of the others' CTAs."""
+    work = []
+    for i, (rows, width, out) in enumerate([(4096, 2048, 1280), (128, 16384, 1024), (60, 4096, 4608), (1, 8192, 8192), (700, 4096, 2304)]):
+        x, q, s = ref.make(rows, width, out, seed=i, device="cuda")
+        work.append((x, w8.PackedLinear(q, s)))
+    want = [w8.linear(x, p) for x, p in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    got = [[] for _ in work]
+    for _ in range(20):
+        for i, (s, (x, p)) in enumerate(zip(streams, work)):
+            with torch.cuda.stream(s):
+                got[i].append(w8.linear(x, p))
+    torch.cuda.synchronize()
+    import cpmcu.C as C
+    for s in streams:
+        C.stream_check(s.cuda_stream)
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+
+
+def test_calls_from_several_threads(w8):
+    import threading
+    x, q, s = ref.make(64, 1024, 512, seed=1, device="cuda")
+    packed = w8.PackedLinear(q, s)
+    want = w8.linear(x, packed)
+    torch.cuda.synchronize()
+    failed = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y = w8.linear(x, packed)
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(y, want):
+                failed.append(1)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+
+
+def test_offsets_beyond_32_bits(w8):
+    """Inputs, integers, activations and outputs of more than 2^31 elements: the last rows are right."""
+    rows, width = 70000, 33000
+    x = torch.zeros(rows, width, dtype=BF16, device="cuda")
+    last, q, s = ref.make(300, width, 96, seed=1, device="cuda")
+    x[-300:] = last
+    y = w8.linear(x, w8.PackedLinear(q, s))
+    want, tol, _ = ref.linear(last, q, s)
+    near(y[-300:], want, tol)
+    assert not bool(y[:-300].any())
+    del x, y
+    rows, width, out = 70000, 64, 33000
+    x = torch.zeros(rows, width, dtype=BF16, device="cuda")
+    last, q, s = ref.make(300, width, out, seed=1, device="cuda")
+    x[-300:] = last
+    y = w8.linear(x, w8.PackedLinear(q, s))
+    want, tol, _ = ref.linear(last, q, s)
+    near(y[-300:], want, tol)
+    assert not bool(y[:-300].any())
+    del y
+    _, up, us = ref.make(1, width, out, seed=2, device="cuda")
+    _, d, ds = ref.make(1, out, width, seed=3, device="cuda")
+    f = w8.gated_ffn(x, w8.PackedGateUp(q, s, up, us), w8.PackedLinear(d, ds))
+    want, tol, _ = ref.ffn(last, q, s, up, us, d, ds)
+    near(f[-300:], want, tol)
+    assert not bool(f[:-300].any())
+
+
+def test_refusals_on_the_gpu(w8):
+    x, q, s = ref.make(4, 64, 32, device="cuda")
+    p = w8.PackedLinear(q, s)
+    with pytest.raises(ValueError, match="x must be"):
+        w8.linear(x.float(), p)
+    with pytest.raises(ValueError, match="x must be"):
+        w8.linear(x[:, :63], p)
+    with pytest.raises(ValueError, match="x must be"):
+        w8.linear(x.cpu(), p)
+    with pytest.raises(ValueError, match="matrix"):
+        w8.linear(x[0], p)
+    with pytest.raises(ValueError, match="consecutive"):
+        w8.linear(torch.zeros(64, 4, dtype=BF16, device="cuda").t(), p)
+    with pytest.raises(ValueError, match="consecutive"):
+        w8.linear(x[:1].expand(4, 64), p)
+    with pytest.raises(ValueError, match="bias"):
+        w8.linear(x, p, bias=torch.zeros(31, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError, match="norm_weight"):
+        w8.linear(x, p, delta=x)
+    with pytest.raises(ValueError, match="delta"):
+        w8.linear(x, p, norm_weight=torch.ones(64, dtype=BF16, device="cuda"), delta=x[:3])
+    with pytest.raises(ValueError, match="out"):
+        w8.linear(x, p, out=torch.zeros(4, 33, dtype=BF16, device="cuda"))
+    square = w8.PackedLinear(*ref.make(1, 64, 64, device="cuda")[1:])
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        w8.linear(x, square, out=x)
+    with pytest.raises(ValueError, match="down must be"):
+        w8.gated_ffn(x, w8.PackedGateUp(q, s, q, s), p)
+    with pytest.raises(ValueError, match="scale"):
+        w8.PackedLinear(q, s[:-1])
+    with pytest.raises(ValueError, match="131072"):
+        w8.PackedLinear(torch.zeros(1, 131073, dtype=torch.int8, device="cuda"), s[:1])
