@@ -396,9 +396,11 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
             grid_dep_wait();
         }
     } else if (warp == 1) {
-        // ------------------------------------------------ MMA issuer (pairs: rank 0)
-        if (lane == 0 && rank == 0) {
+        // ------------------------------------------------ MMA issuer (pairs: rank 0).  The whole warp walks the blocks and one lane issues: descriptors
+        // that are the same in all lanes stay in uniform registers, where the instruction takes them.
+        if (rank == 0) {
             constexpr uint32_t idesc = idesc_s8(CSZ * TILE_ROWS, MT);
+            const bool leader = ptx::elect_one();
             int stage = 0;
             uint32_t phase = 0;
             int acc = 0;
@@ -406,20 +408,26 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
             int tile, kb0, kb1;
             bool ok = true;
             while (ok && it.next(tile, kb0, kb1)) {
-                if (!ptx::mbar_wait(&acc_empty[acc], acc_phase ^ 1, abort_flag)) break;
+                if (!ptx::mbar_wait_warp(&acc_empty[acc], acc_phase ^ 1, abort_flag)) break;
                 ptx::tc_fence_after();
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!ptx::mbar_wait(&full[stage], phase, abort_flag)) { ok = false; break; }
+                    if (!ptx::mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
                     ptx::tc_fence_after();
-                    const uint32_t wa = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
-                    umma_block<PAIR>(tmem_base + acc * MT, wa, wa + BLOCK_BYTES, idesc, kb == kb0);
-                    if constexpr (PAIR) ptx::umma_commit_pair(&empty[stage]);
-                    else ptx::umma_commit(&empty[stage]);
+                    if (leader) {
+                        const uint32_t wa = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
+                        umma_block<PAIR>(tmem_base + acc * MT, wa, wa + BLOCK_BYTES, idesc, kb == kb0);
+                        if constexpr (PAIR) ptx::umma_commit_pair(&empty[stage]);
+                        else ptx::umma_commit(&empty[stage]);
+                    }
+                    __syncwarp();
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
                 }
                 if (!ok) break;
-                if constexpr (PAIR) ptx::umma_commit_pair(&acc_full[acc]);
-                else ptx::umma_commit(&acc_full[acc]);
+                if (leader) {
+                    if constexpr (PAIR) ptx::umma_commit_pair(&acc_full[acc]);
+                    else ptx::umma_commit(&acc_full[acc]);
+                }
+                __syncwarp();
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1;
             }
@@ -531,21 +539,24 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
             grid_dep_wait();
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_s8(TILE_ROWS, MT);
-            int stage = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int i = 0; i < kpc; ++i) {
-                if (!ptx::mbar_wait(&full[stage], phase, abort_flag)) { ok = false; break; }
-                ptx::tc_fence_after();
+        constexpr uint32_t idesc = idesc_s8(TILE_ROWS, MT);
+        const bool leader = ptx::elect_one();
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int i = 0; i < kpc; ++i) {
+            if (!ptx::mbar_wait_warp(&full[stage], phase, abort_flag)) { ok = false; break; }
+            ptx::tc_fence_after();
+            if (leader) {
                 const uint32_t wa = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
                 umma_block<false>(tmem_base, wa, wa + BLOCK_BYTES, idesc, i == 0);
                 ptx::umma_commit(&empty[stage]);
-                if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }
-            if (ok) ptx::umma_commit(acc_full);
+            __syncwarp();
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
         }
+        if (ok && leader) ptx::umma_commit(acc_full);
+        __syncwarp();
     } else {
         // scales while the sums are being made
         ws = a.ws[tile * TILE_ROWS + row];
