@@ -1,7 +1,7 @@
-"""Build libcpmcu_b200.so in-tree with nvcc for sm_100a.
+"""Build libcpmcu_b200.so in-tree with nvcc for sm_100a, and the Python module _ops.so over it with g++ against torch's headers.
 
 Usage: python cpm.cu_b200/build.py [--force]
-The library lands next to the Python package (cpm.cu_b200/cpmcu/) so that it
+Both land next to the Python package (cpm.cu_b200/cpmcu/) so that it
 travels with the source tree; nothing is installed into site-packages.
 """
 import concurrent.futures
@@ -15,6 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "cpmcu")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(OUT_DIR, "libcpmcu_b200.so")
+OPS = os.path.join(OUT_DIR, "_ops.so")   # Python module over the library, for torch tensors
 SOURCES = ["runtime.cu", "gemm_umma.cu", "gemm_pair.cu", "gemm_w4_umma.cu", "elementwise.cu", "tree_attn.cu", "pair_attn.cu", "draft_tree.cu", "accept.cu",
            "marlin_unpack.cu", "sparse_select.cu", "sparse_stage1.cu", "layered_ops.cu", "plain_ops.cu", "one_row.cu", "tanh_rows.cu", "recurrence.cu", "moe.cu", "engine.cu", "engine_layered.cu", "w8a8_rows.cu", "w8a8_one_row.cu", "gemm_w8a8.cu", "rotary.cu", "capi_ops.cu", "capi.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -34,7 +35,7 @@ def _stamp():
     h = hashlib.sha256()
     for root in (CSRC, os.path.join(os.path.dirname(HERE), "include")):
         for name in sorted(os.listdir(root)):
-            if name.endswith((".cu", ".cuh", ".h")):
+            if name.endswith((".cu", ".cuh", ".h", ".cpp")):
                 with open(os.path.join(root, name), "rb") as f:
                     h.update(name.encode())
                     h.update(f.read())
@@ -42,11 +43,25 @@ def _stamp():
     return h.hexdigest()
 
 
+def _ops_command(cuda_home):
+    """g++ command that compiles csrc/torch_ops.cpp and links it against the library beside it and torch's own libraries."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+           os.path.join(CSRC, "torch_ops.cpp"), "-o", OPS]
+    cmd += ["-isystem" + d for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                     os.path.join(cuda_home, "include"), sysconfig.get_paths()["include"])]
+    return cmd + ["-L" + OUT_DIR, "-l:libcpmcu_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+                  "-ltorch_python"]
+
+
 def build(force=False, verbose=True):
     os.makedirs(OBJ_DIR, exist_ok=True)
     stamp_file = os.path.join(OBJ_DIR, "stamp")
     stamp = _stamp()
-    if not force and os.path.exists(LIB) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp:
+    if not force and os.path.exists(LIB) and os.path.exists(OPS) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp:
         return LIB
     nvcc = _nvcc()
 
@@ -64,6 +79,10 @@ def build(force=False, verbose=True):
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
+    home = os.path.dirname(os.path.dirname(nvcc)) if os.path.isabs(nvcc) else "/usr/local/cuda"
+    res = subprocess.run(_ops_command(home), capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed for torch_ops.cpp:\n%s\n%s" % (res.stdout, res.stderr))
     with open(stamp_file, "w") as f:
         f.write(stamp)
     if verbose:

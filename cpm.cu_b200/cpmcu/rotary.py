@@ -7,10 +7,9 @@ import math
 
 import torch
 
-from . import C
-from .w8a8 import _call, _check, _ld
+from . import _ops   # raises where it has not been built (`python cpm.cu_b200/build.py`)
 
-_BF16, _F32, _I32, _F64 = torch.bfloat16, torch.float32, torch.int32, torch.float64
+_F32, _F64 = torch.float32, torch.float64
 
 
 def frequencies(rot_dims, base, scaling=None, length=None, max_position=None):
@@ -100,27 +99,5 @@ def append(qkv, heads, kv_heads, dim, inv_freq, positions, k_cache=None, v_cache
     """Rotated queries [rows, heads * dim] of qkv [rows, (heads + 2 kv_heads) * dim] bf16; rotated keys, and values, go to rows `slots` of the
     caches [cache_rows, kv_heads * dim] (a negative slot: to none).  inv_freq [rot_dims / 2] fp32, positions and slots [rows] int32.
     rot_dims: rotated elements of each head (default: all, None).  out: where the queries go; a view of qkv's own query part is allowed."""
-    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2:
-        raise ValueError("qkv must be a matrix")
-    rows, device = qkv.shape[0], qkv.device
-    rot = dim if rot_dims is None else rot_dims
-    _check(qkv, "qkv", _BF16, (rows, (heads + 2 * kv_heads) * dim), rows=True)
-    _check(inv_freq, "inv_freq", _F32, (rot // 2,), device)
-    _check(positions, "positions", _I32, (rows,), device)
-    if kv_heads > 0:
-        if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 2:
-            raise ValueError("k_cache must be a matrix")
-        cache_rows = k_cache.shape[0]
-        _check(k_cache, "k_cache", _BF16, (cache_rows, kv_heads * dim), device)
-        _check(v_cache, "v_cache", _BF16, k_cache.shape, device)
-        _check(slots, "slots", _I32, (rows,), device)
-        keys = (k_cache.data_ptr(), v_cache.data_ptr(), cache_rows, slots.data_ptr())
-    else:
-        keys = (None, None, 0, None)
-    if out is None:
-        out = qkv.new_empty((rows, heads * dim))
-    else:
-        _check(out, "out", _BF16, (rows, heads * dim), device, rows=True)
-    _call("cpmcu_rotary_append", qkv.get_device(), qkv.data_ptr(), _ld(qkv), rows, heads, kv_heads, dim, rot, interleaved, inv_freq.data_ptr(), factor,
-          positions.data_ptr(), out.data_ptr(), _ld(out), *keys)
-    return out
+    return _ops.rotary_append(qkv, heads, kv_heads, dim, dim if rot_dims is None else rot_dims, interleaved, inv_freq, factor, positions, k_cache, v_cache,
+                              slots, out)

@@ -8,20 +8,16 @@ scale each, exact 32-bit sums (formulas at cpmcu_w8a8_norm in include/cpmcu_b200
 
 Calls run on torch's current stream and return without waiting; they can be captured into CUDA graphs.
 """
-import functools
-
 import torch
 
 from . import C
+from . import _ops   # raises where it has not been built (`python cpm.cu_b200/build.py`)
 
 _BF16, _I8, _F32 = torch.bfloat16, torch.int8, torch.float32
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice   # torch.cuda.current_stream(i).cuda_stream, a tenth of its time
 
 
 def _check(t, what, dtype, shape, device=None, rows=False):
     """rows: any distance between the rows; otherwise contiguous."""
-    if type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape and (t.is_cuda if device is None else t.device == device) and t.is_contiguous():
-        return
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what} must be {dtype} of shape {tuple(shape)}" +
                          (f", got {t.dtype} {tuple(t.shape)}" if isinstance(t, torch.Tensor) else ""))
@@ -35,25 +31,10 @@ def _check(t, what, dtype, shape, device=None, rows=False):
         raise ValueError(f"{what} must have consecutive elements in rows that do not overlap")
 
 
-def _ld(t):
-    return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
-
-
-_functions = {}
-
-
-def _call(name, index, *args):
-    """The entry point on torch's current stream of GPU `index`."""
-    fn = _functions.get(name)
-    if fn is None:
-        fn = _functions[name] = getattr(C.load(), name)
-    if index == _current_device():
-        code = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            code = fn(*args, _raw_stream(index))
-    if code < 0:
-        raise RuntimeError(C.load().cpmcu_last_error().decode())
+def _call(name, device, *args):
+    """The entry point on torch's current stream of `device`."""
+    with torch.cuda.device(device):
+        C.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 
 
 def quantize(x):
@@ -62,7 +43,8 @@ def quantize(x):
         raise ValueError("x must be a matrix")
     _check(x, "x", _BF16, x.shape, rows=True)
     q, scale = torch.empty(x.shape, dtype=_I8, device=x.device), torch.empty(x.shape[0], dtype=_F32, device=x.device)
-    _call("cpmcu_w8a8_quantize", x.get_device(), x.data_ptr(), _ld(x), x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr())
+    ld = x.stride(0) if x.shape[0] > 1 else max(1, x.shape[1])
+    _call("cpmcu_w8a8_quantize", x.device, x.data_ptr(), ld, x.shape[0], x.shape[1], q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -78,7 +60,7 @@ class _Packed:
         self.data = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.ptr = self.data.data_ptr()
         for part, (q, scale) in enumerate(parts, start=int(gated)):
-            _call("cpmcu_w8a8_pack", self.index, q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr)
+            _call("cpmcu_w8a8_pack", self.device, q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr)
 
 
 class PackedLinear(_Packed):
@@ -114,77 +96,12 @@ class PackedGateUp(_Packed):
         return cls(*quantize(gate), *quantize(up))
 
 
-def _rows(x, weight):
-    """Checks x; (rows, distance of the rows)."""
-    try:
-        rows, width = x.shape
-    except (AttributeError, ValueError):
-        raise ValueError("x must be a matrix") from None
-    if x.dtype is _BF16 and width == weight.width and x.get_device() == weight.index and x.is_contiguous():
-        return rows, width
-    _check(x, "x", _BF16, (rows, weight.width), weight.device, rows=True)
-    return rows, _ld(x)
-
-
-def _norm(x, norm_weight, eps, delta, delta_scale):
-    """(arguments, total)"""
-    if norm_weight is None:
-        if delta is not None:
-            raise ValueError("delta needs norm_weight")
-        return _NO_NORM, None
-    _check(norm_weight, "norm_weight", _BF16, x.shape[1:], x.device)
-    if delta is None:
-        return (norm_weight.data_ptr(), eps, None, 1.0, None), None
-    _check(delta, "delta", _BF16, x.shape, x.device)
-    total = torch.empty_like(delta)
-    return (norm_weight.data_ptr(), eps, delta.data_ptr(), delta_scale, total.data_ptr()), total
-
-
-_NO_NORM = (None, 0.0, None, 1.0, None)
-
-
-def _out(out, x, rows, width):
-    """(tensor, distance of its rows)"""
-    if out is None:
-        if width == x.shape[1] and x.is_contiguous():
-            return torch.empty_like(x), width
-        return x.new_empty((rows, width)), width
-    _check(out, "out", _BF16, (rows, width), x.device, rows=True)
-    return out, _ld(out)
-
-
-@functools.lru_cache(maxsize=4096)
-def _workspace_bytes(rows, out, width, inter):
-    n = C.load().cpmcu_w8a8_workspace_bytes(rows, out, width, inter)
-    if n < 0:
-        raise ValueError(C.load().cpmcu_last_error().decode())
-    return n
-
-
-def _workspace(x, *sizes):
-    """(tensor that holds it, address, bytes): of torch's allocator, so that calls of several streams and graphs have their own."""
-    n = _workspace_bytes(*sizes)
-    if n == 0:
-        return None, None, 0
-    t = x.new_empty(n // 2)
-    return t, t.data_ptr(), n
-
-
 def linear(x, weight, bias=None, norm_weight=None, eps=1e-5, delta=None, delta_scale=1.0, out=None):
     """y [rows, out] of x [rows, in].  With norm_weight the rows are RMS norms; with delta, of t = x + delta_scale * delta, and (y, t) is
     returned.  bias [out] bf16.  x (and out) may be rows of a wider matrix."""
     if type(weight) is not PackedLinear:
         raise ValueError("weight must be a PackedLinear")
-    rows, ldx = _rows(x, weight)
-    width, n = weight.width, weight.out
-    if bias is not None:
-        _check(bias, "bias", _BF16, (n,), weight.device)
-        bias = bias.data_ptr()
-    norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
-    y, ldy = _out(out, x, rows, n)
-    keep, ws, size = _workspace(x, rows, n, width, 0)
-    _call("cpmcu_w8a8_linear", weight.index, x.data_ptr(), ldx, weight.ptr, bias, *norm, y.data_ptr(), ldy, rows, n, width, ws, size)
-    return y if total is None else (y, total)
+    return _ops.linear(x, weight.ptr, weight.out, weight.width, weight.index, bias, norm_weight, eps, delta, delta_scale, out)
 
 
 def gated_ffn(x, gate_up, down, norm_weight=None, eps=1e-5, delta=None, delta_scale=1.0, out=None):
@@ -194,9 +111,4 @@ def gated_ffn(x, gate_up, down, norm_weight=None, eps=1e-5, delta=None, delta_sc
     width, inter = gate_up.width, gate_up.out
     if down.width != inter or down.out != width or down.index != gate_up.index:
         raise ValueError(f"down must be [{width}, {inter}] on {gate_up.device}")
-    rows, ldx = _rows(x, gate_up)
-    norm, total = _norm(x, norm_weight, eps, delta, delta_scale)
-    y, ldy = _out(out, x, rows, width)
-    keep, ws, size = _workspace(x, rows, width, width, inter)
-    _call("cpmcu_w8a8_ffn", gate_up.index, x.data_ptr(), ldx, gate_up.ptr, down.ptr, *norm, y.data_ptr(), ldy, rows, width, inter, ws, size)
-    return y if total is None else (y, total)
+    return _ops.ffn(x, gate_up.ptr, down.ptr, width, inter, gate_up.index, norm_weight, eps, delta, delta_scale, out)
