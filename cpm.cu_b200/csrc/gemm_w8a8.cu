@@ -693,12 +693,12 @@ Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
         }
     }
     // Otherwise the kind of tile, and whether the tiles of the last wave are cut into equal pieces, that is expected to end first.  In cycles, from runs of all
-    // kinds over 23 shapes: a k-block; what a launch shows of a tile's way out of tensor memory (beyond that of 64 tokens); and the sum over a cut
+    // kinds over 28 shapes: a k-block; what a launch shows of a tile's way out of tensor memory (beyond that of 64 tokens); and the sum over a cut
     // tile's pieces, as far as whole tiles behind it do not hide it.  Rows x columns x outputs, whole tiles of 64, 128, 256 and pairs, and the best cut
-    // one: 300 x 4096 x 4096 22.5, 13.8, 16.0, 16.1 (21.3) us; 1000 x 4096 x 4608 39.7, 23.0, 16.1, 16.7 (27.7); 2048 x 4096 x 4096 67.4, 42.3,
-    // 26.6, 26.6 (39.9); 128 x 16384 x 4096 38.3, 38.6, 44.4, - (26.6).
+    // one: 300 x 4096 x 4096 19.3, 12.6, 16.1, 15.8 (20.6) us; 1000 x 4096 x 4608 33.6, 20.8, 16.2, 16.8 (26.9); 2048 x 4096 x 4096 55.9, 36.6,
+    // 26.3, 25.7 (36.6); 128 x 16384 x 4096 32.6, 34.3, 44.4, - (25.1); 4096 x 16384 x 4096 408, 233, 206, 177 (174).
     struct Kind { int mt; bool pair; int block, out, sum; };
-    const Kind kinds[] = {{std::min(d.mt, 64), false, 500, 0, 14000}, {128, false, 560, 1100, 20000}, {256, false, 580, 3600, 45000}, {256, true, 540, 6000, 45000}};
+    const Kind kinds[] = {{std::min(d.mt, 64), false, 420, 0, 20000}, {128, false, 500, 1100, 30000}, {256, false, 580, 3600, 45000}, {256, true, 540, 6000, 45000}};
     bool cut = false;
     long long best = -1;
     for (const Kind& k : kinds) {
