@@ -10,9 +10,9 @@
 //                            of the last wave are cut
 // Bound: the weights' bytes from HBM up to some 300 rows, the tensor pipe (and, with warm passes, the power cap) beyond.
 //
-// Cut tiles: each piece but the last counted one leaves its int32 sums in a workspace slot, the one counted last adds them to its own.  Integer
-// sums have no order, so the result does not depend on who is last, and no CTA waits for another one: the launch need not be resident as
-// a whole, and may share the device with launches of other streams.  (Clusters are resident as a whole by definition.)
+// Cut tiles: each piece leaves its int32 sums in a workspace slot, and the one counted last adds them up.  Integer sums have no order, so the
+// result does not depend on who is last, and no CTA waits for another one: the launch need not be resident as a whole, and may share the
+// device with launches of other streams.  (Clusters are resident as a whole by definition.)
 #include <algorithm>
 
 #include "gemm_common.cuh"
@@ -675,6 +675,7 @@ struct Division {
     int mt = 0, m_tiles = 0;
     int cluster = 0;       // CTAs per tile, one tile per cluster
     bool pair = false;
+    bool cut = false;      // pieces of tiles, which are summed through the workspace
     int workers = 0;       // CTAs, pairs, or clusters
     int wave_tiles = 0, tail_grid = 0;
 };
@@ -699,7 +700,6 @@ Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
     // 26.3, 25.7 (36.6); 128 x 16384 x 4096 32.6, 34.3, 44.4, - (25.1); 4096 x 16384 x 4096 408, 233, 206, 177 (174).
     struct Kind { int mt; bool pair; int block, out, sum; };
     const Kind kinds[] = {{std::min(d.mt, 64), false, 420, 0, 20000}, {128, false, 500, 1100, 30000}, {256, false, 580, 3600, 45000}, {256, true, 540, 6000, 45000}};
-    bool cut = false;
     long long best = -1;
     for (const Kind& k : kinds) {
         if ((k.mt > 64 && M <= 64) || (k.pair && (tiles % 2 != 0 || M <= 128))) continue;
@@ -714,13 +714,13 @@ Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
                 d.mt = k.mt;
                 d.pair = k.pair;
                 d.m_tiles = m_tiles;
-                cut = c == 1;
+                d.cut = c == 1;
             }
         }
     }
     const int n_tiles = d.pair ? tiles / 2 : tiles, most = d.pair ? sms / 2 : sms;
     const long long all = static_cast<long long>(n_tiles) * d.m_tiles;
-    if (!cut) {
+    if (!d.cut) {
         const long long rounds = (all + most - 1) / most;
         d.workers = static_cast<int>(std::min<long long>(d.m_tiles == 1 ? (all + rounds - 1) / rounds : most, all));
         d.wave_tiles = static_cast<int>(all);
@@ -739,12 +739,13 @@ int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TIL
 size_t product_partial_bytes(int M, int N, int K, bool gated) {
     if (gated || M <= 1) return 0;
     const Division d = divide(M, tiles_of(N, gated), pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms);
-    return d.cluster > 0 ? 0 : static_cast<size_t>(d.workers) * (d.pair ? 2 : 1) * 2 * d.mt * TILE_ROWS * sizeof(int);
+    return d.cut ? static_cast<size_t>(d.workers) * (d.pair ? 2 : 1) * 2 * d.mt * TILE_ROWS * sizeof(int) : 0;
 }
 int product_tickets(int M, int N, int K, bool gated) {
     if (gated || M <= 1) return 0;
     const int tiles = tiles_of(N, gated);
-    return tiles * divide(M, tiles, pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms).m_tiles;
+    const Division d = divide(M, tiles, pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms);
+    return d.cut ? tiles * d.m_tiles : 0;
 }
 
 void launch_product(const Product& p, cudaStream_t s) {

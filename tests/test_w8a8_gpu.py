@@ -74,7 +74,7 @@ def test_integers_behind_a_norm(w8, rows):
 SIZES = [(1, 64, 64), (1, 1, 1), (1, 4096, 512), (1, 1000, 333), (1, 16384, 130), (1, 50000, 20), (1, 128, 8192),
          (2, 64, 64), (2, 1, 1), (3, 129, 127), (16, 1024, 4096), (17, 2048, 640), (60, 4096, 384), (64, 512, 20000), (64, 704, 1000),
          (65, 512, 256), (100, 4096, 1024), (128, 256, 4736), (129, 1024, 512), (256, 2048, 300), (257, 512, 512), (300, 1024, 384),
-         (333, 713, 1001), (512, 4096, 2048), (700, 256, 5000), (1025, 640, 768), (40, 16384, 256), (2, 131072, 40)]
+         (333, 713, 1001), (512, 4096, 2048), (700, 256, 5000), (1025, 640, 768), (40, 16384, 256), (2, 131072, 40), (60, 256, 19200), (17, 384, 38016), (3, 256, 19100), (64, 512, 40000)]
 
 
 @pytest.mark.parametrize("rows,width,out", SIZES)
@@ -118,7 +118,7 @@ def make_ffn(rows, width, inter, seed):
 
 
 @pytest.mark.parametrize("rows,width,inter", [(1, 64, 64), (1, 1, 1), (1, 4096, 1024), (1, 1000, 333), (2, 128, 64), (3, 100, 65), (16, 512, 704), (60, 4096, 1024),
-                                              (60, 512, 9472), (64, 256, 640), (65, 512, 512), (200, 1024, 1000), (257, 512, 512), (300, 1024, 320), (600, 2048, 2048)])
+                                              (60, 512, 9472), (60, 256, 9536), (5, 128, 9530), (30, 256, 19200), (64, 256, 640), (65, 512, 512), (200, 1024, 1000), (257, 512, 512), (300, 1024, 320), (600, 2048, 2048)])
 @pytest.mark.parametrize("norm", [False, True])
 def test_gated_ffn(w8, rows, width, inter, norm):
     x, gate, up, down = make_ffn(rows, width, inter, rows + inter)
