@@ -6,7 +6,8 @@ scale each, exact 32-bit sums (formulas at cpmcu_w8a8_norm in include/cpmcu_b200
     y, t = linear(x, w, norm_weight=g, delta=d)    # t = x + d, y of rms_norm(t) * g
     y = gated_ffn(x, PackedGateUp(...), w_down)    # down(silu(gate(x)) * up(x))
 
-Calls run on torch's current stream and return without waiting; they can be captured into CUDA graphs.
+Calls run on torch's current stream and return without waiting; they can be captured into CUDA graphs (after a first call outside of one).  What a
+kernel reports (a wait that ran out) is raised by cpmcu.C.stream_check.  Packed weights are not to be written to.
 """
 import torch
 

@@ -2,10 +2,10 @@
 // integers in [-127, 127] (w8a8_rows.cu), W int8, sums exact in 32-bit integers.  Rows of one token go through w8a8_one_row.cu, more
 // through the tensor cores (gemm_w8a8.cu).
 //
-// All launches here are programmatic, on the caller's stream.  A launch lets its successor start only where the note at its kernel says
-// so; packed weights are the one thing that is fetched before the wait for the predecessor.  That is in order because the kernels
-// that write them (pack_kernel) never let a successor start early, so that they have ended, with their writes in L2, before any later launch
-// begins; the fetches go past the first-level cache.
+// All launches here but the packing are programmatic, on the caller's stream.  A launch lets its successor start only where the note at its kernel
+// says so; packed weights are the one thing that is fetched before the wait for the predecessor.  That is in order because the kernel that writes
+// them (pack_kernel) lets no successor start before its CTAs have ended, with their writes in L2, and every later launch starts later still; the
+// fetches go past the first-level cache.
 #pragma once
 #include "common.cuh"
 

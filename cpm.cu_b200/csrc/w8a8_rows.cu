@@ -134,6 +134,7 @@ __global__ void pack_kernel(const int8_t* __restrict__ q, const float* __restric
         *reinterpret_cast<uint4*>(blocks + (static_cast<size_t>(tile) * kblocks + c / BLOCK_COLS) * BLOCK_BYTES + slot * BLOCK_COLS + c % BLOCK_COLS) = v;
         if (c == 0) scales[tile * TILE_ROWS + slot] = r < N ? scale[r] : 0.f;
     }
+    __threadfence();   // in L2 before this CTA ends, which may be when the next launch fetches its first weights
 }
 
 int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TILE_ROWS); }

@@ -483,8 +483,9 @@ int cpmcu_stream_check(void* stream);
  *   y[m][n] = (sum over k of q[m][k] W[n][k]) * s[m] * S[n] + bias[n]             exact sums, rounded once, to bf16
  * A row with an infinity or a NaN gives NaN, a row of zeros the bias.  K <= 131072 (sums of 32 bits).
  *
- * Packed weights are written once, by cpmcu_w8a8_pack, and are read before the launch waits for its predecessor in the stream: write them with that
- * call or with a copy, and not by a kernel of your own that lets its successor start early. */
+ * Packed weights are written once, by cpmcu_w8a8_pack, and the first of them are fetched before a launch waits for its predecessor in the
+ * stream.  A packed buffer that is written in another way (a copy) has to be complete before the call: an event or a synchronisation between. */
+
 /* Bytes of packed weights [N, K] (gated: of N gate rows and N up rows), 256-byte aligned. */
 long cpmcu_w8a8_packed_bytes(int N, int K, int gated);
 /* q [N, K] int8 row-major, scale [N] fp32.  part 0: a matrix of its own; 1 and 2: the gate and the up rows of one gated buffer. */
