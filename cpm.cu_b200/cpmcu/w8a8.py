@@ -1,5 +1,5 @@
 """Linear layers in 8-bit integers: weights int8 with a scale for each output channel, rows of bf16 rounded to 8-bit integers with a
-scale each, exact 32-bit sums (formulas at cpmcu_w8a8_norm in include/cpmcu_b200.h).
+scale each, exact 32-bit sums (formulas at cpmcu_w8a8_linear in include/cpmcu_b200.h).
 
     w = PackedLinear(q, scale)                     # once: int8 [out, in] and fp32 [out] of a checkpoint, or PackedLinear.from_bf16(weight)
     y = linear(x, w)                               # x [rows, in] bf16 -> [rows, out] bf16

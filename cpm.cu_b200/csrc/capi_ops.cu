@@ -1,6 +1,7 @@
 // extern "C" surface of the operators that run on a stream of the caller's choice (part 4 of include/cpmcu_b200.h): 8-bit linear
 // layers and rotations.  They launch and return: no allocation, no synchronisation, no host copy.
 #include <algorithm>
+#include <initializer_list>
 
 #include "../../include/cpmcu_b200.h"
 #include "rotary.cuh"
@@ -48,6 +49,8 @@ bool overlap(const Rows& a, const Rows& b) {
     }
     return true;
 }
+
+Rows whole(const void* p, size_t bytes) { return {p, 1, static_cast<long long>(bytes), static_cast<long long>(bytes), 1}; }
 
 // The library serves the GPU that was current at its first call (one process per GPU).
 void require_device(const char* what) {
@@ -122,12 +125,21 @@ w8::RowSource source_of(const char* what, const void* x, long long ldx, const vo
     return s;
 }
 
-void require_workspace(const char* what, void* ws, long long bytes, const Layout& l) {
+// The workspace, and that it shares nothing with what the call reads and writes.
+void require_workspace(const char* what, void* ws, long long bytes, const Layout& l, std::initializer_list<Rows> others) {
     if (l.total == 0) return;
     if (ws == nullptr || bytes < 0 || static_cast<size_t>(bytes) < l.total) {
         throw std::invalid_argument(std::string("cpmcu_b200: ") + what + ": the workspace needs " + std::to_string(l.total) + " bytes");
     }
     require((addr(ws) & 255) == 0, what, "the workspace must be 256-byte aligned");
+    const Rows wr = whole(ws, l.total);
+    for (const Rows& o : others) require(!overlap(wr, o), what, "the workspace must not overlap what the call reads or writes");
+}
+// What the call writes shares nothing with the weights and the bias.
+void require_apart(const char* what, std::initializer_list<Rows> written, std::initializer_list<Rows> constant) {
+    for (const Rows& w : written) {
+        for (const Rows& c : constant) require(!overlap(w, c), what, "y and total must not overlap the weights or the bias");
+    }
 }
 
 void require_packed(const char* what, const void* packed) {
@@ -165,6 +177,8 @@ int cpmcu_w8a8_pack(const void* q, const float* scale, int N, int K, int part, v
         CPM_REQUIRE(q != nullptr && scale != nullptr, "w8a8_pack: q and scale must not be null");
         CPM_REQUIRE(part >= 0 && part <= 2, "w8a8_pack: part is 0, 1 (gate) or 2 (up)");
         require_packed("w8a8_pack", packed);
+        const Rows pr = whole(packed, w8::packed_bytes(N, K, part != 0));
+        CPM_REQUIRE(!overlap(pr, whole(q, static_cast<size_t>(N) * K)) && !overlap(pr, whole(scale, static_cast<size_t>(N) * 4)), "w8a8_pack: packed must not overlap q or scale");
         require_device("w8a8_pack");
         w8::launch_pack(static_cast<const int8_t*>(q), scale, N, K, static_cast<w8::Role>(part), packed, stream_of(stream));
         return 0;
@@ -207,8 +221,11 @@ int cpmcu_w8a8_linear(const void* x, long long ldx, const void* packed, const vo
         if (rows == 0) return 0;
         require_packed("w8a8_linear", packed);
         const w8::RowSource src = source_of("w8a8_linear", x, ldx, norm, eps, delta, delta_scale, total, rows, K, y, ldy, N);
+        const Rows xr{x, rows, K, ldx, 2}, yr{y, rows, N, ldy, 2}, dr{delta, rows, K, K, 2}, tr{total, rows, K, K, 2}, nr{norm, 1, K, K, 2}, br{bias, 1, N, N, 2};
+        const Rows pr = whole(packed, w8::packed_bytes(N, K, false));
+        require_apart("w8a8_linear", {yr, tr}, {pr, br});
         const Layout l = layout_of(rows, N, K, 0);
-        require_workspace("w8a8_linear", workspace, workspace_bytes, l);
+        require_workspace("w8a8_linear", workspace, workspace_bytes, l, {xr, yr, dr, tr, nr, br, pr});
         require_device("w8a8_linear");
         cudaStream_t s = stream_of(stream);
         const w8::Packed w = w8::packed_view(packed, N, K, false);
@@ -242,8 +259,11 @@ int cpmcu_w8a8_ffn(const void* x, long long ldx, const void* gate_up, const void
         require_packed("w8a8_ffn", gate_up);
         require_packed("w8a8_ffn", down);
         const w8::RowSource src = source_of("w8a8_ffn", x, ldx, norm, eps, delta, delta_scale, total, rows, K, y, ldy, K);
+        const Rows xr{x, rows, K, ldx, 2}, yr{y, rows, K, ldy, 2}, dr{delta, rows, K, K, 2}, tr{total, rows, K, K, 2}, nr{norm, 1, K, K, 2};
+        const Rows gr = whole(gate_up, w8::packed_bytes(inter, K, true)), pr = whole(down, w8::packed_bytes(K, inter, false));
+        require_apart("w8a8_ffn", {yr, tr}, {gr, pr});
         const Layout l = layout_of(rows, K, K, inter);
-        require_workspace("w8a8_ffn", workspace, workspace_bytes, l);
+        require_workspace("w8a8_ffn", workspace, workspace_bytes, l, {xr, yr, dr, tr, nr, gr, pr});
         require_device("w8a8_ffn");
         cudaStream_t s = stream_of(stream);
         const w8::Packed wg = w8::packed_view(gate_up, inter, K, true), wd = w8::packed_view(down, K, inter, false);
@@ -300,6 +320,11 @@ int cpmcu_rotary_append(const void* qkv, long long ld, int rows, int heads, int 
             const Rows kr{k_cache, cache_rows, kv_dim, kv_dim, 2}, vr{v_cache, cache_rows, kv_dim, kv_dim, 2};
             CPM_REQUIRE(!overlap(in, kr) && !overlap(in, vr) && !overlap(qr, kr) && !overlap(qr, vr) && !overlap(kr, vr),
                         "rotary_append: the caches must not overlap each other, qkv or q");
+        }
+        const Rows written[] = {qr, {kv_heads > 0 ? k_cache : nullptr, cache_rows, kv_dim, kv_dim, 2}, {kv_heads > 0 ? v_cache : nullptr, cache_rows, kv_dim, kv_dim, 2}};
+        for (const Rows& w : written) {
+            CPM_REQUIRE(!overlap(w, whole(pos, 4ull * rows)) && !overlap(w, whole(kv_heads > 0 ? slots : nullptr, 4ull * rows)) && !overlap(w, whole(inv_freq, 2ull * rot_dims)),
+                        "rotary_append: q and the caches must not overlap positions, slots or frequencies");
         }
         require_device("rotary_append");
         RotaryArgs a;

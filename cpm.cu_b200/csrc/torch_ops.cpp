@@ -87,17 +87,21 @@ at::Tensor empty(std::initializer_list<int64_t> shape, at::ScalarType type, int 
     return at::empty(at::IntArrayRef(shape), at::TensorOptions().dtype(type).device(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))));
 }
 
-// Runs an entry point with GPU `device` current, on torch's current stream of it, without the interpreter's lock.
+// Runs an entry point with GPU `device` current, on torch's current stream of it, without the interpreter's lock.  What torch throws in there is
+// carried out of it as text: an exception must not pass the point where the lock is taken again.
 template <typename F>
 void run(int device, F&& call) {
-    int code;
+    int code = -1;
     std::string text;
     Py_BEGIN_ALLOW_THREADS
-    {
+    try {
         c10::cuda::OptionalCUDAGuard guard;
         if (c10::cuda::current_device() != device) guard.set_index(static_cast<c10::DeviceIndex>(device));
         code = call(static_cast<void*>(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()));
         if (code < 0) text = cpmcu_last_error();
+    } catch (const std::exception& e) {
+        code = -1;
+        text = e.what();
     }
     Py_END_ALLOW_THREADS
     if (code < 0) throw Raised{PyExc_RuntimeError, text};

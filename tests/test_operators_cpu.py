@@ -45,6 +45,25 @@ def test_linear_refusals():
     assert "y must not overlap x" in linear(ldx=96, y=X + 126, ldy=96)
 
 
+def test_what_is_written_shares_nothing():
+    n, d, t = 0x70000000, 0x50000000, 0x60000000
+    assert "weights or the bias" in linear(bias=Y + 64)
+    assert "weights or the bias" in linear(y=PACKED + 128 * 128)                  # the packed scales
+    assert "weights or the bias" in linear(norm=n, delta=d, total=PACKED + 256)
+    assert "weights or the bias" in linear(norm=n, delta=d, total=t, bias=t)
+
+    def ffn(y):
+        return refused("cpmcu_w8a8_ffn", X, 64, PACKED, 0x18000000, None, 1e-5, None, 1.0, None, y, 64, 4, 64, 128, WS, 1 << 30, None)
+
+    assert "weights or the bias" in ffn(PACKED)
+    assert "weights or the bias" in ffn(0x18000000)
+    assert "packed must not overlap" in refused("cpmcu_w8a8_pack", PACKED + 16, Y, 4, 4, 0, PACKED, None)
+    assert "packed must not overlap" in refused("cpmcu_w8a8_pack", X, PACKED + 128 * 128, 4, 4, 1, PACKED, None)
+    for name in ("pos", "slots", "inv"):
+        assert "positions, slots or frequencies" in rotary(**{name: Y + 8}), name
+        assert "positions, slots or frequencies" in rotary(**{name: 0x60000000 + 64}), name
+
+
 def test_ffn_refusals():
     def ffn(x=X, ldx=64, up=PACKED, down=PACKED, y=Y, ldy=64, rows=4, k=64, inter=128):
         return refused("cpmcu_w8a8_ffn", x, ldx, up, down, None, 1e-5, None, 1.0, None, y, ldy, rows, k, inter, WS, 1 << 30, None)

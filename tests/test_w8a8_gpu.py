@@ -3,6 +3,7 @@ division of the work changes, with odd widths and strides, and for rows with zer
 import pytest
 import torch
 
+import cpmcu.C as C
 import w8a8_cases as ref
 
 pytestmark = pytest.mark.gpu
@@ -332,3 +333,37 @@ def test_refusals_on_the_gpu(w8):
         w8.PackedLinear(q, s[:-1])
     with pytest.raises(ValueError, match="131072"):
         w8.PackedLinear(torch.zeros(1, 131073, dtype=torch.int8, device="cuda"), s[:1])
+
+
+@pytest.mark.parametrize("other", ["x", "y", "bias", "norm", "delta", "total", "packed"])
+@pytest.mark.parametrize("ffn", [False, True])
+def test_workspace_apart(other, ffn):
+    """A workspace that shares memory with what the call reads or writes is refused, before any launch; next to it is fine."""
+    rows, k, n = 4, 64, 64
+    lib = C.load()
+    size = lib.cpmcu_w8a8_workspace_bytes(rows, n, k, 128 if ffn else 0)
+    assert size > 0
+    packed = [lib.cpmcu_w8a8_packed_bytes(*s) for s in (((128, 64, 1), (64, 128, 0)) if ffn else ((n, k, 0),))]
+    pool = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    at = (pool.data_ptr() + 255) // 256 * 256
+    place, ends = {}, {}
+    for name, bytes_ in [("ws", size), ("x", 2 * rows * k), ("y", 2 * rows * n), ("bias", 2 * n), ("norm", 2 * k), ("delta", 2 * rows * k), ("total", 2 * rows * k),
+                         ("packed", packed[-1]), ("up", packed[0])]:
+        place[name], ends[name] = at, at + bytes_
+        at = (at + bytes_ + 255) // 256 * 256
+    assert at <= pool.data_ptr() + pool.numel()
+
+    def call(p, s):
+        if ffn:
+            C.call("cpmcu_w8a8_ffn", p["x"], k, p["up"], p["packed"], p["norm"], 1e-5, p["delta"], 1.0, p["total"], p["y"], n, rows, k, 128, p["ws"], s, None)
+        else:
+            C.call("cpmcu_w8a8_linear", p["x"], k, p["packed"], p["bias"], p["norm"], 1e-5, p["delta"], 1.0, p["total"], p["y"], n, rows, n, k, p["ws"], s, None)
+
+    call(place, size)
+    if not (ffn and other == "bias"):
+        for ws in (place[other], (ends[other] - 1) // 256 * 256):   # the first and the last of its bytes
+            with pytest.raises(RuntimeError, match="the workspace must not overlap"):
+                call({**place, "ws": ws}, 1 << 19)
+    with pytest.raises(RuntimeError, match=f"needs {size} bytes"):
+        call(place, size - 1)
+    torch.cuda.synchronize()
