@@ -91,10 +91,10 @@ Layout layout_of(int rows, int N, int K, int inter) {
         l.q = take(static_cast<size_t>(rows) * std::max(w8::pad_cols(K), inter > 0 ? w8::pad_cols(inter) : 0));
         l.xs = take(align256(rows) * sizeof(float));
         // the down projection's, or the only product's
-        const int k_last = inter > 0 ? inter : K;
-        l.n_tickets = w8::product_tickets(rows, N, k_last, false);
+        const w8::Scratch scratch = w8::product_scratch(rows, N, inter > 0 ? inter : K);
+        l.n_tickets = scratch.tickets;
         l.tickets = take(l.n_tickets * sizeof(int));
-        l.partials = take(w8::product_partial_bytes(rows, N, k_last, false));
+        l.partials = take(scratch.partial_bytes);
     }
     l.total = at;
     return l;
@@ -269,18 +269,20 @@ int cpmcu_w8a8_ffn(const void* x, long long ldx, const void* gate_up, const void
         const w8::Packed wg = w8::packed_view(gate_up, inter, K, true), wd = w8::packed_view(down, K, inter, false);
         char* ws = static_cast<char*>(workspace);
         float* act = reinterpret_cast<float*>(ws + l.act);
+        // Activations in rows of a multiple of eight: the columns behind `inter` are products with the packed zeros, 0, or NaN in a row that is NaN anyway.
+        const int middle_cols = static_cast<int>(l.act_ld);
         w8::RowSource middle;
         middle.x32 = act;
         middle.ldx = l.act_ld;
         if (rows == 1) {
-            w8::launch_one_row(src, inter, K, wg, nullptr, nullptr, act, s);
-            w8::launch_one_row(middle, K, inter, wd, nullptr, static_cast<bf16*>(y), nullptr, s);
+            w8::launch_one_row(src, middle_cols, K, wg, nullptr, nullptr, act, s);
+            w8::launch_one_row(middle, K, middle_cols, wd, nullptr, static_cast<bf16*>(y), nullptr, s);
             return 0;
         }
         int8_t* q = reinterpret_cast<int8_t*>(ws + l.q);
         float* xs = reinterpret_cast<float*>(ws + l.xs);
         w8::Product p;
-        p.M = rows; p.N = inter; p.K = K;
+        p.M = rows; p.N = middle_cols; p.K = K;
         p.w = wg;
         p.q = q; p.xs = xs;
         p.act = act; p.ldy = l.act_ld;
@@ -293,7 +295,7 @@ int cpmcu_w8a8_ffn(const void* x, long long ldx, const void* gate_up, const void
         p.y = static_cast<bf16*>(y); p.ldy = ldy;
         p.partials = ws + l.partials;
         p.tickets = reinterpret_cast<int*>(ws + l.tickets);
-        w8::launch_quantize(middle, rows, inter, q, w8::pad_cols(inter), w8::pad_cols(inter), xs, p.tickets, l.n_tickets, s);
+        w8::launch_quantize(middle, rows, middle_cols, q, w8::pad_cols(inter), w8::pad_cols(inter), xs, p.tickets, l.n_tickets, s);
         w8::launch_product(p, s);
         return 0;
     });

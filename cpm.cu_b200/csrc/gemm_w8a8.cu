@@ -3,11 +3,10 @@
 //
 // Operand mapping as for the bf16 products (gemm_umma.cu): weights are the A operand (128 rows of a tile), token rows the B operand, the
 // accumulator is Y^T.  A k-block is 128 integers, one 128-byte swizzle row, so a stage has the bytes of a bf16 stage and twice the products.
-//   M <= 64, and few tiles   clusters of 2 to 4 CTAs that cut a tile's k-blocks evenly and sum it in distributed shared memory
-//   M <= 64                  single CTAs on whole tiles, or the line of all (tile, k-block) units cut evenly (stream-K)
-//   M > 64                   token tiles of 64, 128 or 256 on single CTAs, or pairs of CTAs on tiles of 256 x 256 (tcgen05 cta_group::2: half of the
-//                            operand bytes per product), whichever division divide() expects to end first; whole tiles in waves, and only those
-//                            of the last wave are cut
+//   few tiles   clusters of 2 to 8 CTAs that cut a tile's k-blocks evenly and sum it in distributed shared memory, token tiles of 16 to 128
+//   more        token tiles of 16 to 256 on single CTAs, or pairs of CTAs on tiles of 256 x 256 (tcgen05 cta_group::2: half of the operand bytes per
+//               product); whole tiles in waves, and only those of the last wave are cut (stream-K), where that pays
+// whichever find_division() expects to end first.
 // Bound: the weights' bytes from HBM up to some 300 rows, the tensor pipe (and, with warm passes, the power cap) beyond.
 //
 // Cut tiles: each piece leaves its int32 sums in a workspace slot, and the one counted last adds them up.  Integer sums have no order, so the
@@ -457,7 +456,7 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
 template <int MT, int CS>
 struct ClusterCfg {
     static constexpr int STAGE_BYTES = Cfg<MT, false>::STAGE_BYTES;
-    static constexpr int STAGES = Cfg<MT, false>::STAGES;
+    static constexpr int STAGES = MT <= 64 ? Cfg<MT, false>::STAGES : 5;
     static constexpr int TPR = MT / CS + (MT % CS != 0);            // tokens summed and stored by each rank
     static constexpr int RED_BYTES = CS * TPR * TILE_ROWS * 4;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + RED_BYTES + CTRL_BYTES + 1024;
@@ -480,7 +479,8 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = static_cast<int>(ptx::cluster_ctarank());
-    const int tile = blockIdx.x / CS, kblocks = a.sched.kblocks;
+    const int m_tile = blockIdx.x / CS / a.sched.n_tiles, tile = blockIdx.x / CS - m_tile * a.sched.n_tiles, kblocks = a.sched.kblocks;
+    const int m_base = m_tile * MT;
     const int kb_begin = kblocks * rank / CS, kpc = kblocks * (rank + 1) / CS - kb_begin;
     grid_dep_trigger();
     ptx::cluster_arrive_relaxed();   // "this CTA runs"
@@ -508,7 +508,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
 
     const int q = warp & 3, row = q * 32 + lane;
     bool summed = false;   // epilogue threads: this CTA's sums are in tensor memory
-    const int m_cnt = min(a.sched.M, MT), t0 = rank * C::TPR, cnt = min(m_cnt - t0, C::TPR);   // this CTA's share of the tokens
+    const int m_cnt = min(a.sched.M - m_base, MT), t0 = rank * C::TPR, cnt = min(m_cnt - t0, C::TPR);   // this CTA's share of the tile's tokens
     float ws = 0.f, bias = 0.f;
     if (warp == 0) {
         if (lane == 0) {
@@ -528,7 +528,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
                     ptx::mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
                     ptx::tma_load_2d(dst, &tm_w, &full[stage], 0, (tile * kblocks + kb_begin + i) * TILE_ROWS);
                 }
-                ptx::tma_load_2d(dst + BLOCK_BYTES, &tm_x, &full[stage], (kb_begin + i) * BLOCK_COLS, 0);
+                ptx::tma_load_2d(dst + BLOCK_BYTES, &tm_x, &full[stage], (kb_begin + i) * BLOCK_COLS, m_base);
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
             }
             if (!ok) {   // copies already in flight land before the CTA retires
@@ -561,7 +561,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
         // scales while the sums are being made
         ws = a.ws[tile * TILE_ROWS + row];
         if (a.act == nullptr && a.bias != nullptr && tile * TILE_ROWS + row < a.N) bias = __bfloat162float(a.bias[tile * TILE_ROWS + row]);
-        if (threadIdx.x - 64 < C::TPR) xs[threadIdx.x - 64] = static_cast<int>(threadIdx.x) - 64 < cnt ? a.xs[t0 + threadIdx.x - 64] : 0.f;
+        if (threadIdx.x - 64 < C::TPR) xs[threadIdx.x - 64] = static_cast<int>(threadIdx.x) - 64 < cnt ? a.xs[m_base + t0 + threadIdx.x - 64] : 0.f;
         summed = ptx::mbar_wait_warp(acc_full, 0, abort_flag);
         ptx::tc_fence_after();
     }
@@ -598,7 +598,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
                 int sum = 0;
 #pragma unroll
                 for (int s = 0; s < CS; ++s) sum += red[(s * C::TPR + t) * TILE_ROWS + row];
-                if (n < a.N) a.y[static_cast<long long>(t0 + t) * a.ldy + n] = __float2bfloat16(fmaf(static_cast<float>(sum) * xs[t], ws, bias));
+                if (n < a.N) a.y[static_cast<long long>(m_base + t0 + t) * a.ldy + n] = __float2bfloat16(fmaf(static_cast<float>(sum) * xs[t], ws, bias));
             }
         } else {
             // gate rows 0-63 and up rows 64-127 meet in the first source's place, scaled
@@ -613,7 +613,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
             ptx::named_bar_sync(1, 128);
             const int f = row & 63, n = tile * 64 + f;
             for (int t = row >> 6; t < cnt; t += 2) {
-                if (n < a.N) a.act[static_cast<long long>(t0 + t) * a.ldy + n] = silu_fast(meet[t * TILE_ROWS + f]) * meet[t * TILE_ROWS + 64 + f];
+                if (n < a.N) a.act[static_cast<long long>(m_base + t0 + t) * a.ldy + n] = silu_fast(meet[t * TILE_ROWS + f]) * meet[t * TILE_ROWS + 64 + f];
             }
         }
     }
@@ -655,7 +655,8 @@ template <int MT>
 void run_cluster(int cs, const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
     if (cs == 2) run_cluster<MT, 2>(tw, tx, a, grid, s);
     else if (cs == 3) run_cluster<MT, 3>(tw, tx, a, grid, s);
-    else run_cluster<MT, 4>(tw, tx, a, grid, s);
+    else if (cs == 4) run_cluster<MT, 4>(tw, tx, a, grid, s);
+    else run_cluster<MT, 8>(tw, tx, a, grid, s);
 }
 template <int MT, int CS>
 int capacity_of() {
@@ -667,8 +668,8 @@ int capacity_of() {
 }
 // clusters the device runs at once; the kernels differ in their stages only by the token tile, and by less than a CTA's worth
 template <int MT>
-int capacity(int cs) { return cs == 2 ? capacity_of<MT, 2>() : cs == 3 ? capacity_of<MT, 3>() : capacity_of<MT, 4>(); }
-int cluster_capacity(int mt, int cs) { return mt == 16 ? capacity<16>(cs) : mt == 32 ? capacity<32>(cs) : capacity<64>(cs); }
+int capacity(int cs) { return cs == 2 ? capacity_of<MT, 2>() : cs == 3 ? capacity_of<MT, 3>() : cs == 4 ? capacity_of<MT, 4>() : capacity_of<MT, 8>(); }
+int cluster_capacity(int mt, int cs) { return mt == 16 ? capacity<16>(cs) : mt == 32 ? capacity<32>(cs) : mt == 64 ? capacity<64>(cs) : capacity<128>(cs); }
 
 // How a product is divided: by its sizes alone.
 struct Division {
@@ -679,44 +680,68 @@ struct Division {
     int workers = 0;       // CTAs, pairs, or clusters
     int wave_tiles = 0, tail_grid = 0;
 };
-Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
+// Of all kinds of tiles the one that is expected to end first.  In cycles, fitted to runs of all kinds: block, a k-block of a CTA (the weights no sooner than
+// HBM gives them); out, a tile's way out of tensor memory, where no other tile hides it (clusters: with the sum); next, what one tile takes at least
+// where another one follows.
+Division find_division(int M, int tiles, int kblocks, bool gated, int sms) {
     Division d;
-    d.mt = linear_pick_mt(M);
-    d.m_tiles = ceil_div(M, d.mt);
-    if (d.m_tiles == 1 && d.mt <= 64) {
-        // the most CTAs per tile that run at once and have two k-blocks each
-        for (int cs = 4; cs >= 2; --cs) {
-            if (kblocks >= 2 * cs && static_cast<long long>(tiles) * cs <= sms && cluster_capacity(d.mt, cs) >= tiles) {
-                d.cluster = cs;
-                d.workers = tiles;
-                return d;
-            }
+    const int widest = linear_pick_mt(M), from_hbm = static_cast<int>(static_cast<long long>(tiles) * kblocks * BLOCK_BYTES / 3440);
+    long long best = -1;
+    auto better = [&](long long cost) {
+        if (best >= 0 && cost >= best) return false;
+        best = cost;
+        return true;
+    };
+    // One tile per cluster, all clusters at once.  Rows x columns x outputs, single CTAs (whole or cut) and the best cluster: 95 x 2624 x 256 10.0, 4.6 us
+    // (tiles of 16, 8 CTAs); 200 x 1024 x 1024 7.1, 5.7 (32, 2); 300 x 4096 x 1024 12.9, 10.3 (64, 3); 128 x 16384 x 4096 28.2, 19.9 (128, 4); but
+    // 333 x 713 x 1001 7.7, 8.7 and 100 x 128 x 1024 whole (the rows' own kernel in all of them).
+    struct Cluster { int mt, block, out; };
+    constexpr Cluster clusters[] = {{16, 400, 2500}, {32, 420, 2800}, {64, 440, 5400}, {128, 490, 8900}};
+    for (const Cluster& k : clusters) {
+        const long long n = static_cast<long long>(tiles) * ceil_div(M, k.mt);
+        if (k.mt > widest || 2 * n > sms) continue;
+        for (int cs : {8, 4, 3, 2}) {
+            if (kblocks < 2 * cs || n * cs > sms) continue;
+            const long long cost = std::max(ceil_div(kblocks, cs) * k.block, from_hbm) + k.out;
+            if ((best >= 0 && cost >= best) || cluster_capacity(k.mt, cs) < n) continue;
+            best = cost;
+            d.mt = k.mt;
+            d.cluster = cs;
         }
     }
-    // Otherwise the kind of tile, and whether the tiles of the last wave are cut into equal pieces, that is expected to end first.  In cycles, from runs of all
-    // kinds over 28 shapes: a k-block; what a launch shows of a tile's way out of tensor memory (beyond that of 64 tokens); and the sum over a cut
-    // tile's pieces, as far as whole tiles behind it do not hide it.  Rows x columns x outputs, whole tiles of 64, 128, 256 and pairs, and the best cut
+    // Single CTAs and pairs, and whether the tiles of the last wave are cut into equal pieces: whole tiles of 64, 128, 256 and pairs, and the best cut
     // one: 300 x 4096 x 4096 19.3, 12.6, 16.1, 15.8 (20.6) us; 1000 x 4096 x 4608 33.6, 20.8, 16.2, 16.8 (26.9); 2048 x 4096 x 4096 55.9, 36.6,
-    // 26.3, 25.7 (36.6); 128 x 16384 x 4096 32.6, 34.3, 44.4, - (25.1); 4096 x 16384 x 4096 408, 233, 206, 177 (174).
-    struct Kind { int mt; bool pair; int block, out, sum; };
-    const Kind kinds[] = {{std::min(d.mt, 64), false, 420, 0, 20000}, {128, false, 500, 1100, 30000}, {256, false, 580, 3600, 45000}, {256, true, 540, 6000, 45000}};
-    long long best = -1;
+    // 26.3, 25.7 (36.6); 4096 x 16384 x 4096 408, 233, 206, 177 (174).  Few columns, whole tiles of 16, 32, 64, 128, 256 and pairs, with the rows' kernel:
+    // 150 x 64 x 16384 13.4, 10.1, 8.5, 8.8, 7.2, 8.1; 250 x 74 x 3519 9.6, 6.7, 5.9, 7.4, 10.8, 11.8; 2000 x 512 x 2048 23.4, 15.8, 13.4, 12.0, 10.7, 11.9.
+    // sum: over a cut tile's pieces, as far as whole tiles behind it do not hide it.
+    struct Kind { int mt; bool pair; int block, out, next, sum; };
+    constexpr Kind kinds[] = {{16, false, 420, 2200, 2000, 20000}, {32, false, 440, 2400, 2300, 20000}, {64, false, 420, 3200, 3200, 20000},
+                              {128, false, 500, 4300, 5500, 30000}, {256, false, 580, 6800, 9000, 45000}, {256, true, 540, 9200, 10500, 45000}};
     for (const Kind& k : kinds) {
-        if ((k.mt > 64 && M <= 64) || (k.pair && (tiles % 2 != 0 || M <= 128))) continue;
-        const int m_tiles = ceil_div(M, k.mt);
-        const long long n = static_cast<long long>(k.pair ? tiles / 2 : tiles) * m_tiles, workers = k.pair ? sms / 2 : sms, waves = n / workers;
-        for (int c = 0; c <= (gated ? 0 : 1); ++c) {                                 // gate/up tiles: the activation needs complete sums
-            if (c == 1 && (n % workers == 0 || n % workers * kblocks < workers * 4)) continue;   // pieces of four blocks at least
-            long long cost = (c == 0 ? (n + workers - 1) / workers * kblocks : (n * kblocks + workers - 1) / workers) * k.block + k.out;
-            if (c == 1) cost += 6000 + std::max<long long>(0, k.sum - waves * kblocks * k.block);
-            if (best < 0 || cost < best) {
-                best = cost;
-                d.mt = k.mt;
-                d.pair = k.pair;
-                d.m_tiles = m_tiles;
-                d.cut = c == 1;
-            }
+        if (k.mt > widest || (k.pair && tiles % 2 != 0)) continue;
+        const long long n = static_cast<long long>(k.pair ? tiles / 2 : tiles) * ceil_div(M, k.mt);
+        const int workers = k.pair ? sms / 2 : sms;
+        const long long waves = n / workers, last = n - waves * workers, one = static_cast<long long>(kblocks) * k.block;
+        const long long behind = last > 0 ? waves : waves - 1;    // waves that another one follows
+        if (better(std::max<long long>(behind * std::max<long long>(one, k.next) + one, from_hbm) + k.out)) {
+            d.mt = k.mt;
+            d.pair = k.pair;
+            d.cut = false;
+            d.cluster = 0;
         }
+        if (gated || last == 0 || last * kblocks < workers * 4) continue;   // gate/up tiles: the activation needs complete sums; pieces of four blocks at least
+        const long long sum = std::max<long long>(0, k.sum - waves * one), share = (n * kblocks + workers - 1) / workers * k.block;
+        if (better(std::max({share, waves * k.next, static_cast<long long>(from_hbm)}) + k.out + 6000 + sum)) {
+            d.mt = k.mt;
+            d.pair = k.pair;
+            d.cut = true;
+            d.cluster = 0;
+        }
+    }
+    d.m_tiles = ceil_div(M, d.mt);
+    if (d.cluster > 0) {
+        d.workers = tiles * d.m_tiles;
+        return d;
     }
     const int n_tiles = d.pair ? tiles / 2 : tiles, most = d.pair ? sms / 2 : sms;
     const long long all = static_cast<long long>(n_tiles) * d.m_tiles;
@@ -732,25 +757,46 @@ Division divide(int M, int tiles, int kblocks, bool gated, int sms) {
     return d;
 }
 
+// A call asks several times for the division of the same sizes (its workspace, its layout, its launch), and a model's layers repeat theirs: each thread keeps
+// the last ones (0.3 us a search).
+Division divide(int M, int tiles, int kblocks, bool gated) {
+    struct Found {
+        int M = -1, tiles = 0, kblocks = 0;
+        bool gated = false;
+        Division d;
+    };
+    thread_local Found found[16];
+    Found& f = found[(static_cast<unsigned>(M) * 31u + static_cast<unsigned>(tiles) * 7u + static_cast<unsigned>(kblocks) * 3u + gated) % 16u];
+    if (f.M != M || f.tiles != tiles || f.kblocks != kblocks || f.gated != gated) {
+        f.M = -1;   // an exception leaves no entry
+        f.d = find_division(M, tiles, kblocks, gated, runtime().num_sms);
+        f.M = M;
+        f.tiles = tiles;
+        f.kblocks = kblocks;
+        f.gated = gated;
+    }
+    return f.d;
+}
+
 int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TILE_ROWS); }
 
 }  // namespace
 
-size_t product_partial_bytes(int M, int N, int K, bool gated) {
-    if (gated || M <= 1) return 0;
-    const Division d = divide(M, tiles_of(N, gated), pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms);
-    return d.cut ? static_cast<size_t>(d.workers) * (d.pair ? 2 : 1) * 2 * d.mt * TILE_ROWS * sizeof(int) : 0;
-}
-int product_tickets(int M, int N, int K, bool gated) {
-    if (gated || M <= 1) return 0;
-    const int tiles = tiles_of(N, gated);
-    const Division d = divide(M, tiles, pad_cols(K) / BLOCK_COLS, gated, runtime().num_sms);
-    return d.cut ? tiles * d.m_tiles : 0;
+Scratch product_scratch(int M, int N, int K) {
+    Scratch s;
+    if (M <= 1) return s;
+    const int tiles = tiles_of(N, false);
+    const Division d = divide(M, tiles, pad_cols(K) / BLOCK_COLS, false);
+    if (d.cut) {
+        s.partial_bytes = static_cast<size_t>(d.workers) * (d.pair ? 2 : 1) * 2 * d.mt * TILE_ROWS * sizeof(int);
+        s.tickets = tiles * d.m_tiles;
+    }
+    return s;
 }
 
 void launch_product(const Product& p, cudaStream_t s) {
     const bool gated = p.act != nullptr;
-    const Division d = divide(p.M, p.w.tiles, p.w.kblocks, gated, runtime().num_sms);
+    const Division d = divide(p.M, p.w.tiles, p.w.kblocks, gated);
     ProductArgs a;
     gemm::LinearArgs& w = a.sched;
     w = gemm::LinearArgs();
@@ -774,7 +820,8 @@ void launch_product(const Product& p, cudaStream_t s) {
         const int grid = d.workers * d.cluster;
         if (d.mt == 16) run_cluster<16>(d.cluster, tw, tx, a, grid, s);
         else if (d.mt == 32) run_cluster<32>(d.cluster, tw, tx, a, grid, s);
-        else run_cluster<64>(d.cluster, tw, tx, a, grid, s);
+        else if (d.mt == 64) run_cluster<64>(d.cluster, tw, tx, a, grid, s);
+        else run_cluster<128>(d.cluster, tw, tx, a, grid, s);
         return;
     }
     if (d.pair) {

@@ -34,7 +34,7 @@ void launch_pack(const int8_t* q, const float* scale, int N, int K, Role role, v
 // What the integers of a row are made of.
 struct RowSource {
     const bf16* x = nullptr;        // rows of K values, ldx apart; or
-    const float* x32 = nullptr;     // fp32 rows
+    const float* x32 = nullptr;     // fp32 rows of whole vectors: K and ldx multiples of 8, 16-byte aligned
     long long ldx = 0;
     // norm != null: integers of t * norm, t = bf16(x + delta_scale * delta) (delta may be null: t = x), whose scale carries 1 / rms(t)
     const bf16* norm = nullptr;
@@ -57,8 +57,11 @@ struct Product {
     void* partials = nullptr;
     int* tickets = nullptr;         // zero
 };
-size_t product_partial_bytes(int M, int N, int K, bool gated);
-int product_tickets(int M, int N, int K, bool gated);
+struct Scratch {                    // what cut tiles need; gate/up tiles are never cut
+    size_t partial_bytes = 0;
+    int tickets = 0;
+};
+Scratch product_scratch(int M, int N, int K);
 void launch_product(const Product& p, cudaStream_t s);
 // one row, straight from its source
 void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const bf16* bias, bf16* y, float* act, cudaStream_t s);

@@ -44,7 +44,7 @@ __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
 }
 
 // Lets its successor start behind its own wait, so that the successor's weights are older than this launch's predecessor.
-template <Source SRC, int VEC, bool GATED, bool DEEP>
+template <Source SRC, bool WIDE, bool GATED, bool DEEP>
 __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const OneRowArgs a) {
     constexpr int SETS = GATED ? 2 : 1;               // gate and up rows of the same features
     constexpr int STEP = MAX_STEP / SETS, PER_STEP = STEP * SETS, DEPTH = SLOTS<DEEP> / PER_STEP;   // copies of a lane; steps in flight
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const
         }
     };
     // the row's lines first: behind the weights' they would be late
-    if (static_cast<int>(threadIdx.x) * VEC < a.K && threadIdx.x % 8 == 0) Values<SRC, VEC>::ask(a.src, 0, a.K, threadIdx.x * VEC);
+    if (static_cast<int>(threadIdx.x) * 8 < a.K && threadIdx.x % 8 == 0) Values<SRC, WIDE>::ask(a.src, 0, a.K, threadIdx.x * 8);
     seek();
 #pragma unroll 1
     for (int i = 0; i < DEPTH; ++i) issue();
@@ -102,21 +102,21 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const
     int8_t* q = reinterpret_cast<int8_t*>(smem + RING_BYTES<DEEP>);
     uint32_t top = 0u;
     float ss = 0.f;
-    Values<SRC, VEC> kept[KEEP];
+    Values<SRC, WIDE> kept[KEEP];
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-        const int c = (threadIdx.x + j * THREADS) * VEC;
+        const int c = (threadIdx.x + j * THREADS) * 8;
         if (c < a.K) kept[j].fetch(a.src, 0, a.K, c);
     }
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-        const int c = (threadIdx.x + j * THREADS) * VEC;
+        const int c = (threadIdx.x + j * THREADS) * 8;
         if (c < a.K) {
             kept[j].combine(a.src, 0, a.K, c, blockIdx.x == 0, top, ss);
         }
     }
-    for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {   // of longer rows: read again below
-        Values<SRC, VEC> r;
+    for (int c = (threadIdx.x + KEEP * THREADS) * 8; c < a.K; c += THREADS * 8) {   // of longer rows: read again below
+        Values<SRC, WIDE> r;
         r.fetch(a.src, 0, a.K, c);
         r.combine(a.src, 0, a.K, c, blockIdx.x == 0, top, ss);
     }
@@ -126,21 +126,21 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const
     const RowRound round8(top, HAS_NORM<SRC>, SRC != SRC_F32);
 #pragma unroll
     for (int j = 0; j < KEEP; ++j) {
-        const int c = (threadIdx.x + j * THREADS) * VEC;
+        const int c = (threadIdx.x + j * THREADS) * 8;
         if (c < a.K) {
-            float v[VEC];
+            float v[8];
             kept[j].values(v);
-            store_ints<HAS_NORM<SRC>, VEC>(q + c, round8, v);
+            *reinterpret_cast<uint2*>(q + c) = ints_of<HAS_NORM<SRC>>(round8, v);
         }
     }
-    for (int c = (threadIdx.x + KEEP * THREADS) * VEC; c < a.K; c += THREADS * VEC) {
-        Values<SRC, VEC> r;
-        float v[VEC], squares = 0.f;
+    for (int c = (threadIdx.x + KEEP * THREADS) * 8; c < a.K; c += THREADS * 8) {
+        Values<SRC, WIDE> r;
+        float v[8], squares = 0.f;
         uint32_t known = 0u;
         r.fetch(a.src, 0, a.K, c);
         r.combine(a.src, 0, a.K, c, false, known, squares);
         r.values(v);
-        store_ints<HAS_NORM<SRC>, VEC>(q + c, round8, v);
+        *reinterpret_cast<uint2*>(q + c) = ints_of<HAS_NORM<SRC>>(round8, v);
     }
     for (int c = a.K + threadIdx.x; c < (kblocks + STEP - 1) / STEP * STEP * BLOCK_COLS; c += THREADS) q[c] = 0;
     const float scale = RowRound::scale(top, factor);
@@ -210,20 +210,22 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const
     ptx::cp_async_wait<0>();
 }
 
-template <Source SRC, int VEC, bool GATED, bool DEEP>
+template <Source SRC, bool WIDE, bool GATED, bool DEEP>
 void run(const OneRowArgs& a, int grid, size_t ints, cudaStream_t s) {
     static const bool allowed = [] {   // the library runs on one device
-        CUDA_CHECK(cudaFuncSetAttribute(one_row_s8_kernel<SRC, VEC, GATED, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_DYNAMIC_SMEM));
+        CUDA_CHECK(cudaFuncSetAttribute(one_row_s8_kernel<SRC, WIDE, GATED, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_DYNAMIC_SMEM));
         return true;
     }();
     (void)allowed;
-    launch_on(one_row_s8_kernel<SRC, VEC, GATED, DEEP>, grid, THREADS, RING_BYTES<DEEP> + ints, s, 1, true, a);
+    launch_on(one_row_s8_kernel<SRC, WIDE, GATED, DEEP>, grid, THREADS, RING_BYTES<DEEP> + ints, s, 1, true, a);
 }
 template <Source SRC, bool GATED>
-void run(const OneRowArgs& a, int grid, size_t ints, bool vec, bool deep, cudaStream_t s) {
-    if (!vec) run<SRC, 1, GATED, false>(a, grid, ints, s);
-    else if (deep) run<SRC, 8, GATED, true>(a, grid, ints, s);
-    else run<SRC, 8, GATED, false>(a, grid, ints, s);
+void run(const OneRowArgs& a, int grid, size_t ints, bool wide, bool deep, cudaStream_t s) {
+    if constexpr (SRC != SRC_F32) {   // activations come in whole vectors
+        if (!wide) { run<SRC, false, GATED, false>(a, grid, ints, s); return; }
+    }
+    if (deep) run<SRC, true, GATED, true>(a, grid, ints, s);
+    else run<SRC, true, GATED, false>(a, grid, ints, s);
 }
 
 }  // namespace
@@ -251,12 +253,12 @@ void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const b
     }
     const int grid = std::min(sms, ceil_div(a.units, WARPS / a.share));
     const size_t ints = static_cast<size_t>(all_steps) * step_blocks * BLOCK_COLS;
-    const bool vec = rows_in_vectors(src, K);
+    const bool wide = rows_in_vectors(src, K);
     const bool deep = static_cast<size_t>(w.tiles) * w.kblocks * BLOCK_BYTES > static_cast<size_t>(sms) * RING_BYTES<true> && RING_BYTES<true> + ints <= MAX_DYNAMIC_SMEM;
-    if (src.x32 != nullptr) run<SRC_F32, false>(a, grid, ints, vec, deep, s);
-    else if (src.norm == nullptr) gated ? run<SRC_PLAIN, true>(a, grid, ints, vec, deep, s) : run<SRC_PLAIN, false>(a, grid, ints, vec, deep, s);
-    else if (src.delta == nullptr) gated ? run<SRC_NORM, true>(a, grid, ints, vec, deep, s) : run<SRC_NORM, false>(a, grid, ints, vec, deep, s);
-    else gated ? run<SRC_ADD_NORM, true>(a, grid, ints, vec, deep, s) : run<SRC_ADD_NORM, false>(a, grid, ints, vec, deep, s);
+    if (src.x32 != nullptr) run<SRC_F32, false>(a, grid, ints, wide, deep, s);
+    else if (src.norm == nullptr) gated ? run<SRC_PLAIN, true>(a, grid, ints, wide, deep, s) : run<SRC_PLAIN, false>(a, grid, ints, wide, deep, s);
+    else if (src.delta == nullptr) gated ? run<SRC_NORM, true>(a, grid, ints, wide, deep, s) : run<SRC_NORM, false>(a, grid, ints, wide, deep, s);
+    else gated ? run<SRC_ADD_NORM, true>(a, grid, ints, wide, deep, s) : run<SRC_ADD_NORM, false>(a, grid, ints, wide, deep, s);
 }
 
 }  // namespace w8

@@ -6,7 +6,7 @@
 // do not depend on the order of any sum.
 //
 // Bound: bytes.  One CTA per row, which stays in registers between the pass that finds the maximum and the one that rounds; rows too
-// long or not aligned for that are read twice.  A row with an infinity or a NaN gets the scale NaN and integers 0, a row of zeros the scale 0.
+// long for that are read twice.  A row with an infinity or a NaN gets the scale NaN and integers 0, a row of zeros the scale 0.
 #include "w8a8_rows.cuh"
 
 namespace w8 {
@@ -17,42 +17,45 @@ struct QuantizeArgs {
     int K, pad_to;
     int8_t* q;
     long long ldq;
+    bool q_wide;     // rows of q are 8-byte aligned and have room for whole vectors
     float* scale;
     int* clear;
     int n_clear;
 };
 
-// VPT > 0: a thread's VPT vectors of 8 stay in registers; 0: the row is read twice, VEC elements at a time.
+// VPT > 0: a thread's VPT pieces of eight elements stay in registers; 0: the row is read twice.
 // Lets its successor start behind its own wait: a product may then fetch weights, which are older than this launch's predecessor.
-template <Source SRC, int VPT, int VEC>
-__global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 1024 : VPT == 4 ? 512 : 256) quantize_kernel(const QuantizeArgs a) {
+template <int VPT>
+constexpr int MOST_THREADS = VPT == 1 || VPT == 2 ? 1024 : VPT == 4 ? 512 : 256;
+template <Source SRC, int VPT, bool WIDE>
+__global__ void __launch_bounds__(MOST_THREADS<VPT>) quantize_kernel(const QuantizeArgs a) {
     __shared__ uint32_t sh_top[32];
     __shared__ float sh_sum[32];
     const size_t row = blockIdx.x;
-    if (static_cast<int>(threadIdx.x) * VEC < a.K && threadIdx.x % 8 == 0) Values<SRC, VEC>::ask(a.src, row, a.K, threadIdx.x * VEC);
+    if (static_cast<int>(threadIdx.x) * 8 < a.K && threadIdx.x % 8 == 0) Values<SRC, WIDE>::ask(a.src, row, a.K, threadIdx.x * 8);
     grid_dep_wait();
     grid_dep_trigger();
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < a.n_clear; i += gridDim.x * blockDim.x) a.clear[i] = 0;
-    Values<SRC, VEC> kept[VPT > 0 ? VPT : 1];
+    Values<SRC, WIDE> kept[VPT > 0 ? VPT : 1];
     float ss = 0.f;
     uint32_t top = 0u;
-    const int step = blockDim.x * VEC;
+    const int step = blockDim.x * 8;
     if constexpr (VPT > 0) {
         // every load of the row is in flight before the first sum is stored
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int c = threadIdx.x * VEC + j * step;
+            const int c = threadIdx.x * 8 + j * step;
             if (c < a.K) kept[j].fetch(a.src, row, a.K, c);
         }
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int c = threadIdx.x * VEC + j * step;
+            const int c = threadIdx.x * 8 + j * step;
             if (c < a.K) {
                 kept[j].combine(a.src, row, a.K, c, true, top, ss);
             }
         }
     } else {
-        for (int c = threadIdx.x * VEC; c < a.K; c += step) {
+        for (int c = threadIdx.x * 8; c < a.K; c += step) {
             kept[0].fetch(a.src, row, a.K, c);
             kept[0].combine(a.src, row, a.K, c, true, top, ss);
         }
@@ -62,19 +65,27 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 1024 : VPT == 4 ? 512 :
     if constexpr (HAS_NORM<SRC>) factor = 1.f / sqrtf(block_total(ss, sh_sum) / a.K + a.src.eps);
     const RowRound round(top, HAS_NORM<SRC>, SRC != SRC_F32);
     int8_t* q = a.q + row * a.ldq;
-    auto finish = [&](const Values<SRC, VEC>& r, int c) {
-        float v[VEC];
+    auto finish = [&](const Values<SRC, WIDE>& r, int c) {
+        float v[8];
         r.values(v);
-        store_ints<HAS_NORM<SRC>, VEC>(q + c, round, v);
+        const uint2 w = ints_of<HAS_NORM<SRC>>(round, v);
+        if (WIDE || a.q_wide) {
+            *reinterpret_cast<uint2*>(q + c) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (c + i < a.K) q[c + i] = static_cast<int8_t>((i < 4 ? w.x : w.y) >> (i % 4 * 8));
+            }
+        }
     };
     if constexpr (VPT > 0) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int c = threadIdx.x * VEC + j * step;
+            const int c = threadIdx.x * 8 + j * step;
             if (c < a.K) finish(kept[j], c);
         }
     } else {
-        for (int c = threadIdx.x * VEC; c < a.K; c += step) {
+        for (int c = threadIdx.x * 8; c < a.K; c += step) {
             kept[0].fetch(a.src, row, a.K, c);
             uint32_t known = 0u;
             float squares = 0.f;
@@ -86,26 +97,31 @@ __global__ void __launch_bounds__(VPT == 1 || VPT == 2 ? 1024 : VPT == 4 ? 512 :
     if (threadIdx.x == 0) a.scale[row] = RowRound::scale(top, factor);
 }
 
-template <Source SRC>
-void run_quantize(const QuantizeArgs& a, int rows, bool vec, cudaStream_t s) {
-    auto go = [&](void (*kernel)(QuantizeArgs), int threads) { launch_on(kernel, rows, threads, 0, s, 1, true, a); };
-    if (!vec) { go(quantize_kernel<SRC, 0, 1>, 256); return; }
-    const int vectors = a.K / 8, round32 = (vectors + 31) / 32 * 32;
+template <Source SRC, bool WIDE>
+void run_quantize(const QuantizeArgs& a, int rows, cudaStream_t s) {
+    // the kernel, and how many of a row's vectors a thread has
+    auto go = [&](void (*kernel)(QuantizeArgs), int vectors, int each) { launch_on(kernel, rows, (ceil_div(vectors, each) + 31) / 32 * 32, 0, s, 1, true, a); };
+    const int vectors = ceil_div(a.K, 8);
     if (rows <= 2 * runtime().num_sms) {
         // few rows: a row's own time counts, and the fewer vectors a thread has the shorter it is (60 x 16384: 4.2 us with eight on 256 threads, 2.9
         // with two on 1024)
-        if (vectors <= 1024) go(quantize_kernel<SRC, 1, 8>, round32);
-        else if (vectors <= 2048) go(quantize_kernel<SRC, 2, 8>, 1024);
-        else go(quantize_kernel<SRC, 0, 8>, 256);
+        if (vectors <= 1024) go(quantize_kernel<SRC, 1, WIDE>, vectors, 1);
+        else if (vectors <= 2048) go(quantize_kernel<SRC, 2, WIDE>, vectors, 2);
+        else go(quantize_kernel<SRC, 0, WIDE>, 256, 1);
         return;
     }
     // many rows: several CTAs beside one another on an SM
-    if (vectors <= 256) go(quantize_kernel<SRC, 1, 8>, round32);
-    else if (vectors <= 512) go(quantize_kernel<SRC, 2, 8>, 256);
-    else if (vectors <= 1024) go(quantize_kernel<SRC, 4, 8>, 256);
-    else if (vectors <= 2048 && SRC == SRC_PLAIN) go(quantize_kernel<SRC_PLAIN, 8, 8>, 256);
-    else if (vectors <= 2048) go(quantize_kernel<SRC, 4, 8>, 512);
-    else go(quantize_kernel<SRC, 0, 8>, 256);
+    if (vectors <= 256) go(quantize_kernel<SRC, 1, WIDE>, vectors, 1);
+    else if (vectors <= 512) go(quantize_kernel<SRC, 2, WIDE>, vectors, 2);
+    else if (vectors <= 1024) go(quantize_kernel<SRC, 4, WIDE>, vectors, 4);
+    else if (vectors <= 2048 && SRC == SRC_PLAIN) go(quantize_kernel<SRC_PLAIN, 8, WIDE>, vectors, 8);
+    else if (vectors <= 2048) go(quantize_kernel<SRC, 4, WIDE>, vectors, 4);
+    else go(quantize_kernel<SRC, 0, WIDE>, 256, 1);
+}
+template <Source SRC>
+void run_quantize(const QuantizeArgs& a, int rows, bool wide, cudaStream_t s) {
+    if (wide) run_quantize<SRC, true>(a, rows, s);
+    else run_quantize<SRC, false>(a, rows, s);
 }
 
 // one thread per 16 bytes of the packed blocks; R rows of a role per tile
@@ -174,11 +190,12 @@ void launch_quantize(const RowSource& src, int rows, int K, int8_t* q, long long
     a.q = q; a.ldq = ldq;
     a.scale = scale;
     a.clear = clear; a.n_clear = n_clear;
-    const bool vec = rows_in_vectors(src, K) && (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldq % 8 == 0;
-    if (src.x32 != nullptr) run_quantize<SRC_F32>(a, rows, vec, s);
-    else if (src.norm == nullptr) run_quantize<SRC_PLAIN>(a, rows, vec, s);
-    else if (src.delta == nullptr) run_quantize<SRC_NORM>(a, rows, vec, s);
-    else run_quantize<SRC_ADD_NORM>(a, rows, vec, s);
+    a.q_wide = (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldq % 8 == 0;
+    const bool wide = rows_in_vectors(src, K) && a.q_wide;
+    if (src.x32 != nullptr) run_quantize<SRC_F32, true>(a, rows, s);
+    else if (src.norm == nullptr) run_quantize<SRC_PLAIN>(a, rows, wide, s);
+    else if (src.delta == nullptr) run_quantize<SRC_NORM>(a, rows, wide, s);
+    else run_quantize<SRC_ADD_NORM>(a, rows, wide, s);
 }
 
 }  // namespace w8

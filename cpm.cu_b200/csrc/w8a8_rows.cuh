@@ -12,7 +12,7 @@ enum Source { SRC_PLAIN, SRC_NORM, SRC_ADD_NORM, SRC_F32 };
 template <Source S>
 constexpr bool HAS_NORM = S == SRC_NORM || S == SRC_ADD_NORM;
 
-// whether 16-byte accesses fit the source
+// whether 16-byte accesses fit the source (activations are made for them)
 inline bool rows_in_vectors(const RowSource& s, int K) {
     auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
     return K % 8 == 0 && s.ldx % 8 == 0 && ((bits(s.x) | bits(s.x32) | bits(s.norm) | bits(s.delta) | bits(s.total)) & 15) == 0;
@@ -118,39 +118,58 @@ __device__ __noinline__ uint2 exact8(float v0, float v1, float v2, float v3, flo
                       RowRound::low_bytes(r.exact(v4), r.exact(v5), r.exact(v6), r.exact(v7)));
 }
 
-template <bool PRODUCTS, int VEC>
-__device__ __forceinline__ void store_ints(int8_t* q, const RowRound& round, const float (&v)[VEC]) {
-    if constexpr (VEC == 8) {
-        uint2 w = make_uint2(0u, 0u);
-        if (round.plain) w = make_uint2(round.four<PRODUCTS>(v), round.four<PRODUCTS>(v + 4));
-        else if (round.finite) w = exact8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], round.c127, round.top, round.inv);
-        *reinterpret_cast<uint2*>(q) = w;
-    } else {
-        *q = static_cast<int8_t>(round.finite ? round.exact(v[0]) : 0);
-    }
+// eight values to eight integers
+template <bool PRODUCTS>
+__device__ __forceinline__ uint2 ints_of(const RowRound& round, const float (&v)[8]) {
+    if (round.plain) return make_uint2(round.four<PRODUCTS>(v), round.four<PRODUCTS>(v + 4));
+    if (round.finite) return exact8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], round.c127, round.top, round.inv);
+    return make_uint2(0u, 0u);
 }
 
-// ---------------------------------------------------------------- VEC consecutive elements of a row
+// ---------------------------------------------------------------- eight consecutive elements of a row
 // fetch() loads them, combine() makes the residual sum, the largest magnitude and the squares of it, values() gives what is rounded.  A row waits for its
 // maximum in registers: as it came (bf16, fp32), or as the products with the norm's weights (fp32, in the registers of x and the weights).
-template <Source SRC, int VEC>
+// WIDE: 16-byte accesses; otherwise element by element (rows at odd places, or of other widths than multiples of eight), zeros beyond the row's end.
+// (2000 rows of 5121 and a product of 64 columns: 17.8 us; one element per thread and step 33.5.)
+template <Source SRC, bool WIDE>
 struct Values {
     using T = typename std::conditional<SRC == SRC_F32, float, bf16>::type;
-    struct alignas(VEC == 8 ? 16 : sizeof(T)) Block {
-        T e[VEC];
+    struct alignas(16) Block {
+        T e[8];
         __device__ __forceinline__ float at(int i) const {
             if constexpr (SRC == SRC_F32) {
                 return e[i];
-            } else if constexpr (VEC == 8) {
+            } else {
                 const uint32_t two = reinterpret_cast<const uint32_t*>(e)[i >> 1];
                 return i & 1 ? high(two) : low(two);
+            }
+        }
+        __device__ __forceinline__ void load(const T* p, int left) {   // left: elements to the row's end
+            if constexpr (WIDE) {
+                *this = *reinterpret_cast<const Block*>(p);
             } else {
-                return __bfloat162float(e[i]);
+                uint16_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = i < left ? reinterpret_cast<const uint16_t*>(p)[i] : uint16_t(0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(e)[i] = w[2 * i] | static_cast<uint32_t>(w[2 * i + 1]) << 16;
+            }
+        }
+        __device__ __forceinline__ void store(T* p, int left) const {
+            if constexpr (WIDE) {
+                *reinterpret_cast<Block*>(p) = *this;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t two = reinterpret_cast<const uint32_t*>(e)[i >> 1];
+                    if (i < left) reinterpret_cast<uint16_t*>(p)[i] = static_cast<uint16_t>(i & 1 ? two >> 16 : two);
+                }
             }
         }
     };
+    static_assert(WIDE || SRC != SRC_F32, "activations come in whole vectors");
     Block t, d, w;
-    float p[VEC];
+    float p[8];
     __device__ __forceinline__ static const T* base(const RowSource& s) {
         if constexpr (SRC == SRC_F32) return s.x32;
         else return s.x;
@@ -162,24 +181,20 @@ struct Values {
         if constexpr (HAS_NORM<SRC>) prefetch_l2(s.norm + c);
     }
     __device__ __forceinline__ void fetch(const RowSource& s, size_t row, int K, int c) {
-        t = *reinterpret_cast<const Block*>(base(s) + row * s.ldx + c);
-        if constexpr (SRC == SRC_ADD_NORM) d = *reinterpret_cast<const Block*>(s.delta + row * K + c);
-        if constexpr (HAS_NORM<SRC>) w = *reinterpret_cast<const Block*>(s.norm + c);
+        t.load(base(s) + row * s.ldx + c, K - c);
+        if constexpr (SRC == SRC_ADD_NORM) d.load(s.delta + row * K + c, K - c);
+        if constexpr (HAS_NORM<SRC>) w.load(s.norm + c, K - c);
     }
     // `write`: stores the residual sum
     __device__ __forceinline__ void combine(const RowSource& s, size_t row, int K, int c, bool write, uint32_t& top, float& ss) {
         if constexpr (SRC == SRC_ADD_NORM) {
-            if constexpr (VEC == 8) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    reinterpret_cast<uint32_t*>(t.e)[i] = two_bf16(fmaf(d.at(2 * i), s.delta_scale, t.at(2 * i)), fmaf(d.at(2 * i + 1), s.delta_scale, t.at(2 * i + 1)));
-                }
-            } else {
-                t.e[0] = __float2bfloat16(fmaf(d.at(0), s.delta_scale, t.at(0)));
+            for (int i = 0; i < 4; ++i) {
+                reinterpret_cast<uint32_t*>(t.e)[i] = two_bf16(fmaf(d.at(2 * i), s.delta_scale, t.at(2 * i)), fmaf(d.at(2 * i + 1), s.delta_scale, t.at(2 * i + 1)));
             }
-            if (write) *reinterpret_cast<Block*>(s.total + row * K + c) = t;
+            if (write) t.store(s.total + row * K + c, K - c);
         }
-        if constexpr (SRC == SRC_PLAIN && VEC == 8) {   // two magnitudes at a time, as 16-bit patterns
+        if constexpr (SRC == SRC_PLAIN) {   // two magnitudes at a time, as 16-bit patterns
             const uint32_t* pairs = reinterpret_cast<const uint32_t*>(t.e);
             uint32_t m = 0u;
 #pragma unroll
@@ -188,7 +203,7 @@ struct Values {
         } else {
             float m = 0.f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
+            for (int e = 0; e < 8; ++e) {
                 float v = t.at(e);
                 if constexpr (HAS_NORM<SRC>) {
                     ss = fmaf(v, v, ss);
@@ -200,9 +215,9 @@ struct Values {
             top = max(top, __float_as_uint(m));
         }
     }
-    __device__ __forceinline__ void values(float (&v)[VEC]) const {
+    __device__ __forceinline__ void values(float (&v)[8]) const {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
+        for (int e = 0; e < 8; ++e) {
             if constexpr (HAS_NORM<SRC>) v[e] = p[e];
             else v[e] = t.at(e);
         }

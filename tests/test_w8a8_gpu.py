@@ -367,3 +367,76 @@ def test_workspace_apart(other, ffn):
     with pytest.raises(RuntimeError, match=f"needs {size} bytes"):
         call(place, size - 1)
     torch.cuda.synchronize()
+
+
+# Sizes at which clusters of 2, 3, 4 and 8 CTAs have token tiles of 16, 32, 64 and 128, several of them, the last one partly filled or with a single token, and
+# columns that the CTAs do not share evenly.
+TILED = [(95, 2624, 256), (97, 1100, 130), (26, 7168, 256), (17, 2500, 200), (60, 16384, 512), (60, 4096, 2048), (60, 4096, 4096), (31, 2000, 700), (200, 1024, 1024),
+         (225, 1000, 500), (300, 4096, 1024), (257, 4096, 1024), (290, 5760, 200), (128, 8192, 4096), (127, 6400, 4000), (65, 4096, 4096), (129, 9000, 128), (513, 300, 260),
+         (66, 1000, 1500), (128, 16384, 1500), (200, 16384, 1100), (1000, 2048, 128)]
+
+
+@pytest.mark.parametrize("rows,width,out", TILED)
+def test_linear_of_several_token_tiles(w8, rows, width, out):
+    x, q, s = ref.make(rows, width, out, seed=rows + width + out, device="cuda")
+    bias = torch.randn(out, generator=torch.Generator("cuda").manual_seed(2), device="cuda").to(BF16)
+    wide = torch.full((rows + 1, out + 3), 7.0, dtype=BF16, device="cuda")
+    y = wide[:rows, :out]
+    w8.linear(x, w8.PackedLinear(q, s), bias=bias, out=y)
+    want, tol, _ = ref.linear(x, q, s, bias)
+    near(y, want, tol)
+    assert bool((wide[rows:] == 7).all()) and bool((wide[:, out:] == 7).all())   # nothing behind the rows and columns
+
+
+@pytest.mark.parametrize("rows,width,inter", [(95, 2624, 256), (26, 7168, 250), (33, 5000, 129), (60, 4096, 1024), (200, 1024, 333), (300, 4096, 511), (290, 5760, 100), (128, 8192, 2048),
+                                              (257, 2048, 512), (66, 1000, 1500), (200, 8192, 550)])
+def test_gated_ffn_of_several_token_tiles(w8, rows, width, inter):
+    x, gate, up, down = make_ffn(rows, width, inter, rows + inter)
+    got = w8.gated_ffn(x, w8.PackedGateUp(*gate, *up), w8.PackedLinear(*down))
+    want, tol, _ = ref.ffn(x, *gate, *up, *down)
+    near(got, want, tol)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 100, 400])
+@pytest.mark.parametrize("inter", [3, 333, 1001])
+def test_gated_ffn_of_odd_widths(w8, rows, inter):
+    """Activations are padded to whole vectors: neither the padding nor rows that are NaN or zero may reach the other rows."""
+    width = 200
+    x, gate, up, down = make_ffn(rows, width, inter, rows + inter)
+    packed = w8.PackedGateUp(*gate, *up), w8.PackedLinear(*down)
+    torch.full((1 << 22,), float("nan"), device="cuda")          # what the workspace's memory may hold
+    want = w8.gated_ffn(x, *packed)
+    full, tol, _ = ref.ffn(x, *gate, *up, *down)
+    near(want, full, tol)
+    bad = x.clone()
+    bad[0, 5] = float("nan")
+    if rows > 2:
+        bad[rows // 2] = 0
+        bad[rows - 1, 0] = float("inf")
+    got = w8.gated_ffn(bad, *packed)
+    assert bool(torch.isnan(got[0]).all())
+    if rows > 2:
+        assert bool(torch.isnan(got[rows - 1]).all()) and not bool(got[rows // 2].any())
+        kept = [i for i in range(rows) if i not in (0, rows // 2, rows - 1)]
+        assert torch.equal(got[kept], want[kept])
+
+
+@pytest.mark.parametrize("rows,width", [(1, 5121), (3, 5121), (7, 8192), (400, 1025), (400, 2049), (400, 4099), (310, 8191), (300, 16383), (5, 16390), (2, 20001), (600, 256)])
+@pytest.mark.parametrize("shift", [0, 1, 4])
+def test_rows_at_odd_places(w8, rows, width, shift):
+    """Rows that start anywhere and have any width give the integers and sums of the same rows side by side."""
+    x, q, s = ref.make(rows, width, 40, seed=width + shift, device="cuda")
+    buffer = torch.full((rows * (width + 5) + shift,), float("nan"), dtype=BF16, device="cuda")
+    odd = buffer[shift:].view(rows, width + 5)[:, :width]
+    odd.copy_(x)
+    got, scale = w8.quantize(odd)
+    r, top, _ = ref.ints(x.double())
+    assert torch.equal(got.double(), r)
+    assert float(((scale.double() - top[:, 0] / 127).abs() / top[:, 0].clamp(min=1e-30)).max()) < 2.0 ** -24
+    packed = w8.PackedLinear(q, s)
+    weight = (0.5 + torch.rand(width, generator=torch.Generator("cuda").manual_seed(1), device="cuda")).to(BF16)
+    assert torch.equal(w8.linear(odd, packed), w8.linear(x.contiguous(), packed))
+    y, total = w8.linear(odd, packed, norm_weight=weight, delta=x.flip(0).contiguous(), delta_scale=0.5)
+    assert float((total != ref.residual(x, x.flip(0), 0.5)).float().mean()) < 1e-3
+    want, tol, _ = ref.linear(total, q, s, norm_weight=weight)
+    near(y, want, tol)
