@@ -24,12 +24,12 @@ namespace w8 {
 namespace {
 
 constexpr int UMMA_K = 32;
-// Warp 0 TMA, warp 1 MMA + TMEM, then the epilogue.  Two warps for each quarter of the tensor memory's lanes take turns with the tokens: one alone on
-// its scheduler waits for its own instructions most of the time, and a gate/up tile of 256 tokens took 27000 cycles beside 16400 of products at K = 4096.
-constexpr int EPI_WARPS = 8;
-constexpr int NUM_THREADS = 64 + EPI_WARPS * 32;
+// Warp 0 TMA, warp 1 MMA + TMEM, then the epilogue: on each quarter of the tensor memory's lanes up to two warps, which take turns with batches of 16
+// tokens.  (One alone waits for its own instructions most of the time: a gate/up tile of 256 tokens took 27000 cycles beside 16400 of products at
+// K = 4096.  Four: 4096 x 128 x 4096 21.7 us, two 22.0; 60 x 128 x 38000 6.4, two 6.1.)
+constexpr int BATCH = 16, MAX_PARTS = 2;
+constexpr int EPI_BUF_BYTES = 1024;    // a warp's own: 16 tokens of 32 features in bf16, or 8 in 32 bits
 constexpr int CLUSTER_THREADS = 192;   // of the cluster kernel, whose epilogue is short
-constexpr int XCH_BYTES = EPI_WARPS * gemm::EPI_WARP_BYTES;
 constexpr int CTRL_BYTES = 256;
 
 struct ProductArgs {
@@ -76,13 +76,18 @@ __device__ __forceinline__ void umma_block(uint32_t d, uint32_t wa, uint32_t xa,
     }
 }
 
+template <int MT>
+constexpr int PARTS_OF = MT / BATCH < MAX_PARTS ? MT / BATCH : MAX_PARTS;   // epilogue warps on a quarter
 template <int MT, bool PAIR>
 struct Cfg {
     static constexpr int X_ROWS = PAIR ? MT / 2 : MT;           // token rows that this CTA loads
     static constexpr int STAGE_BYTES = BLOCK_BYTES + X_ROWS * BLOCK_COLS;
     static constexpr int STAGES = PAIR ? 6 : (MT <= 16) ? 10 : (MT <= 32) ? 9 : (MT <= 64) ? 8 : (MT <= 128) ? 6 : 4;
     static constexpr int TMEM_COLS = 2 * MT;
-    static constexpr int SCALE_BYTES = EPI_WARPS * MT * 4;      // per epilogue warp the token scales of its tile
+    static constexpr int PARTS = PARTS_OF<MT>, EPI_WARPS = 4 * PARTS, THREADS = 64 + EPI_WARPS * 32;
+    static constexpr int TURNS = MT / (BATCH * PARTS);          // batches of an epilogue warp
+    static constexpr int XCH_BYTES = EPI_WARPS * EPI_BUF_BYTES;
+    static constexpr int SCALE_BYTES = EPI_WARPS * TURNS * BATCH * 4;   // per epilogue warp the scales of its tokens
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CTRL_BYTES + XCH_BYTES + SCALE_BYTES + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
@@ -134,20 +139,21 @@ __device__ __forceinline__ void store16(bf16* y, long long ldy, int N, long long
 
 // silu(gate) * up of a whole tile: lanes 0-63 hold the gate sums of 64 features, 64-127 the up sums of the same ones.  Warps q and q + 2 hand
 // each other the sums of half of the tokens of a batch, so that both compute.  fp32: what is rounded next is the row of 8-bit integers.
+// xs: the scales of this warp's batches, one after another.
 template <int MT>
 __device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act, long long ld, int N, long long row0, int n0, const float* xs, float ws_gate,
-                                          float ws_up, float* xch, int q, int half, int lane) {
-    constexpr int HB = MT >= 32 ? 16 : 8;
-    int* out = reinterpret_cast<int*>(xch) + (half * 4 + q) * (gemm::EPI_WARP_BYTES / 4) + lane;
-    const int* in = reinterpret_cast<const int*>(xch) + (half * 4 + (q ^ 2)) * (gemm::EPI_WARP_BYTES / 4) + lane;
-    const int pair_bar = 2 + half * 2 + (q & 1);
+                                          float ws_up, uint8_t* xch, int q, int part, int lane) {
+    constexpr int HB = BATCH / 2, PARTS = PARTS_OF<MT>;
+    int* out = reinterpret_cast<int*>(xch + (part * 4 + q) * EPI_BUF_BYTES) + lane;
+    const int* in = reinterpret_cast<const int*>(xch + (part * 4 + (q ^ 2)) * EPI_BUF_BYTES) + lane;
+    const int pair_bar = 2 + part * 2 + (q & 1);
     const bool gates = q < 2;
     const bool column = n0 + lane < N;
+    xs += gates ? 0 : HB;
 #pragma unroll 1
-    for (int c0 = half * 2 * HB; c0 < m_cnt; c0 += 4 * HB) {   // uniform across the warps of a half
-        uint32_t r[2 * HB];
+    for (int c0 = part * BATCH; c0 < m_cnt; c0 += PARTS * BATCH, xs += BATCH) {   // the same in both warps
+        uint32_t r[BATCH];
         ptx::tmem_ld16(t_addr + c0, r);
-        if constexpr (HB == 16) ptx::tmem_ld16(t_addr + c0 + 16, r + 16);
         ptx::tmem_wait_ld();
         // gate warps keep the first half of the tokens, up warps the second
 #pragma unroll
@@ -157,7 +163,7 @@ __device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act
         float v[HB];
 #pragma unroll
         for (int c = 0; c < HB; c += 4) {
-            const float4 s4 = *reinterpret_cast<const float4*>(xs + first + c);
+            const float4 s4 = *reinterpret_cast<const float4*>(xs + c);
             const float s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -180,35 +186,59 @@ __device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act
 // The epilogue threads of one CTA walk the segments of `it`; rank: of a pair's CTA, which has 128 of the tile's 256 weight rows.
 template <int MT, bool PAIR>
 __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint32_t tmem_base, uint64_t* acc_full, uint64_t* acc_empty,
-                                         volatile int* abort_flag, volatile int* s_last, int warp, int lane, int epi_tid, int g, int G, float* xch,
+                                         volatile int* abort_flag, volatile int* s_last, int warp, int lane, int epi_tid, int g, int G, uint8_t* xch,
                                          float* scales, int rank) {
-    constexpr int CSZ = PAIR ? 2 : 1;
+    using C = Cfg<MT, PAIR>;
+    constexpr int CSZ = PAIR ? 2 : 1, STEP = C::PARTS * BATCH, MINE = C::TURNS * BATCH;   // tokens of this warp
     const gemm::LinearArgs& w = a.sched;
-    const int q = warp & 3, row = q * 32 + lane, half = (warp - 2) >> 2;   // batches of tokens alternate between the halves
-    uint8_t* buf = reinterpret_cast<uint8_t*>(xch) + (half * 4 + q) * gemm::EPI_WARP_BYTES;
-    float* xs = scales + (half * 4 + q) * MT;
+    const int q = warp & 3, row = q * 32 + lane, part = (warp - 2) >> 2;
+    uint8_t* buf = xch + (part * 4 + q) * EPI_BUF_BYTES;
+    float* xs = scales + (part * 4 + q) * MINE;
     const bool vec = a.act == nullptr && ((reinterpret_cast<uintptr_t>(a.y) | (static_cast<uintptr_t>(a.ldy) * 2) | (static_cast<uintptr_t>(a.N) * 2)) & 15) == 0;
     const int gt = w.tail_grid > 0 ? w.tail_grid : G;
     int acc = 0;
     uint32_t acc_phase = 0;
-    int tile, kb0, kb1;
-    while (it.next(tile, kb0, kb1)) {
+    // A tile's scales (and bias) are asked for while the tile before it is on its way out (4096 x 128 x 4096: 26.4 -> 22.0 us).
+    struct Ahead {
+        int tile, kb0, kb1, m_base, n_tile;
+        float xs[(MINE + 31) / 32], ws, ws_up, bias;
+    };
+    auto look = [&](Ahead& t) {
+        if (!it.next(t.tile, t.kb0, t.kb1)) return false;
         int m_tile, n_tile;
-        gemm::tile_to_mn(w, tile, m_tile, n_tile);
-        n_tile = n_tile * CSZ + rank;
-        const int m_base = m_tile * MT;
+        gemm::tile_to_mn(w, t.tile, m_tile, n_tile);
+        t.n_tile = n_tile * CSZ + rank;
+        t.m_base = m_tile * MT;
+#pragma unroll
+        for (int i = 0; i < (MINE + 31) / 32; ++i) {
+            const int l = lane + i * 32, m = t.m_base + l / BATCH * STEP + part * BATCH + l % BATCH;
+            t.xs[i] = l < MINE && m < w.M ? a.xs[m] : 0.f;
+        }
+        const int n = t.n_tile * TILE_ROWS + row;
+        t.ws = a.ws[a.act == nullptr ? n : t.n_tile * TILE_ROWS + (row & 63)];                       // gate/up tiles: of the gate
+        t.ws_up = a.act == nullptr ? 0.f : a.ws[t.n_tile * TILE_ROWS + 64 + (row & 63)];
+        t.bias = a.act == nullptr && a.bias != nullptr && n < a.N ? __bfloat162float(a.bias[n]) : 0.f;
+        return true;
+    };
+    Ahead next;
+    bool more = look(next);
+    while (more) {
+        const int tile = next.tile, kb0 = next.kb0, kb1 = next.kb1, m_base = next.m_base, n_tile = next.n_tile;
         const int m_cnt = min(w.M - m_base, MT);
-        // scales of the tokens and of this feature, while the sums are being made
-        for (int t = lane; t < MT; t += 32) xs[t] = t < m_cnt ? a.xs[m_base + t] : 0.f;
-        const float ws = a.ws[n_tile * TILE_ROWS + (a.act == nullptr ? row : row & 63)];             // gate/up tiles: of the gate
-        const float ws_up = a.act == nullptr ? 0.f : a.ws[n_tile * TILE_ROWS + 64 + (row & 63)];
+        const float ws = next.ws, ws_up = next.ws_up, bias = next.bias;
+        __syncwarp();   // the tile before has done with the scales
+#pragma unroll
+        for (int i = 0; i < (MINE + 31) / 32; ++i) {
+            if (lane + i * 32 < MINE) xs[lane + i * 32] = next.xs[i];
+        }
         __syncwarp();
+        more = look(next);
         if (!ptx::mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag)) break;
         ptx::tc_fence_after();
         const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * MT;
         const int n0 = n_tile * TILE_ROWS + q * 32;
         int* const slot = a.partials + (static_cast<size_t>(g * CSZ + rank) * 2 + (kb0 == 0 ? 1 : 0)) * (MT * TILE_ROWS);
-        bool whole = kb0 == 0 && kb1 == w.kblocks;
+        const bool whole = kb0 == 0 && kb1 == w.kblocks;
         int first = 0, pieces = 1;
         if (!whole) {
             const long long u0 = static_cast<long long>(tile - w.wave_tiles) * w.kblocks;
@@ -216,21 +246,21 @@ __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint3
             pieces = gemm::unit_owner(u0 + w.kblocks - 1, w.total_units, gt) - first + 1;
         }
         if (a.act != nullptr) {
-            gate_tile<MT>(t_addr, m_cnt, a.act, a.ldy, a.N, m_base, n_tile * 64 + (q & 1) * 32, xs, ws, ws_up, xch, q, half, lane);
+            gate_tile<MT>(t_addr, m_cnt, a.act, a.ldy, a.N, m_base, n_tile * 64 + (q & 1) * 32, xs, ws, ws_up, xch, q, part, lane);
         } else if (whole) {
-            const float bias = a.bias != nullptr && n0 + lane < a.N ? __bfloat162float(a.bias[n0 + lane]) : 0.f;
+            const float* s = xs;
 #pragma unroll 1
-            for (int c0 = half * 16; c0 < m_cnt; c0 += 32) {
+            for (int c0 = part * BATCH; c0 < m_cnt; c0 += STEP, s += BATCH) {
                 int r[16];
                 float v[16];
                 load16(t_addr + c0, r);
                 ptx::tmem_wait_ld();
-                scale16(r, xs + c0, ws, bias, v);
+                scale16(r, s, ws, bias, v);
                 store16(a.y, a.ldy, a.N, m_base + c0, m_cnt - c0, n0, v, buf, lane, vec);
             }
         } else {
 #pragma unroll 1
-            for (int c0 = half * 16; c0 < m_cnt; c0 += 32) {
+            for (int c0 = part * BATCH; c0 < m_cnt; c0 += STEP) {
                 int r[16];
                 load16(t_addr + c0, r);
                 ptx::tmem_wait_ld();
@@ -248,48 +278,47 @@ __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint3
 
         if (!whole) {
             __threadfence();   // this thread's sums are visible before the count
-            ptx::named_bar_sync(1, EPI_WARPS * 32);
+            ptx::named_bar_sync(1, C::EPI_WARPS * 32);
             if (epi_tid == 0) *s_last = atomicAdd(&a.tickets[tile * CSZ + rank], 1) == pieces - 1;
-            ptx::named_bar_sync(1, EPI_WARPS * 32);
+            ptx::named_bar_sync(1, C::EPI_WARPS * 32);
             const bool last = *s_last != 0;
-            ptx::named_bar_sync(1, EPI_WARPS * 32);   // everyone has read s_last before it can change
+            ptx::named_bar_sync(1, C::EPI_WARPS * 32);   // everyone has read s_last before it can change
             if (last) {
                 __threadfence();
-                const float bias = a.bias != nullptr && n0 + lane < a.N ? __bfloat162float(a.bias[n0 + lane]) : 0.f;
+                const float* sc = xs;
 #pragma unroll 1
-                for (int c0 = half * 16; c0 < m_cnt; c0 += 32) {
+                for (int c0 = part * BATCH; c0 < m_cnt; c0 += STEP, sc += BATCH) {
                     int sum[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) sum[c] = 0;
 #pragma unroll 1
-                    for (int p0 = 0; p0 < pieces; p0 += 4) {
-                        int r[4][16];
+                    for (int p0 = 0; p0 < pieces; p0 += 2) {
+                        int r[2][16];
 #pragma unroll
-                        for (int s = 0; s < 4; ++s) {
+                        for (int s = 0; s < 2; ++s) {
                             const int gg = first + p0 + s;
                             const int* from = a.partials + (static_cast<size_t>(gg * CSZ + rank) * 2 + (gg == first ? 1 : 0)) * (MT * TILE_ROWS) + c0 * TILE_ROWS + row;
 #pragma unroll
                             for (int c = 0; c < 16; ++c) r[s][c] = p0 + s < pieces && c0 + c < m_cnt ? __ldcg(from + c * TILE_ROWS) : 0;
                         }
 #pragma unroll
-                        for (int s = 0; s < 4; ++s) {
+                        for (int s = 0; s < 2; ++s) {
 #pragma unroll
                             for (int c = 0; c < 16; ++c) sum[c] += r[s][c];
                         }
                     }
                     float v[16];
-                    scale16(sum, xs + c0, ws, bias, v);
+                    scale16(sum, sc, ws, bias, v);
                     store16(a.y, a.ldy, a.N, m_base + c0, m_cnt - c0, n0, v, buf, lane, vec);
                 }
             }
         }
-        __syncwarp();   // the scales may be replaced
     }
 }
 
 // Lets its successor start at once: what a successor fetches before its own wait are packed weights only.
 template <int MT, bool PAIR>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(Cfg<MT, PAIR>::THREADS, 1)
 product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const ProductArgs a) {
     using C = Cfg<MT, PAIR>;
     constexpr int CSZ = PAIR ? 2 : 1;
@@ -302,8 +331,8 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* s_last = abort_flag + 1;
-    float* xch = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE_BYTES + CTRL_BYTES);
-    float* scales = xch + XCH_BYTES / 4;
+    uint8_t* xch = smem + C::STAGES * C::STAGE_BYTES + CTRL_BYTES;
+    float* scales = reinterpret_cast<float*>(xch + C::XCH_BYTES);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? static_cast<int>(ptx::cluster_ctarank()) : 0;
@@ -318,7 +347,7 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         }
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(&acc_full[s], 1);
-            ptx::mbar_init(&acc_empty[s], CSZ * EPI_WARPS * 32);
+            ptx::mbar_init(&acc_empty[s], CSZ * C::EPI_WARPS * 32);
         }
         *abort_flag = 0;
         *s_last = 0;
@@ -642,7 +671,7 @@ void run(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int
     using C = Cfg<MT, PAIR>;
     static const bool allowed = allow_smem(product_s8_kernel<MT, PAIR>, C::SMEM_BYTES);   // the library runs on one device
     (void)allowed;
-    launch_on(product_s8_kernel<MT, PAIR>, grid, NUM_THREADS, C::SMEM_BYTES, s, PAIR ? 2 : 1, true, tw, tx, a);
+    launch_on(product_s8_kernel<MT, PAIR>, grid, C::THREADS, C::SMEM_BYTES, s, PAIR ? 2 : 1, true, tw, tx, a);
 }
 template <int MT, int CS>
 void run_cluster(const CUtensorMap& tw, const CUtensorMap& tx, const ProductArgs& a, int grid, cudaStream_t s) {
@@ -709,10 +738,10 @@ Division find_division(int M, int tiles, int kblocks, bool gated, int sms) {
             d.cluster = cs;
         }
     }
-    // Single CTAs and pairs, and whether the tiles of the last wave are cut into equal pieces: whole tiles of 64, 128, 256 and pairs, and the best cut
-    // one: 300 x 4096 x 4096 19.3, 12.6, 16.1, 15.8 (20.6) us; 1000 x 4096 x 4608 33.6, 20.8, 16.2, 16.8 (26.9); 2048 x 4096 x 4096 55.9, 36.6,
-    // 26.3, 25.7 (36.6); 4096 x 16384 x 4096 408, 233, 206, 177 (174).  Few columns, whole tiles of 16, 32, 64, 128, 256 and pairs, with the rows' kernel:
-    // 150 x 64 x 16384 13.4, 10.1, 8.5, 8.8, 7.2, 8.1; 250 x 74 x 3519 9.6, 6.7, 5.9, 7.4, 10.8, 11.8; 2000 x 512 x 2048 23.4, 15.8, 13.4, 12.0, 10.7, 11.9.
+    // Single CTAs and pairs, and whether the tiles of the last wave are cut into equal pieces.  Whole tiles of 64, 128, 256 and pairs, with the rows' kernel:
+    // 300 x 4096 x 4096 21.3, 14.4, 18.0, 18.0 us; 1000 x 4096 x 4608 37.3, 24.2, 19.6, 20.0; 2048 x 4096 x 4096 61.8, 42.1, 31.9, 30.8.  Of 16, 32, 64, 128,
+    // 256 and pairs: 150 x 64 x 16384 13.3, 9.8, 7.9, 7.9, 6.7, 7.7; 250 x 74 x 3519 9.0, 6.5, 5.9, 6.9, 9.3, 10.2; 2000 x 512 x 2048 23.7, 16.1, 12.5,
+    // 11.0, 10.5, 11.5.  Cut tiles, products alone: 4096 x 16384 x 4096 pairs 177, cut 174; but 2048 x 4096 x 4096 pairs 25.7, cut 36.6.
     // sum: over a cut tile's pieces, as far as whole tiles behind it do not hide it.
     struct Kind { int mt; bool pair; int block, out, next, sum; };
     constexpr Kind kinds[] = {{16, false, 420, 2200, 2000, 20000}, {32, false, 440, 2400, 2300, 20000}, {64, false, 420, 3200, 3200, 20000},
