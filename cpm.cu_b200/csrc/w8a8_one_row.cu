@@ -7,6 +7,7 @@
 // warp four rows (512 bytes) per k-block; S warps share the k-blocks of a group of rows and meet in shared memory, S chosen so
 // that the groups divide evenly among the SMs.  dp4a sums four products: 4 of them per 16 bytes, far below what the lanes can do at
 // the HBM rate.
+// Back to back, weights from HBM: 4096 x 4096 4.8 us (3.5 TB/s), 16384 x 4096 13.2 (5.1), gate/up 4096 x 2 * 16384 21.5 (6.2).
 #include <algorithm>
 
 #include "ptx.cuh"
