@@ -440,3 +440,54 @@ def test_rows_at_odd_places(w8, rows, width, shift):
     assert float((total != ref.residual(x, x.flip(0), 0.5)).float().mean()) < 1e-3
     want, tol, _ = ref.linear(total, q, s, norm_weight=weight)
     near(y, want, tol)
+
+
+# Up to 16 rows and one beyond: clusters of 2, 3, 4 and 8 CTAs, columns that they share unevenly, rows longer than registers hold.
+@pytest.mark.parametrize("rows", [2, 3, 4, 5, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("width,out", [(512, 128), (520, 200), (1000, 9000), (1032, 5000), (4096, 4608), (4096, 500), (16384, 4096), (16392, 130), (32768, 256), (40000, 100), (2056, 6144)])
+def test_few_rows(w8, rows, width, out):
+    x, q, s = ref.make(rows, width, out, seed=rows + width + out, device="cuda")
+    g = torch.Generator("cuda").manual_seed(rows)
+    bias = torch.randn(out, generator=g, device="cuda").to(BF16)
+    weight = (0.5 + torch.rand(width, generator=g, device="cuda")).to(BF16)
+    packed = w8.PackedLinear(q, s)
+    want, tol, _ = ref.linear(x, q, s, bias)
+    near(w8.linear(x, packed, bias=bias), want, tol)
+    want, tol, _ = ref.linear(x, q, s, norm_weight=weight)
+    near(w8.linear(x, packed, norm_weight=weight), want, tol)
+    y, total = w8.linear(x, packed, norm_weight=weight, delta=x.flip(0).contiguous(), delta_scale=0.5)
+    assert float((total != ref.residual(x, x.flip(0), 0.5)).float().mean()) < 1e-3
+    want, tol, _ = ref.linear(total, q, s, norm_weight=weight)
+    near(y, want, tol)
+
+
+@pytest.mark.parametrize("rows", [2, 5, 16])
+@pytest.mark.parametrize("width,inter", [(512, 320), (2048, 1024), (4096, 4700), (1000, 333)])
+def test_gated_ffn_of_few_rows(w8, rows, width, inter):
+    x, gate, up, down = make_ffn(rows, width, inter, rows + inter)
+    packed = w8.PackedGateUp(*gate, *up), w8.PackedLinear(*down)
+    got = w8.gated_ffn(x, *packed)
+    want, tol, _ = ref.ffn(x, *gate, *up, *down)
+    near(got, want, tol)
+    bad = x.clone()
+    bad[0, 1], bad[1] = float("inf"), 0
+    again = w8.gated_ffn(bad, *packed)
+    assert bool(torch.isnan(again[0]).all()) and not bool(again[1].any()) and torch.equal(again[2:], got[2:])
+
+
+def test_few_rows_round_exactly(w8):
+    """Behind an identity: half-way values, tiny and huge rows."""
+    width = 512
+    eye = w8.PackedLinear(torch.eye(width, dtype=torch.int8, device="cuda"), torch.ones(width, device="cuda"))
+    g = torch.Generator("cuda").manual_seed(3)
+    for rows in (2, 7, 16):
+        for top in (254.0, 3.0, 127.0, 2.0 ** -126, float(torch.finfo(BF16).max)):
+            x = (torch.randint(-127, 128, (rows, width), generator=g, device="cuda").double() / 127 * top).to(BF16)
+            x[:, 0], x[:, 1], x[:, 2] = top, top / 2, -top / 2
+            r, t, _ = ref.ints(x.double())
+            y = w8.linear(x, eye)
+            if top > 1e38 or top < 1e-30:   # the identity's outputs leave bf16's accuracy there: the rows' kernel says which integers
+                q, scale = w8.quantize(x)
+                assert torch.equal(q.double(), r) and torch.equal(y, (q.float() * scale[:, None]).to(BF16))
+            else:
+                assert torch.equal((y.double() / (t / 127)).round(), r), (rows, top)
