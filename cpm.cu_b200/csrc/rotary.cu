@@ -206,12 +206,12 @@ struct Divisor {
 struct RingArgs {
     RotaryArgs a;
     int rows, group, groups, row_bytes;
-    int turned, copied;                       // pieces of 16 rotated elements, and of 8 copied ones, per head
+    int turned, copied;                       // pieces of rotated elements (two vectors, or one where interleaved heads have an odd number), and copied vectors, per head
+    int apart;                                // of a piece's vectors: interleaved pairs lie in them, the others across them
     Divisor by_items, by_turned, by_copies, by_copied, by_values;
 };
-template <bool INTERLEAVED>
+template <bool INTERLEAVED, int VEC, bool TWO = true>
 __global__ void __launch_bounds__(256, RING_CTAS) rotary_ring_kernel(const RingArgs g) {
-    constexpr int VEC = 8;
     const RotaryArgs& a = g.a;
     const int G = g.group, pad = 2 * padded(a.half), stage_bytes = G * g.row_bytes;
     extern __shared__ __align__(128) uint8_t smem[];   // stages of G rows, then two sets of G tables
@@ -221,8 +221,6 @@ __global__ void __launch_bounds__(256, RING_CTAS) rotary_ring_kernel(const RingA
     __shared__ int abort_flag;
     const int kv_dim = a.kv_heads * a.dim, all = a.heads + a.kv_heads;
     const int items = all * g.turned, copies = all * g.copied, values = kv_dim / VEC;
-    // a piece is two vectors, this far apart: interleaved pairs lie in the vectors, the others across them
-    const int apart = INTERLEAVED ? a.dim / 2 : a.half;
     const int n = (g.groups - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1;   // groups of this CTA
     auto row_of = [&](int i, int r) { return (static_cast<long long>(blockIdx.x) + static_cast<long long>(i) * gridDim.x) * G + r; };
     auto rows_in = [&](int i) { return static_cast<int>(min(static_cast<long long>(G), g.rows - row_of(i, 0))); };
@@ -293,12 +291,12 @@ __global__ void __launch_bounds__(256, RING_CTAS) rotary_ring_kernel(const RingA
             e.load(at, a.half);
             if constexpr (INTERLEAVED) {
                 Piece<VEC, true, true> e2;
-                e2.load(at + apart, a.half);
+                if constexpr (TWO) e2.load(at + g.apart, a.half);
                 e.rotate(c, a.half, table + r * pad);
-                e2.rotate(c + apart, a.half, table + r * pad);
+                if constexpr (TWO) e2.rotate(c + g.apart, a.half, table + r * pad);
                 auto store = [&](bf16* to) {
                     e.store(to, a.half);
-                    e2.store(to + apart, a.half);
+                    if constexpr (TWO) e2.store(to + g.apart, a.half);
                 };
                 put(store, r, h, c);
             } else {
@@ -359,33 +357,40 @@ void launch_rotary(const RotaryArgs& a, int rows, bool interleaved, cudaStream_t
     // Rings where every SM has eight rows, or three groups of several short rows: 8192 rows of 32 + 2 * 8 heads of 128 35.5 us (one CTA per row 45.0),
     // of 16 + 2 * 4 interleaved 19.1 (27.5), 2000 rows of 15 + 2 * 5 heads of 80 6.8 (7.3), 8000 rows of 4 + 2 heads of 64 6.3 (9.8); but
     // 1000 rows of 32 + 2 * 8 heads of 128 7.8 (7.4), 1000 of 12 + 2 * 4 heads of 64 3.8 (3.2).
+    // (Narrower pieces where the halves of a head are no vectors of eight: 8192 rows of 3 + 2 * 3 heads of 72 7.3 (11.7), 4000 of 12 + 2 * 4 heads of 96, 24 elements
+    // rotated, 9.2 (13.4).)
     const int group = std::max(1, std::min({RING_GROUP_BYTES / row_bytes, a.half > 0 ? 256 / a.half : RING_MAX_GROUP, RING_MAX_GROUP}));
     const int groups = ceil_div(rows, group);
-    if (vec == 8 && (!interleaved || a.dim % 16 == 0) && row_bytes <= RING_MAX_ROW_BYTES && groups >= (group > 1 ? 3 : 8) * sms) {
+    const bool bulk = (bits(a.qkv) & 15) == 0 && a.ld % 8 == 0 && row_bytes % 16 == 0;   // rows may be brought by bulk copies
+    if (bulk && wide && vec >= (interleaved ? 8 : 2) && row_bytes <= RING_MAX_ROW_BYTES && groups >= (group > 1 ? 3 : 8) * sms) {
         RingArgs g;
         g.a = a;
         g.rows = rows;
         g.row_bytes = row_bytes;
         g.group = group;
         g.groups = groups;
-        g.turned = interleaved ? a.dim / 16 : a.half / 8;
-        g.copied = interleaved ? 0 : (a.dim - 2 * a.half) / 8;
+        const bool two = a.dim % 16 == 0;
+        g.apart = interleaved ? a.dim / 2 : a.half;
+        g.turned = !interleaved ? a.half / vec : two ? a.dim / 16 : a.dim / 8;
+        g.copied = interleaved ? 0 : (a.dim - 2 * a.half) / vec;
         const int all = a.heads + a.kv_heads;
         g.by_items.set(std::max(1, all * g.turned));
         g.by_turned.set(std::max(1, g.turned));
         g.by_copies.set(std::max(1, all * g.copied));
         g.by_copied.set(std::max(1, g.copied));
-        g.by_values.set(std::max(1, a.kv_heads * a.dim / 8));
+        g.by_values.set(std::max(1, a.kv_heads * a.dim / vec));
         const int smem = RING_STAGES * g.group * row_bytes + 2 * g.group * 2 * padded(a.half) * static_cast<int>(sizeof(float));
+        auto* kernel = interleaved ? (two ? rotary_ring_kernel<true, 8> : rotary_ring_kernel<true, 8, false>) : vec == 8 ? rotary_ring_kernel<false, 8> : vec == 4 ? rotary_ring_kernel<false, 4> : rotary_ring_kernel<false, 2>;
         static const bool allowed = [] {   // the library runs on one device
-            for (auto* kernel : {rotary_ring_kernel<true>, rotary_ring_kernel<false>}) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
+            for (auto* k : {rotary_ring_kernel<true, 8>, rotary_ring_kernel<true, 8, false>, rotary_ring_kernel<false, 8>, rotary_ring_kernel<false, 4>, rotary_ring_kernel<false, 2>}) {
+                CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
+            }
             return true;
         }();
         (void)allowed;
         const int per_sm = std::max(1, std::min(RING_CTAS, 227 * 1024 / (smem + 1280)));
         const int grid = std::min(g.groups, per_sm * sms);
-        if (interleaved) go(rotary_ring_kernel<true>, grid, 256, smem, g);
-        else go(rotary_ring_kernel<false>, grid, 256, smem, g);
+        go(kernel, grid, 256, smem, g);
         return;
     }
     const int threads = pieces >= 256 ? 256 : (pieces + 31) / 32 * 32;

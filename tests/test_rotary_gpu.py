@@ -191,3 +191,11 @@ def test_refusals_on_the_gpu(rotary):
         rotary.append(qkv, 1, 1, 64, inv, pos, k, k, pos)
     with pytest.raises(RuntimeError, match="query part"):
         rotary.append(qkv, 1, 1, 64, inv, pos, k, v, pos, out=qkv[:, 64:128])
+
+
+@pytest.mark.parametrize("heads,kv,dim,rot,interleaved", [(3, 3, 72, 72, False), (3, 3, 72, 72, True), (12, 4, 72, 36, False), (4, 4, 80, 20, False), (4, 4, 80, 40, False), (12, 4, 96, 24, False),
+                                                          (6, 2, 112, 28, False), (2, 1, 8, 4, False), (1, 1, 40, 40, True), (1, 1, 8, 8, True), (2, 1, 72, 18, False), (2, 2, 256, 4, False)])
+@pytest.mark.parametrize("rows,pad", [(4100, 0), (6001, 8), (6001, 4), (4100, 1)])
+def test_many_rows_of_narrow_pieces(rotary, heads, kv, dim, rot, interleaved, rows, pad):
+    """Rings of rows whose heads' halves are not vectors of eight; rows at places that no bulk copy reaches."""
+    test_rotation(rotary, heads, kv, dim, rot, interleaved, rows, pad)
