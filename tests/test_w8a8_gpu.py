@@ -491,3 +491,38 @@ def test_few_rows_round_exactly(w8):
                 assert torch.equal(q.double(), r) and torch.equal(y, (q.float() * scale[:, None]).to(BF16))
             else:
                 assert torch.equal((y.double() / (t / 127)).round(), r), (rows, top)
+
+
+CAPTURE = """
+import torch, cpmcu.w8a8 as w8, cpmcu.rotary as rotary
+BF16 = torch.bfloat16
+w8.quantize(torch.ones(1, 8, dtype=BF16, device="cuda"))          # the one call outside of a capture
+packed, x = {}, {}
+shapes = [(1, 640, 300), (3, 1500, 400), (77, 2000, 500), (300, 1024, 1024), (90, 300, 20000), (1100, 512, 2048), (128, 5120, 4096)]
+for s in shapes:
+    g = torch.Generator("cuda").manual_seed(sum(s))
+    x[s] = torch.randn(s[0], s[1], generator=g, device="cuda").to(BF16)
+    packed[s] = w8.PackedLinear(torch.randint(-127, 128, (s[2], s[1]), generator=g, device="cuda").to(torch.int8), torch.rand(s[2], generator=g, device="cuda"))
+qkv = torch.randn(5000, 6 * 72, device="cuda").to(BF16)
+inv, pos, cache = torch.rand(36, device="cuda"), torch.arange(5000, device="cuda", dtype=torch.int32), torch.zeros(2, 5000, 72, dtype=BF16, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = {s: w8.linear(x[s], packed[s]) for s in shapes}
+    q = rotary.append(qkv, 4, 1, 72, inv, pos, cache[0], cache[1], pos)
+for _ in range(3): graph.replay()
+torch.cuda.synchronize()
+for s in shapes: assert torch.equal(y[s], w8.linear(x[s], packed[s])), s
+assert torch.equal(q, rotary.append(qkv, 4, 1, 72, inv, pos, cache[0], cache[1], pos))
+print("same")
+"""
+
+
+def test_first_calls_of_their_sizes_in_a_capture():
+    """Kernels and divisions of work that the process has not used before are set up inside a capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "cpm.cu_b200")
+    out = subprocess.run([sys.executable, "-c", CAPTURE], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
