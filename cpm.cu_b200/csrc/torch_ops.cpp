@@ -7,7 +7,8 @@
 #include <limits>
 #include <string>
 
-#include <ATen/ops/empty.h>
+#include <ATen/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -83,8 +84,17 @@ float real(PyObject* o) {
     return static_cast<float>(v);
 }
 
+// Makes a GPU current for a while.
+struct Device {
+    c10::cuda::OptionalCUDAGuard guard;
+    explicit Device(int device) {
+        if (c10::cuda::current_device() != device) guard.set_index(static_cast<c10::DeviceIndex>(device));
+    }
+};
+// Straight from torch's allocator: the dispatcher's way there takes longer than the allocation.
 at::Tensor empty(std::initializer_list<int64_t> shape, at::ScalarType type, int device) {
-    return at::empty(at::IntArrayRef(shape), at::TensorOptions().dtype(type).device(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))));
+    const Device current(device);
+    return at::detail::empty_generic(at::IntArrayRef(shape), c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
 }
 
 // Runs an entry point with GPU `device` current, on torch's current stream of it, without the interpreter's lock.  What torch throws in there is
@@ -95,8 +105,7 @@ void run(int device, F&& call) {
     std::string text;
     Py_BEGIN_ALLOW_THREADS
     try {
-        c10::cuda::OptionalCUDAGuard guard;
-        if (c10::cuda::current_device() != device) guard.set_index(static_cast<c10::DeviceIndex>(device));
+        const Device current(device);
         code = call(static_cast<void*>(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()));
         if (code < 0) text = cpmcu_last_error();
     } catch (const std::exception& e) {
@@ -141,10 +150,12 @@ Input input_of(PyObject* x, int width, int out, int device, PyObject* norm, PyOb
     }
     return in;
 }
-at::Tensor workspace_of(const Input& in, int out, int width, int inter, long& bytes) {
+c10::DataPtr workspace_of(const Input& in, int out, int width, int inter, long& bytes) {
     bytes = cpmcu_w8a8_workspace_bytes(in.rows, out, width, inter);
     if (bytes < 0) refuse(cpmcu_last_error());
-    return bytes == 0 ? at::Tensor() : empty({bytes}, at::kByte, in.device);
+    if (bytes == 0) return c10::DataPtr();
+    const Device current(in.device);
+    return c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes));
 }
 PyObject* result_of(const Input& in) {
     PyObject* y = THPVariable_Wrap(in.out);
@@ -182,12 +193,12 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
             check(bias, "bias", at::kBFloat16, {out}, device);
         }
         long bytes;
-        const at::Tensor ws = workspace_of(in, out, width, 0, bytes);
+        const c10::DataPtr ws = workspace_of(in, out, width, 0, bytes);
         if (in.rows > 0) {
             run(device, [&](void* stream) {
                 return cpmcu_w8a8_linear(in.x.data_ptr(), ld_of(in.x), packed, in.pointer(bias), in.pointer(in.norm), in.eps, in.pointer(in.delta), in.delta_scale,
                                          in.total.defined() ? in.total.data_ptr() : nullptr, in.out.data_ptr(), ld_of(in.out), in.rows, out, width,
-                                         ws.defined() ? ws.data_ptr() : nullptr, bytes, stream);
+                                         ws.get(), bytes, stream);
             });
         }
         return result_of(in);
@@ -201,12 +212,12 @@ PyObject* ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int width = small(a[3], "width"), inter = small(a[4], "inter"), device = small(a[5], "device");
         Input in = input_of(a[0], width, width, device, a[6], a[7], a[8], a[9], a[10]);
         long bytes;
-        const at::Tensor ws = workspace_of(in, width, width, inter, bytes);
+        const c10::DataPtr ws = workspace_of(in, width, width, inter, bytes);
         if (in.rows > 0) {
             run(device, [&](void* stream) {
                 return cpmcu_w8a8_ffn(in.x.data_ptr(), ld_of(in.x), gate_up, down, in.pointer(in.norm), in.eps, in.pointer(in.delta), in.delta_scale,
                                       in.total.defined() ? in.total.data_ptr() : nullptr, in.out.data_ptr(), ld_of(in.out), in.rows, width, inter,
-                                      ws.defined() ? ws.data_ptr() : nullptr, bytes, stream);
+                                      ws.get(), bytes, stream);
             });
         }
         return result_of(in);
