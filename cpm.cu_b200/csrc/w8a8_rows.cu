@@ -7,7 +7,7 @@
 //
 // Bound: bytes.  One CTA per row, which stays in registers between the pass that finds the maximum and the one that rounds; rows too
 // long for that are read twice.  A row with an infinity or a NaN gets the scale NaN and integers 0, a row of zeros the scale 0.
-// 4096 rows of 16384: 36.8 us (5.5 TB/s), of 4096: 10.2 (4.9); 60 rows of 16384: 2.8, of 4096: 1.6.
+// 4096 rows of 16384: 36.8 us (5.5 TB/s), of 4096: 9.1 (5.5); 60 rows of 16384: 2.8, of 4096: 1.6.
 #include "w8a8_rows.cuh"
 
 namespace w8 {
@@ -111,13 +111,23 @@ void run_quantize(const QuantizeArgs& a, int rows, cudaStream_t s) {
         else go(quantize_kernel<SRC, 0, WIDE>, 256, 1);
         return;
     }
-    // many rows: several CTAs beside one another on an SM
-    if (vectors <= 256) go(quantize_kernel<SRC, 1, WIDE>, vectors, 1);
-    else if (vectors <= 512) go(quantize_kernel<SRC, 2, WIDE>, vectors, 2);
-    else if (vectors <= 1024) go(quantize_kernel<SRC, 4, WIDE>, vectors, 4);
-    else if (vectors <= 2048 && SRC == SRC_PLAIN) go(quantize_kernel<SRC_PLAIN, 8, WIDE>, vectors, 8);
-    else if (vectors <= 2048) go(quantize_kernel<SRC, 4, WIDE>, vectors, 4);
-    else go(quantize_kernel<SRC, 0, WIDE>, 256, 1);
+    // Many rows: several CTAs beside one another on an SM; where they come in more than eight rounds, fewer threads with more vectors each (4096 rows of 4096: four
+    // vectors 9.1 us, two 10.0, behind a norm 23.1, 25.2; of 2048: two 5.5, one 6.2; but 400 of 4096: four 2.6, two 2.2; 2000 of 1536 behind a norm: two
+    // 11.6, one 10.8).  Element by element the fewest (2000 rows of 5121 behind a residual sum and a norm: two 44.8, four 52.2).
+    const bool rounds = rows > 8 * runtime().num_sms;
+    if (vectors > 2048) {
+        go(quantize_kernel<SRC, 0, WIDE>, 256, 1);
+    } else if (vectors > 1024) {
+        if constexpr (SRC == SRC_PLAIN) go(quantize_kernel<SRC, 8, WIDE>, vectors, 8);
+        else go(quantize_kernel<SRC, 4, WIDE>, vectors, 4);
+    } else if constexpr (WIDE) {
+        if (vectors > (rounds ? 256 : 512)) go(quantize_kernel<SRC, 4, WIDE>, vectors, 4);
+        else if (vectors > (SRC == SRC_PLAIN && rounds ? 128 : 256)) go(quantize_kernel<SRC, 2, WIDE>, vectors, 2);
+        else go(quantize_kernel<SRC, 1, WIDE>, vectors, 1);
+    } else {
+        if (vectors > 512) go(quantize_kernel<SRC, 2, WIDE>, vectors, 2);
+        else go(quantize_kernel<SRC, 1, WIDE>, vectors, 1);
+    }
 }
 template <Source SRC>
 void run_quantize(const QuantizeArgs& a, int rows, bool wide, cudaStream_t s) {

@@ -526,3 +526,29 @@ def test_first_calls_of_their_sizes_in_a_capture():
     root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "cpm.cu_b200")
     out = subprocess.run([sys.executable, "-c", CAPTURE], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows,width", [(1300, 800), (1300, 1600), (1300, 2400), (1300, 4808), (1300, 8800), (1200, 16000), (1200, 17000), (1300, 4801), (1300, 9001), (310, 1600), (310, 4104), (310, 6000)])
+def test_many_rows(w8, rows, width):
+    """Each way of sharing a row among threads, for plain rows, rows behind a norm, and behind a residual sum and a norm."""
+    x, q, s = ref.make(rows, width, 24, seed=rows + width, device="cuda")
+    got, scale = w8.quantize(x)
+    r, top, _ = ref.ints(x.double())
+    assert torch.equal(got.double(), r)
+    packed = w8.PackedLinear(q, s)
+    weight = (0.5 + torch.rand(width, generator=torch.Generator("cuda").manual_seed(1), device="cuda")).to(BF16)
+    for more in ({}, {"norm_weight": weight}):
+        want, tol, _ = ref.linear(x, q, s, **more)
+        near(w8.linear(x, packed, **more), want, tol)
+    y, total = w8.linear(x, packed, norm_weight=weight, delta=x.flip(0).contiguous(), delta_scale=0.5)
+    assert float((total != ref.residual(x, x.flip(0), 0.5)).float().mean()) < 1e-3
+    want, tol, _ = ref.linear(total, q, s, norm_weight=weight)
+    near(y, want, tol)
+
+
+@pytest.mark.parametrize("rows,inter", [(1300, 1600), (1300, 4096), (1200, 9000), (310, 2400)])
+def test_gated_ffn_of_many_rows(w8, rows, inter):
+    x, gate, up, down = make_ffn(rows, 256, inter, rows + inter)
+    got = w8.gated_ffn(x, w8.PackedGateUp(*gate, *up), w8.PackedLinear(*down))
+    want, tol, _ = ref.ffn(x, *gate, *up, *down)
+    near(got, want, tol)
