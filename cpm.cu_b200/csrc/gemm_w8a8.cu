@@ -235,7 +235,8 @@ __device__ __forceinline__ void epilogue(const ProductArgs& a, SegIter it, uint3
         }
         __syncwarp();
         more = look(next);
-        if (!ptx::mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag)) break;
+        // A wait that ran out (the launch reports it) does not end the walk: the warps meet at barriers further down, and must all come to each of them.
+        ptx::mbar_wait_warp(&acc_full[acc], acc_phase, abort_flag);
         ptx::tc_fence_after();
         const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * MT;
         const int n0 = n_tile * TILE_ROWS + q * 32;
