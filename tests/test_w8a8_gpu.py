@@ -552,3 +552,32 @@ def test_gated_ffn_of_many_rows(w8, rows, inter):
     got = w8.gated_ffn(x, w8.PackedGateUp(*gate, *up), w8.PackedLinear(*down))
     want, tol, _ = ref.ffn(x, *gate, *up, *down)
     near(got, want, tol)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 60, 300, 1000])
+def test_activations_keep_32_bits(rows):
+    """silu(gate) * up as the down projection's rounding finds it, at the start of the workspace.  Integers of the rows and powers of two as scales make gate
+    and up exact; what is left are an exponential (off by one unit in the last place at most, 2^-23), a sum, a quotient and a product of 2^-24 each:
+    less than 6 * 2^-24 relative."""
+    width, inter = 512, 320
+    g = torch.Generator("cuda").manual_seed(rows)
+    x = torch.randint(-127, 128, (rows, width), generator=g, device="cuda")
+    x[:, 7] = 127                                                       # the scale of every row is 1
+    weights = [torch.zeros(inter, width, dtype=torch.int8, device="cuda") for _ in range(2)]
+    at = torch.randint(0, width, (inter,), generator=g, device="cuda")   # each feature is one column of x
+    for w in weights:
+        w[torch.arange(inter, device="cuda"), at] = torch.randint(1, 128, (inter,), generator=g, device="cuda").to(torch.int8)
+    scales = [torch.full((inter,), 2.0 ** -9, device="cuda"), torch.full((inter,), 2.0 ** -12, device="cuda")]
+    down = torch.ones(width, inter, dtype=torch.int8, device="cuda")
+    import cpmcu.w8a8 as w8
+    gate_up, down = w8.PackedGateUp(weights[0], scales[0], weights[1], scales[1]), w8.PackedLinear(down, torch.ones(width, device="cuda"))
+    size = C.load().cpmcu_w8a8_workspace_bytes(rows, width, width, inter)
+    workspace = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    xb, y = x.to(BF16), torch.empty(rows, width, dtype=BF16, device="cuda")
+    C.call("cpmcu_w8a8_ffn", xb.data_ptr(), width, gate_up.data.data_ptr(), down.data.data_ptr(), None, 1e-5, None, 1.0, None, y.data_ptr(), width, rows, width, inter,
+           workspace.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    got = workspace[:rows * inter * 4].view(torch.float32).view(rows, inter).double()
+    a, b = (x.double() @ w.double().t() * s.double() for w, s in zip(weights, scales))
+    want = a / (1 + torch.exp(-a)) * b
+    off = ((got - want).abs() / want.abs().clamp(min=1e-30)).max()
+    assert float(off) < 6 * 2.0 ** -24, float(off) * 2 ** 24
