@@ -1,6 +1,7 @@
 // extern "C" surface of the operators that run on a stream of the caller's choice (part 4 of include/cpmcu_b200.h): 8-bit linear
 // layers and rotations.  They launch and return: no allocation, no synchronisation, no host copy.
 #include <algorithm>
+#include <climits>
 #include <initializer_list>
 
 #include "../../include/cpmcu_b200.h"
@@ -70,6 +71,8 @@ void require_sizes(const char* what, int rows, int N, int K) {
     const long long tiles = (static_cast<long long>(N) + 63) / 64;
     require(tiles * (w8::pad_cols(K) / w8::BLOCK_COLS) <= (1ll << 23) && ((static_cast<long long>(rows) + 15) / 16) * tiles <= (1ll << 30), what, "too many tiles");
 }
+// Products count rows in whole token tiles, of up to 256, and in 32 bits.
+void require_rows(const char* what, int rows) { require(rows <= INT_MAX - 256, what, "too many rows"); }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -205,6 +208,7 @@ int cpmcu_w8a8_quantize(const void* x, long long ldx, int rows, int K, void* q, 
 long cpmcu_w8a8_workspace_bytes(int rows, int N, int K, int inter) {
     return guarded([&]() -> long {
         require_sizes("w8a8_workspace_bytes", rows, N, K);
+        require_rows("w8a8_workspace_bytes", rows);
         CPM_REQUIRE(inter >= 0, "w8a8_workspace_bytes: inter must not be negative");
         if (inter > 0) {
             require_sizes("w8a8_workspace_bytes", rows, inter, K);
@@ -218,6 +222,7 @@ int cpmcu_w8a8_linear(const void* x, long long ldx, const void* packed, const vo
                       float delta_scale, void* total, void* y, long long ldy, int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream) {
     return guarded([&] {
         require_sizes("w8a8_linear", rows, N, K);
+        require_rows("w8a8_linear", rows);
         if (rows == 0) return 0;
         require_packed("w8a8_linear", packed);
         const w8::RowSource src = source_of("w8a8_linear", x, ldx, norm, eps, delta, delta_scale, total, rows, K, y, ldy, N);
@@ -255,6 +260,7 @@ int cpmcu_w8a8_ffn(const void* x, long long ldx, const void* gate_up, const void
     return guarded([&] {
         require_sizes("w8a8_ffn", rows, inter, K);
         require_sizes("w8a8_ffn", rows, K, inter);
+        require_rows("w8a8_ffn", rows);
         if (rows == 0) return 0;
         require_packed("w8a8_ffn", gate_up);
         require_packed("w8a8_ffn", down);

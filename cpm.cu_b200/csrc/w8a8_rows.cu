@@ -36,7 +36,8 @@ __global__ void __launch_bounds__(MOST_THREADS<VPT>) quantize_kernel(const Quant
     if (static_cast<int>(threadIdx.x) * 8 < a.K && threadIdx.x % 8 == 0) Values<SRC, WIDE>::ask(a.src, row, a.K, threadIdx.x * 8);
     grid_dep_wait();
     grid_dep_trigger();
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < a.n_clear; i += gridDim.x * blockDim.x) a.clear[i] = 0;
+    // 64 bits: there may be more than 2^31 threads
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < a.n_clear; i += static_cast<long long>(gridDim.x) * blockDim.x) a.clear[i] = 0;
     Values<SRC, WIDE> kept[VPT > 0 ? VPT : 1];
     float ss = 0.f;
     uint32_t top = 0u;

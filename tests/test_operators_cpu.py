@@ -153,3 +153,11 @@ def test_plain_forms_agree_with_torch():
     step = v.abs().amax(1, keepdim=True) / 127
     # the factor of the norm cancels in the integers but for its rounding at exact ties
     assert torch.allclose(y, (v / step).round() * step @ (q.double() * s.double()[:, None]).t(), rtol=1e-6, atol=float(step.max()) * 1e-3)
+
+
+def test_more_rows_than_are_counted_in_32_bits():
+    top = 2 ** 31 - 1
+    assert "too many rows" in linear(rows=top)
+    assert "too many rows" in refused("cpmcu_w8a8_ffn", X, 64, PACKED, PACKED, None, 1e-5, None, 1.0, None, Y, 64, top, 64, 64, WS, 1 << 30, None)
+    assert C.load().cpmcu_w8a8_workspace_bytes(top, 32, 64, 0) == -1 and b"too many rows" in C.load().cpmcu_last_error()
+    assert "too many rows" not in linear(rows=top - 256, ws=None)

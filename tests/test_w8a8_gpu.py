@@ -581,3 +581,22 @@ def test_activations_keep_32_bits(rows):
     want = a / (1 + torch.exp(-a)) * b
     off = ((got - want).abs() / want.abs().clamp(min=1e-30)).max()
     assert float(off) < 6 * 2.0 ** -24, float(off) * 2 ** 24
+
+
+def test_more_rows_than_threads_are_counted_in_32_bits(w8):
+    """Narrow rows: 2^26 of them and more have over 2^31 threads."""
+    rows, width, out = (1 << 26) + 300, 8, 8
+    last, q, s = ref.make(300, width, out, seed=1, device="cuda")
+    x = torch.zeros(rows, width, dtype=BF16, device="cuda")
+    x[-300:] = last
+    got, scale = w8.quantize(x)
+    few, few_scale = w8.quantize(last)
+    assert torch.equal(got[-300:], few) and torch.equal(scale[-300:], few_scale)
+    assert int(got[:-300].count_nonzero()) == 0 and int(scale[:-300].count_nonzero()) == 0
+    del got, scale
+    packed = w8.PackedLinear(q, s)
+    guard = torch.full((1 << 28,), 7, dtype=torch.uint8, device="cuda")   # memory beside the workspace
+    y = w8.linear(x, packed)
+    want, tol, _ = ref.linear(last, q, s)
+    near(y[-300:], want, tol)
+    assert int(y[:-300].count_nonzero()) == 0 and bool((guard == 7).all())
