@@ -7,7 +7,7 @@ scale each, exact 32-bit sums (formulas at cpmcu_w8a8_linear in include/cpmcu_b2
     y = gated_ffn(x, PackedGateUp(...), w_down)    # down(silu(gate(x)) * up(x))
 
 Calls run on torch's current stream and return without waiting; they can be captured into CUDA graphs (after a first call outside of one).  What a
-kernel reports (a wait that ran out) is raised by cpmcu.C.stream_check.  Packed weights are not to be written to.
+kernel reports (a wait that ran out) is raised by cpmcu.C.stream_check.  Packed weights are not to be written to; copy.deepcopy and pickle keep them whole.
 """
 import torch
 
@@ -53,15 +53,24 @@ class _Packed:
     def __init__(self, out, width, gated, parts):
         if out < 1 or width < 1:
             raise ValueError("weights must not be empty")
-        self.out, self.width, self.device = out, width, parts[0][0].device
-        self.index = parts[0][0].get_device()
+        self.out, self.width, device = out, width, parts[0][0].device
         n = C.load().cpmcu_w8a8_packed_bytes(out, width, int(gated))
         if n < 0:
             raise ValueError(C.load().cpmcu_last_error().decode())
-        self.data = torch.empty(n, dtype=torch.uint8, device=self.device)
-        self.ptr = self.data.data_ptr()
+        self.data = torch.empty(n, dtype=torch.uint8, device=device)
         for part, (q, scale) in enumerate(parts, start=int(gated)):
-            _call("cpmcu_w8a8_pack", self.device, q.data_ptr(), scale.data_ptr(), out, width, part, self.ptr)
+            _call("cpmcu_w8a8_pack", device, q.data_ptr(), scale.data_ptr(), out, width, part, self.data.data_ptr())
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def __setstate__(self, state):
+        """Of copies and of unpickled weights.  Their bytes were not written by the packing kernel, and a call fetches weights before it waits for the work
+        ahead of it in the stream: they have to be there."""
+        self.__dict__.update(state)
+        if self.data.is_cuda:
+            torch.cuda.current_stream(self.data.device).synchronize()
 
 
 class PackedLinear(_Packed):
@@ -102,7 +111,7 @@ def linear(x, weight, bias=None, norm_weight=None, eps=1e-5, delta=None, delta_s
     returned.  bias [out] bf16.  x (and out) may be rows of a wider matrix."""
     if type(weight) is not PackedLinear:
         raise ValueError("weight must be a PackedLinear")
-    return _ops.linear(x, weight.ptr, weight.out, weight.width, weight.index, bias, norm_weight, eps, delta, delta_scale, out)
+    return _ops.linear(x, weight.data, weight.out, weight.width, bias, norm_weight, eps, delta, delta_scale, out)
 
 
 def gated_ffn(x, gate_up, down, norm_weight=None, eps=1e-5, delta=None, delta_scale=1.0, out=None):
@@ -110,6 +119,6 @@ def gated_ffn(x, gate_up, down, norm_weight=None, eps=1e-5, delta=None, delta_sc
     if type(gate_up) is not PackedGateUp or type(down) is not PackedLinear:
         raise ValueError("gate_up must be a PackedGateUp and down a PackedLinear")
     width, inter = gate_up.width, gate_up.out
-    if down.width != inter or down.out != width or down.index != gate_up.index:
-        raise ValueError(f"down must be [{width}, {inter}] on {gate_up.device}")
-    return _ops.ffn(x, gate_up.ptr, down.ptr, width, inter, gate_up.index, norm_weight, eps, delta, delta_scale, out)
+    if down.width != inter or down.out != width:
+        raise ValueError(f"down must be [{width}, {inter}]")
+    return _ops.ffn(x, gate_up.data, down.data, width, inter, norm_weight, eps, delta, delta_scale, out)

@@ -35,6 +35,7 @@ const char* dtype_text(at::ScalarType t) {
         case at::kBFloat16: return "torch.bfloat16";
         case at::kFloat: return "torch.float32";
         case at::kInt: return "torch.int32";
+        case at::kByte: return "torch.uint8";
         default: return c10::toString(t);
     }
 }
@@ -167,6 +168,15 @@ PyObject* result_of(const Input& in) {
     return both;
 }
 
+// Packed weights: their bytes, and the GPU they are on.
+const at::Tensor& packed_of(PyObject* o, const char* what, int out, int width, bool gated, int device = -1) {
+    const at::Tensor& t = tensor_of(o, what);
+    const long bytes = cpmcu_w8a8_packed_bytes(out, width, gated);
+    if (bytes < 0) refuse(cpmcu_last_error());
+    check(t, what, at::kByte, {bytes}, device);
+    return t;
+}
+
 template <Py_ssize_t N, typename F>
 PyObject* guarded(Py_ssize_t n, F&& f) {
     if (n != N) return PyErr_Format(PyExc_TypeError, "%zd arguments wanted, got %zd", N, n);
@@ -181,22 +191,23 @@ PyObject* guarded(Py_ssize_t n, F&& f) {
     return nullptr;
 }
 
-// linear(x, packed address, out, width, device, bias, norm_weight, eps, delta, delta_scale, out tensor)
+// linear(x, packed weights, out, width, bias, norm_weight, eps, delta, delta_scale, out tensor)
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded<11>(n, [&] {
-        const void* packed = reinterpret_cast<const void*>(whole(a[1]));
-        const int out = small(a[2], "out"), width = small(a[3], "width"), device = small(a[4], "device");
-        Input in = input_of(a[0], width, out, device, a[6], a[7], a[8], a[9], a[10]);
+    return guarded<10>(n, [&] {
+        const int out = small(a[2], "out"), width = small(a[3], "width");
+        const at::Tensor& packed = packed_of(a[1], "weight", out, width, false);
+        const int device = packed.get_device();
+        Input in = input_of(a[0], width, out, device, a[5], a[6], a[7], a[8], a[9]);
         at::Tensor bias;
-        if (a[5] != Py_None) {
-            bias = tensor_of(a[5], "bias");
+        if (a[4] != Py_None) {
+            bias = tensor_of(a[4], "bias");
             check(bias, "bias", at::kBFloat16, {out}, device);
         }
         long bytes;
         const c10::DataPtr ws = workspace_of(in, out, width, 0, bytes);
         if (in.rows > 0) {
             run(device, [&](void* stream) {
-                return cpmcu_w8a8_linear(in.x.data_ptr(), ld_of(in.x), packed, in.pointer(bias), in.pointer(in.norm), in.eps, in.pointer(in.delta), in.delta_scale,
+                return cpmcu_w8a8_linear(in.x.data_ptr(), ld_of(in.x), packed.data_ptr(), in.pointer(bias), in.pointer(in.norm), in.eps, in.pointer(in.delta), in.delta_scale,
                                          in.total.defined() ? in.total.data_ptr() : nullptr, in.out.data_ptr(), ld_of(in.out), in.rows, out, width,
                                          ws.get(), bytes, stream);
             });
@@ -205,17 +216,19 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// ffn(x, gate/up address, down address, width, inter, device, norm_weight, eps, delta, delta_scale, out tensor)
+// ffn(x, packed gate/up weights, packed down weights, width, inter, norm_weight, eps, delta, delta_scale, out tensor)
 PyObject* ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded<11>(n, [&] {
-        const void *gate_up = reinterpret_cast<const void*>(whole(a[1])), *down = reinterpret_cast<const void*>(whole(a[2]));
-        const int width = small(a[3], "width"), inter = small(a[4], "inter"), device = small(a[5], "device");
-        Input in = input_of(a[0], width, width, device, a[6], a[7], a[8], a[9], a[10]);
+    return guarded<10>(n, [&] {
+        const int width = small(a[3], "width"), inter = small(a[4], "inter");
+        const at::Tensor& gate_up = packed_of(a[1], "gate_up", inter, width, true);
+        const int device = gate_up.get_device();
+        const at::Tensor& down = packed_of(a[2], "down", width, inter, false, device);
+        Input in = input_of(a[0], width, width, device, a[5], a[6], a[7], a[8], a[9]);
         long bytes;
         const c10::DataPtr ws = workspace_of(in, width, width, inter, bytes);
         if (in.rows > 0) {
             run(device, [&](void* stream) {
-                return cpmcu_w8a8_ffn(in.x.data_ptr(), ld_of(in.x), gate_up, down, in.pointer(in.norm), in.eps, in.pointer(in.delta), in.delta_scale,
+                return cpmcu_w8a8_ffn(in.x.data_ptr(), ld_of(in.x), gate_up.data_ptr(), down.data_ptr(), in.pointer(in.norm), in.eps, in.pointer(in.delta), in.delta_scale,
                                       in.total.defined() ? in.total.data_ptr() : nullptr, in.out.data_ptr(), ld_of(in.out), in.rows, width, inter,
                                       ws.get(), bytes, stream);
             });

@@ -161,3 +161,20 @@ def test_more_rows_than_are_counted_in_32_bits():
     assert "too many rows" in refused("cpmcu_w8a8_ffn", X, 64, PACKED, PACKED, None, 1e-5, None, 1.0, None, Y, 64, top, 64, 64, WS, 1 << 30, None)
     assert C.load().cpmcu_w8a8_workspace_bytes(top, 32, 64, 0) == -1 and b"too many rows" in C.load().cpmcu_last_error()
     assert "too many rows" not in linear(rows=top - 256, ws=None)
+
+
+def test_packed_weights_off_the_gpu_are_refused():
+    """What torch.load with a map_location gives: weights whose bytes are somewhere else."""
+    from cpmcu import w8a8 as W
+    w = W.PackedLinear.__new__(W.PackedLinear)
+    w.__setstate__({"out": 4, "width": 4, "data": torch.zeros(128 * 128 + 512, dtype=torch.uint8)})
+    with pytest.raises(ValueError, match="weight must be on the GPU"):
+        W.linear(torch.zeros(1, 4, dtype=torch.bfloat16), w)
+    w.data = w.data[1:]
+    with pytest.raises(ValueError, match="weight must be torch.uint8"):
+        W.linear(torch.zeros(1, 4, dtype=torch.bfloat16), w)
+    g = W.PackedGateUp.__new__(W.PackedGateUp)
+    g.__setstate__({"out": 4, "width": 4, "data": torch.zeros(128 * 128 + 512, dtype=torch.uint8)})
+    w.data = g.data
+    with pytest.raises(ValueError, match="gate_up must be on the GPU"):
+        W.gated_ffn(torch.zeros(1, 4, dtype=torch.bfloat16), g, w)

@@ -600,3 +600,26 @@ def test_more_rows_than_threads_are_counted_in_32_bits(w8):
     want, tol, _ = ref.linear(last, q, s)
     near(y[-300:], want, tol)
     assert int(y[:-300].count_nonzero()) == 0 and bool((guard == 7).all())
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_copies_of_packed_weights_are_their_own(w8, rows):
+    """copy.deepcopy and pickle, used at once; the copy outlives the original, and changes of one leave the other alone."""
+    import copy
+    import pickle
+    x, q, s = ref.make(rows, 512, 300, seed=rows, device="cuda")
+    gate_up, down = w8.PackedGateUp(q, s, q.flip(0).contiguous(), s), w8.PackedLinear(*ref.make(1, 300, 512, 1, "cuda")[1:])
+    linear = w8.PackedLinear(q, s)
+    want, block = w8.linear(x, linear), w8.gated_ffn(x, gate_up, down)
+    for again in (copy.deepcopy, copy.copy, lambda w: pickle.loads(pickle.dumps(w))):
+        a, g, d = again(linear), again(gate_up), again(down)
+        assert a.device == linear.device and (a.data.data_ptr() == linear.data.data_ptr()) == (again is copy.copy)
+        assert torch.equal(w8.linear(x, a), want) and torch.equal(w8.gated_ffn(x, g, d), block)
+    a = copy.deepcopy(linear)
+    a.data.zero_()
+    torch.cuda.synchronize()
+    assert torch.equal(w8.linear(x, linear), want) and not bool(w8.linear(x, a).any())
+    a = copy.deepcopy(linear)
+    linear.data.zero_()
+    torch.cuda.synchronize()
+    assert torch.equal(w8.linear(x, a), want)
