@@ -17,7 +17,7 @@ OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(OUT_DIR, "libcpmcu_b200.so")
 OPS = os.path.join(OUT_DIR, "_ops.so")   # Python module over the library, for torch tensors
 SOURCES = ["runtime.cu", "gemm_umma.cu", "gemm_pair.cu", "gemm_w4_umma.cu", "elementwise.cu", "tree_attn.cu", "pair_attn.cu", "draft_tree.cu", "accept.cu",
-           "marlin_unpack.cu", "sparse_select.cu", "sparse_stage1.cu", "layered_ops.cu", "plain_ops.cu", "one_row.cu", "tanh_rows.cu", "recurrence.cu", "moe.cu", "engine.cu", "engine_layered.cu", "w8a8_rows.cu", "w8a8_one_row.cu", "gemm_w8a8.cu", "rotary.cu", "capi_ops.cu", "capi.cu"]
+           "marlin_unpack.cu", "sparse_select.cu", "sparse_stage1.cu", "layered_ops.cu", "plain_ops.cu", "one_row.cu", "tanh_rows.cu", "recurrence.cu", "moe.cu", "engine.cu", "engine_layered.cu", "w8a8_rows.cu", "w8a8_one_row.cu", "gemm_w8a8.cu", "rotary.cu", "op_errors.cu", "capi_ops.cu", "capi.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--threads", "2"]
 # extra defines for instrumented builds, e.g. CPMCU_BUILD_DEFINES="-DCPMCU_W4_PROFILE=1"

@@ -322,7 +322,8 @@ def profile(on):
 
 
 def stream_check(stream=0):
-    """Waits for a stream (a cudaStream_t; 0: the legacy default stream) and raises what the operators of cpmcu.w8a8 and cpmcu.rotary reported."""
+    """Waits for a stream (a cudaStream_t; 0: the legacy default stream) and raises what the operators of cpmcu.w8a8 and cpmcu.rotary have reported on it since
+    its last check; what launches of captured graphs reported is raised once on every stream, since a graph may run on any."""
     call("cpmcu_stream_check", stream or None)
 
 

@@ -5,6 +5,7 @@
 #include <initializer_list>
 
 #include "../../include/cpmcu_b200.h"
+#include "op_errors.cuh"
 #include "rotary.cuh"
 #include "w8a8.cuh"
 
@@ -155,14 +156,12 @@ extern "C" {
 
 int cpmcu_stream_check(void* stream) {
     return guarded([&] {
-        Runtime& rt = runtime();
         require_device("stream_check");
-        int flags = 0;
-        CUDA_CHECK(cudaStreamSynchronize(stream_of(stream)));
-        CUDA_CHECK(cudaMemcpyAsync(&flags, rt.d_op_error, sizeof(int), cudaMemcpyDeviceToHost, stream_of(stream)));
-        CUDA_CHECK(cudaMemsetAsync(rt.d_op_error, 0, sizeof(int), stream_of(stream)));
-        CUDA_CHECK(cudaStreamSynchronize(stream_of(stream)));
-        if (flags != 0) throw std::runtime_error("cpmcu_b200: kernel error flags " + std::to_string(flags));
+        const OpErrors e = new_op_errors(stream_of(stream));
+        if ((e.own | e.shared) != 0) {
+            throw std::runtime_error("cpmcu_b200: kernel error flags " + std::to_string(e.own | e.shared) +
+                                     (e.shared != 0 ? ", of launches of captured graphs, on this stream or another one, " + std::to_string(e.shared) : ""));
+        }
         return 0;
     });
 }
@@ -344,7 +343,7 @@ int cpmcu_rotary_append(const void* qkv, long long ld, int rows, int heads, int 
         a.ldq = heads > 0 ? ldq : 0;
         a.k_cache = static_cast<bf16*>(k_cache); a.v_cache = static_cast<bf16*>(v_cache);
         a.cache_rows = cache_rows; a.slots = slots;
-        a.error = runtime().d_op_error;
+        a.errors = op_counters(stream_of(stream));
         launch_rotary(a, rows, interleaved != 0, stream_of(stream));
         return 0;
     });

@@ -75,7 +75,7 @@ struct Runtime {
     cudaStream_t stream = nullptr;
     int* d_error = nullptr;  // device error word, or-ed into by kernels
     int* h_error = nullptr;  // pinned copy of it
-    int* d_op_error = nullptr;  // the same for operators on the caller's streams (capi_ops.cu)
+    unsigned long long* d_op_errors = nullptr;  // counters of the operators on the caller's streams (op_errors.cuh)
     unsigned* d_accept_ticket = nullptr;  // CTAs of the acceptance kernel that have read the tree (zero between launches)
     int num_sms = 148;
     int device = 0;
@@ -98,6 +98,7 @@ struct ProfileScope {
 };
 Runtime& runtime();          // lazily initialised, one per process
 int read_and_clear_error();  // synchronises the stream
+size_t op_errors_bytes();
 
 // Kernel launch with programmatic dependent launch enabled: the grid may start
 // while its predecessor in the stream drains; every kernel here executes

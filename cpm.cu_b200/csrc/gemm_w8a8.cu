@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "gemm_common.cuh"
+#include "op_errors.cuh"
 #include "row_ops.cuh"
 #include "w8a8.cuh"
 
@@ -44,7 +45,7 @@ struct ProductArgs {
     float* act;
     int* partials;
     int* tickets;
-    int* error;
+    OpCount* errors;
 };
 
 // kind::i8, both operands signed, K-major, int32 accumulator: bits [4,6) D (2 = s32), [7,10) A (1 = s8), [10,13) B, [17,23) N>>3, [24,29) M>>4
@@ -480,7 +481,7 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         if constexpr (PAIR) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
         else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
-    if (threadIdx.x == 0 && *abort_flag) atomicOr(a.error, ERR_GEMM_TIMEOUT);
+    if (threadIdx.x == 0 && *abort_flag) report(a.errors, OP_TIMEOUT);
 }
 
 // A tile per cluster: CTA `rank` of CS has k-blocks [rank * kblocks / CS, (rank + 1) * kblocks / CS).  Each CTA sends each peer that peer's share of the tokens
@@ -657,7 +658,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, Cfg<MT, false>::TMEM_COLS);
     }
-    if (threadIdx.x == 0 && *abort_flag) atomicOr(a.error, ERR_GEMM_TIMEOUT);
+    if (threadIdx.x == 0 && *abort_flag) report(a.errors, OP_TIMEOUT);
 }
 
 // ---------------------------------------------------------------- host
@@ -847,7 +848,7 @@ void launch_product(const Product& p, cudaStream_t s) {
     a.y = p.y; a.ldy = p.ldy; a.act = p.act;
     a.partials = static_cast<int*>(p.partials);
     a.tickets = p.tickets;
-    a.error = runtime().d_op_error;
+    a.errors = op_counters(s);
     const CUtensorMap tw = map_rows(p.w.blocks, static_cast<long long>(p.w.tiles) * p.w.kblocks * TILE_ROWS, BLOCK_COLS, TILE_ROWS);
     const CUtensorMap tx = map_rows(p.q, p.M, static_cast<long long>(p.w.kblocks) * BLOCK_COLS, d.pair ? d.mt / 2 : d.mt);
     if (d.cluster > 0) {

@@ -1,0 +1,112 @@
+// Host side of op_errors.cuh.
+#include "op_errors.cuh"
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+#include <unordered_map>
+
+namespace {
+
+constexpr int SETS = 1024;   // set 0 is shared; streams beyond the last one use it too
+
+struct Known {
+    int set = 0;
+    OpCount own[OP_ERROR_KINDS] = {}, shared[OP_ERROR_KINDS] = {};   // told so far
+};
+struct Registry {
+    std::mutex lock;
+    std::unordered_map<unsigned long long, Known> streams;   // by id
+    int sets = 1;
+};
+Registry& registry() {
+    static Registry r;
+    return r;
+}
+
+OpCount* counters(int set) { return runtime().d_op_errors + set * OP_ERROR_KINDS; }
+
+Known& known(Registry& r, unsigned long long id) {   // the lock is held
+    const auto [at, fresh] = r.streams.try_emplace(id);
+    if (fresh && r.sets < SETS) at->second.set = r.sets++;
+    return at->second;
+}
+
+// Whether s is in a capture, and else its id, by the driver's own entry points: 24 ns, through the runtime's 80, on every launch that may report.  They want
+// a current context, which a thread that has not called the runtime yet lacks.
+struct StreamQuery {
+    CUresult (*capturing)(CUstream, CUstreamCaptureStatus*) = nullptr;
+    CUresult (*id)(CUstream, unsigned long long*) = nullptr;
+    StreamQuery() {
+        auto find = [](const char* name, auto& fn) {
+            void* p = nullptr;
+            cudaDriverEntryPointQueryResult found;
+            if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+            fn = reinterpret_cast<std::decay_t<decltype(fn)>>(p);
+        };
+        find("cuStreamIsCapturing", capturing);
+        find("cuStreamGetId", id);
+    }
+};
+bool id_outside_captures(cudaStream_t s, unsigned long long& id) {
+    static const StreamQuery ask;
+    CUstreamCaptureStatus state;
+    if (ask.capturing != nullptr && ask.id != nullptr && ask.capturing(s, &state) == CUDA_SUCCESS) {
+        if (state != CU_STREAM_CAPTURE_STATUS_NONE) return false;
+        if (ask.id(s, &id) == CUDA_SUCCESS) return true;
+    }
+    cudaStreamCaptureStatus capture;
+    if (cudaStreamIsCapturing(s, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone && cudaStreamGetId(s, &id) == cudaSuccess) return true;
+    cudaGetLastError();   // what is wrong with the stream the launch will say
+    return false;
+}
+
+// KernelError bits of the counters that grew
+int grown(const OpCount* now, OpCount* told) {
+    constexpr int bit[OP_ERROR_KINDS] = {ERR_GEMM_TIMEOUT, ERR_KV_OVERFLOW};
+    int bits = 0;
+    for (int k = 0; k < OP_ERROR_KINDS; ++k) {
+        if (now[k] > told[k]) bits |= bit[k];
+        told[k] = std::max(told[k], now[k]);   // of two checks at once the later read may come here first
+    }
+    return bits;
+}
+
+}  // namespace
+
+size_t op_errors_bytes() { return sizeof(OpCount) * SETS * OP_ERROR_KINDS; }
+
+OpCount* op_counters(cudaStream_t s) {
+    unsigned long long id;
+    if (!id_outside_captures(s, id)) return counters(0);
+    Registry& r = registry();
+    std::lock_guard<std::mutex> hold(r.lock);
+    const auto at = r.streams.find(id);
+    if (at != r.streams.end()) return counters(at->second.set);
+    return counters(r.sets < SETS ? known(r, id).set : 0);
+}
+
+OpErrors new_op_errors(cudaStream_t s) {
+    cudaStreamCaptureStatus capture;
+    CUDA_CHECK(cudaStreamIsCapturing(s, &capture));
+    CPM_REQUIRE(capture == cudaStreamCaptureStatusNone, "stream_check: the stream is being captured");
+    unsigned long long id;
+    CUDA_CHECK(cudaStreamGetId(s, &id));
+    Registry& r = registry();
+    int set;
+    {
+        std::lock_guard<std::mutex> hold(r.lock);
+        set = known(r, id).set;
+    }
+    OpCount own[OP_ERROR_KINDS], shared[OP_ERROR_KINDS];
+    CUDA_CHECK(cudaStreamSynchronize(s));
+    CUDA_CHECK(cudaMemcpyAsync(own, counters(set), sizeof(own), cudaMemcpyDeviceToHost, s));
+    CUDA_CHECK(cudaMemcpyAsync(shared, counters(0), sizeof(shared), cudaMemcpyDeviceToHost, s));
+    CUDA_CHECK(cudaStreamSynchronize(s));
+    std::lock_guard<std::mutex> hold(r.lock);
+    Known& k = known(r, id);
+    OpErrors e;
+    e.shared = grown(shared, k.shared);
+    if (set != 0) e.own = grown(own, k.own);
+    return e;
+}

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     for (int t = threadIdx.x; t < a.half; t += blockDim.x) fill(table, t, a.half, pos, turns_of(a.inv_freq[t]), a.factor);
     if (slot >= a.cache_rows) {   // memory stays intact; the host hears of it
         slot = -1;
-        if (threadIdx.x == 0) atomicOr(a.error, ERR_KV_OVERFLOW);
+        if (threadIdx.x == 0) report(a.errors, OP_KV_OVERFLOW);
     }
     const bool keep = slot >= 0;
     bf16 *k_row = a.k_cache + slot * kv_dim, *v_row = a.v_cache + slot * kv_dim;
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(256, RING_CTAS) rotary_ring_kernel(const RingA
         if (static_cast<int>(threadIdx.x) < G) {
             if (slot >= a.cache_rows) {   // memory stays intact; the host hears of it
                 slot = -1;
-                atomicOr(a.error, ERR_KV_OVERFLOW);
+                report(a.errors, OP_KV_OVERFLOW);
             }
             slots[i & 1][threadIdx.x] = slot;
         }
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(256, RING_CTAS) rotary_ring_kernel(const RingA
     if (abort_flag) {   // copies in flight land before the CTA retires
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) {}
-        if (threadIdx.x == 0) atomicOr(a.error, ERR_GEMM_TIMEOUT);
+        if (threadIdx.x == 0) report(a.errors, OP_TIMEOUT);
     }
 }
 

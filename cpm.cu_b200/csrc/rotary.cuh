@@ -1,6 +1,6 @@
 // Rotation of fused q/k/v rows with their append to a cache, for any layout of the pairs (rotary.cu).
 #pragma once
-#include "common.cuh"
+#include "op_errors.cuh"
 
 struct RotaryArgs {
     const bf16* qkv = nullptr;        // rows of heads + 2 kv_heads heads of `dim`, ld elements apart
@@ -15,7 +15,7 @@ struct RotaryArgs {
     bf16 *k_cache = nullptr, *v_cache = nullptr;   // [cache_rows, kv_heads * dim]
     int cache_rows = 0;
     const int32_t* slots = nullptr;
-    int* error = nullptr;
+    OpCount* errors = nullptr;
 };
 int rotary_max_pairs();
 void launch_rotary(const RotaryArgs& a, int rows, bool interleaved, cudaStream_t s);

@@ -46,10 +46,11 @@ Runtime make_runtime() {
     rt.num_sms = prop.multiProcessorCount;
     rt.pdl = (getenv("CPMCU_NO_PDL") == nullptr);
     CUDA_CHECK(cudaStreamCreate(&rt.stream));
-    CUDA_CHECK(cudaMalloc(&rt.d_error, 2 * sizeof(int)));
-    CUDA_CHECK(cudaMemset(rt.d_error, 0, 2 * sizeof(int)));
-    rt.d_op_error = rt.d_error + 1;
-    CUDA_CHECK(cudaMallocHost(&rt.h_error, 2 * sizeof(int)));
+    CUDA_CHECK(cudaMalloc(&rt.d_error, sizeof(int)));
+    CUDA_CHECK(cudaMemset(rt.d_error, 0, sizeof(int)));
+    CUDA_CHECK(cudaMalloc(&rt.d_op_errors, op_errors_bytes()));
+    CUDA_CHECK(cudaMemset(rt.d_op_errors, 0, op_errors_bytes()));
+    CUDA_CHECK(cudaMallocHost(&rt.h_error, sizeof(int)));
     CUDA_CHECK(cudaMalloc(&rt.d_accept_ticket, sizeof(unsigned)));
     CUDA_CHECK(cudaMemset(rt.d_accept_ticket, 0, sizeof(unsigned)));
     return rt;

@@ -473,7 +473,9 @@ int cpmcu_accept_fixup(int tree_size, int32_t* pred, const int32_t* gt, const in
  * capture).  All pointers are DEVICE memory of the GPU that was current at the library's first call; it has to be current.  A workspace is scratch
  * of one call: its contents before do not matter and nothing in it is kept, but no other call may use it until this one has ended on the
  * device (calls of one stream may share it; graphs that share it must not run at the same time).  No reference counterparts.
- * Errors that kernels find are reported by cpmcu_stream_check, which waits for the stream; the outputs are then not to be used. */
+ * Errors that kernels find are reported by cpmcu_stream_check, which waits for the stream: those of calls on this stream since its last check, whose
+ * outputs are then not to be used.  Checks of other streams change nothing in that.  A captured graph may run on any stream, so what its launches find is
+ * reported once to every stream that is checked afterwards.  A stream in a capture is refused, and the capture goes on. */
 int cpmcu_stream_check(void* stream);
 
 /* Linear layers in 8-bit integers (weights and activations).

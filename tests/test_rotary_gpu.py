@@ -199,3 +199,117 @@ def test_refusals_on_the_gpu(rotary):
 def test_many_rows_of_narrow_pieces(rotary, heads, kv, dim, rot, interleaved, rows, pad):
     """Rings of rows whose heads' halves are not vectors of eight; rows at places that no bulk copy reaches."""
     test_rotation(rotary, heads, kv, dim, rot, interleaved, rows, pad)
+
+
+def beyond(rotary, stream=None):
+    """A call whose slots lie behind its cache, on `stream`."""
+    qkv = torch.zeros(2, 3 * 64, device="cuda").to(BF16)
+    inv = torch.ones(32, device="cuda")
+    pos = torch.arange(2, dtype=I32, device="cuda")
+    k, v = torch.zeros(2, 1, 64, dtype=BF16, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream or torch.cuda.current_stream()):
+        rotary.append(qkv, 1, 1, 64, inv, pos, k, v, pos)
+    return qkv, inv, pos, k, v
+
+
+def test_a_check_tells_its_own_stream_s_errors(rotary):
+    import cpmcu.C as C
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    C.stream_check(a.cuda_stream)
+    for _ in range(3):
+        beyond(rotary, b)
+        b.synchronize()
+        C.stream_check(a.cuda_stream)                                 # the other stream's is neither told here
+        C.stream_check()
+        with pytest.raises(RuntimeError, match="error flags 8"):      # nor taken away
+            C.stream_check(b.cuda_stream)
+        C.stream_check(b.cuda_stream)
+    # reports that arrive while other streams are being checked
+    for _ in range(20):
+        with torch.cuda.stream(b):
+            torch.cuda._sleep(200000)
+        held = beyond_behind(rotary, b)
+        for _ in range(20):
+            C.stream_check(a.cuda_stream)
+        with pytest.raises(RuntimeError, match="error flags 8"):
+            C.stream_check(b.cuda_stream)
+        del held
+
+
+def beyond_behind(rotary, stream):
+    """The same without a synchronisation ahead of it."""
+    with torch.cuda.stream(stream):
+        qkv, inv, pos = torch.zeros(2, 3 * 64, dtype=BF16, device="cuda"), torch.ones(32, device="cuda"), torch.arange(2, dtype=I32, device="cuda")
+        k, v = torch.zeros(2, 1, 64, dtype=BF16, device="cuda")
+        rotary.append(qkv, 1, 1, 64, inv, pos, k, v, pos)
+    return qkv, inv, pos, k, v
+
+
+def test_checks_from_several_threads_lose_nothing(rotary):
+    import threading
+    import cpmcu.C as C
+    told, failed = [0] * 4, []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            for n in range(40):
+                held = beyond_behind(rotary, stream) if n % 2 else None
+                try:
+                    C.stream_check(stream.cuda_stream)
+                except RuntimeError as e:
+                    assert "error flags 8" in str(e)
+                    told[i] += 1
+                del held
+        except BaseException as e:   # noqa: B036 (shown by the assertion below)
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and told == [20] * 4
+
+
+GRAPH = """
+import torch, cpmcu.C as C, cpmcu.rotary as rotary
+BF16, I32 = torch.bfloat16, torch.int32
+qkv, inv, pos = torch.zeros(2, 192, dtype=BF16, device="cuda"), torch.ones(32, device="cuda"), torch.arange(2, dtype=I32, device="cuda")
+k, v = torch.zeros(2, 1, 64, dtype=BF16, device="cuda")
+slots = torch.zeros(2, dtype=I32, device="cuda")
+slots[1] = -1
+def check(stream):
+    try: C.stream_check(stream.cuda_stream)
+    except RuntimeError as e: return str(e)
+    return ""
+rotary.append(qkv, 1, 1, 64, inv, pos, k, v, slots)
+a, b, late = (torch.cuda.Stream() for _ in range(3))
+assert check(a) == check(b) == ""
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    assert "being captured" in check(torch.cuda.current_stream())    # and the capture goes on
+    q = rotary.append(qkv, 1, 1, 64, inv, pos, k, v, slots)
+for _ in range(2):
+    slots.fill_(1)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a): graph.replay()
+    a.synchronize()
+    assert "flags 8" in check(a) and check(a) == ""
+    assert "flags 8" in check(b) and check(b) == ""    # it could have run there
+    slots.fill_(-1)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a): graph.replay()
+    assert check(a) == check(b) == ""
+assert "captured graphs" in check(late) and check(late) == ""
+print("told")
+"""
+
+
+def test_errors_of_captured_graphs():
+    import os
+    import subprocess
+    import sys
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "cpm.cu_b200")
+    out = subprocess.run([sys.executable, "-c", GRAPH], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "told" in out.stdout, out.stderr[-2000:]
