@@ -1,6 +1,7 @@
 // Python module cpmcu._ops: the operators on the caller's streams (part 4 of include/cpmcu_b200.h) for torch tensors.  Checks of arguments, outputs and
 // workspaces of torch's allocator, and torch's current stream, in one call: through ctypes the same takes 4 to 6 us more, as long as the launch and
-// longer than many of the kernels run (one token's product 7.9 us a call that way).  Refusals are ValueErrors, what the library reports is a RuntimeError.
+// longer than many of the kernels run (one token's product 7.9 us a call that way).  Refusals are ValueErrors, what the library reports is a
+// RuntimeError, and torch's allocator without memory torch.OutOfMemoryError.
 #include <Python.h>
 
 #include <initializer_list>
@@ -177,6 +178,15 @@ const at::Tensor& packed_of(PyObject* o, const char* what, int out, int width, b
     return t;
 }
 
+void out_of_memory(const char* text) {   // torch.OutOfMemoryError
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch != nullptr ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    PyErr_Clear();
+    PyErr_SetString(type != nullptr ? type : PyExc_RuntimeError, text);
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
+}
+
 template <Py_ssize_t N, typename F>
 PyObject* guarded(Py_ssize_t n, F&& f) {
     if (n != N) return PyErr_Format(PyExc_TypeError, "%zd arguments wanted, got %zd", N, n);
@@ -185,6 +195,8 @@ PyObject* guarded(Py_ssize_t n, F&& f) {
     } catch (const Raised& e) {
         PyErr_SetString(e.type, e.text.c_str());
     } catch (const PythonError&) {
+    } catch (const c10::OutOfMemoryError& e) {
+        out_of_memory(e.what_without_backtrace());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     }

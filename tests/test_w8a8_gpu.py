@@ -623,3 +623,17 @@ def test_copies_of_packed_weights_are_their_own(w8, rows):
     linear.data.zero_()
     torch.cuda.synchronize()
     assert torch.equal(w8.linear(x, a), want)
+
+
+def test_outputs_and_workspaces_that_do_not_fit(w8):
+    """torch's own exception, as from any other call; the next call runs."""
+    rows, out = 1 << 22, 100000
+    x = torch.ones(rows, 1, dtype=BF16, device="cuda")
+    wide = w8.PackedLinear(torch.ones(out, 1, dtype=torch.int8, device="cuda"), torch.ones(out, device="cuda"))
+    with pytest.raises(torch.OutOfMemoryError):                     # 839 GB of outputs
+        w8.linear(x, wide)
+    gate_up = w8.PackedGateUp(*[t for _ in range(2) for t in (torch.ones(out, 1, dtype=torch.int8, device="cuda"), torch.ones(out, device="cuda"))])
+    down = w8.PackedLinear(torch.ones(1, out, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"))
+    with pytest.raises(torch.OutOfMemoryError):                     # 1.7 TB of activations
+        w8.gated_ffn(x, gate_up, down)
+    assert bool((w8.linear(x[:5], wide) == 1).all())
