@@ -153,10 +153,10 @@ Input input_of(PyObject* x, int width, int out, int device, PyObject* norm, PyOb
     return in;
 }
 c10::DataPtr workspace_of(const Input& in, int out, int width, int inter, long& bytes) {
+    const Device current(in.device);   // also of the question: the division of the work asks the GPU what it holds
     bytes = cpmcu_w8a8_workspace_bytes(in.rows, out, width, inter);
     if (bytes < 0) refuse(cpmcu_last_error());
     if (bytes == 0) return c10::DataPtr();
-    const Device current(in.device);
     return c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes));
 }
 PyObject* result_of(const Input& in) {
