@@ -112,6 +112,7 @@ _SIGNATURES = {
     "cpmcu_w8a8_pack": (_c_int, [_c_void_p] * 2 + [_c_int] * 3 + [_c_void_p] * 2),
     "cpmcu_w8a8_quantize": (_c_int, [_c_void_p, _c_longlong, _c_int, _c_int] + [_c_void_p] * 3),
     "cpmcu_w8a8_workspace_bytes": (ctypes.c_long, [_c_int] * 4),
+    "cpmcu_debug_w8a8_division": (_c_int, [_c_int] * 4 + [_c_void_p]),
     "cpmcu_w8a8_linear": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 3 + [_c_float, _c_void_p, _c_float] + [_c_void_p] * 2 + [_c_longlong] + [_c_int] * 3 +
                           [_c_void_p, _c_longlong, _c_void_p]),
     "cpmcu_w8a8_ffn": (_c_int, [_c_void_p, _c_longlong] + [_c_void_p] * 3 + [_c_float, _c_void_p, _c_float] + [_c_void_p] * 2 + [_c_longlong] + [_c_int] * 3 +

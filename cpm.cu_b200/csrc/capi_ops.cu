@@ -217,6 +217,19 @@ long cpmcu_w8a8_workspace_bytes(int rows, int N, int K, int inter) {
     });
 }
 
+int cpmcu_debug_w8a8_division(int rows, int N, int K, int gated, int32_t* out) {
+    return guarded([&] {
+        require_sizes("debug_w8a8_division", rows, N, K);
+        require_rows("debug_w8a8_division", rows);
+        CPM_REQUIRE(rows >= 2 && out != nullptr, "debug_w8a8_division: products of two rows and more are divided");
+        require_device("debug_w8a8_division");
+        int32_t d[6];
+        w8::product_division(rows, N, K, gated != 0, d);
+        std::copy(d, d + 6, out);
+        return 0;
+    });
+}
+
 int cpmcu_w8a8_linear(const void* x, long long ldx, const void* packed, const void* bias, const void* norm, float eps, const void* delta,
                       float delta_scale, void* total, void* y, long long ldy, int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream) {
     return guarded([&] {

@@ -829,6 +829,12 @@ Scratch product_scratch(int M, int N, int K) {
     return s;
 }
 
+void product_division(int M, int N, int K, bool gated, int32_t (&out)[6]) {
+    const Division d = divide(M, tiles_of(N, gated), pad_cols(K) / BLOCK_COLS, gated);
+    const int32_t v[6] = {d.mt, d.m_tiles, d.cluster, d.pair, d.cut, d.workers};
+    std::copy(v, v + 6, out);
+}
+
 void launch_product(const Product& p, cudaStream_t s) {
     const bool gated = p.act != nullptr;
     const Division d = divide(p.M, p.w.tiles, p.w.kblocks, gated);

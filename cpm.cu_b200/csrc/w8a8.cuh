@@ -62,6 +62,8 @@ struct Scratch {                    // what cut tiles need; gate/up tiles are ne
     int tickets = 0;
 };
 Scratch product_scratch(int M, int N, int K);
+// How a product is divided: token tile, token tiles, CTAs of a cluster (0: none), pairs of CTAs, cut tiles, and clusters, pairs or CTAs (for tests)
+void product_division(int M, int N, int K, bool gated, int32_t (&out)[6]);
 void launch_product(const Product& p, cudaStream_t s);
 // one row, straight from its source
 void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const bf16* bias, bf16* y, float* act, cudaStream_t s);

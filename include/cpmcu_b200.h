@@ -497,6 +497,9 @@ int cpmcu_w8a8_pack(const void* q, const float* scale, int N, int K, int part, v
 int cpmcu_w8a8_quantize(const void* x, long long ldx, int rows, int K, void* q, float* scale, void* stream);
 /* Bytes of the workspace of a linear layer (inter 0), or of a feed-forward block (N = K = its width); 256-byte aligned. */
 long cpmcu_w8a8_workspace_bytes(int rows, int N, int K, int inter);
+/* How the tensor cores' part of a layer of 2 rows and more is divided (gated: of its gate/up product): out HOST int32[6] = token tile, token tiles, CTAs that share
+ * a tile in a cluster (0: no clusters), 1 for pairs of CTAs, 1 where the tiles of the last wave are cut along K, and the number of clusters, pairs or CTAs. */
+int cpmcu_debug_w8a8_division(int rows, int N, int K, int gated, int32_t* out);
 /* y [rows, N], rows ldy apart; x [rows, K], rows ldx apart; bias [N] bf16 or NULL. */
 int cpmcu_w8a8_linear(const void* x, long long ldx, const void* packed, const void* bias, const void* norm, float eps, const void* delta,
                       float delta_scale, void* total, void* y, long long ldy, int rows, int N, int K, void* workspace, long long workspace_bytes, void* stream);

@@ -637,3 +637,84 @@ def test_outputs_and_workspaces_that_do_not_fit(w8):
     with pytest.raises(torch.OutOfMemoryError):                     # 1.7 TB of activations
         w8.gated_ffn(x, gate_up, down)
     assert bool((w8.linear(x[:5], wide) == 1).all())
+
+
+def division(rows, width, out, gated=False):
+    """(token tile, CTAs of a cluster, pairs of CTAs, cut tiles), and whether there are more tiles than run at once"""
+    import ctypes
+    d = (ctypes.c_int32 * 6)()
+    C.call("cpmcu_debug_w8a8_division", rows, out, width, int(gated), ctypes.cast(d, ctypes.c_void_p))
+    tiles = -(-out // (64 if gated else 128))
+    return (d[0], d[2], d[3], d[4]), d[1] * (tiles // 2 if d[3] else tiles) > d[5]
+
+
+# Every way in which a product is divided, with what find_division() makes of the sizes (148 SMs) and whether whole waves of tiles are ahead: token tiles and
+# features that are partly filled, columns that end inside a block.
+DIVISIONS = [(2, 300, 40, (16, 0, 0, 0), False), (2, 131072, 40, (16, 0, 0, 1), False), (2, 1024, 8192, (16, 2, 0, 0), False), (2, 1024, 4608, (16, 3, 0, 0), False),
+             (2, 1020, 40, (16, 4, 0, 0), False), (2, 2048, 40, (16, 8, 0, 0), False), (3000, 300, 40, (32, 0, 0, 0), False), (17, 131072, 40, (32, 0, 0, 1), False),
+             (2047, 1024, 40, (32, 2, 0, 0), False), (1300, 1024, 40, (32, 3, 0, 0), False), (700, 1024, 40, (32, 4, 0, 0), False), (257, 2048, 40, (32, 8, 0, 0), False),
+             (3000, 300, 130, (64, 0, 0, 0), False), (40, 131072, 40, (64, 0, 0, 1), False), (140, 12000, 6624, (64, 0, 0, 1), True), (3000, 2048, 40, (64, 2, 0, 0), False),
+             (1300, 2048, 130, (64, 3, 0, 0), False), (2047, 4096, 40, (64, 4, 0, 0), False), (700, 8192, 40, (64, 8, 0, 0), False), (200, 300, 5000, (128, 0, 0, 0), False),
+             (700, 131072, 40, (128, 0, 0, 1), False), (3870, 12000, 566, (128, 0, 0, 1), True), (3000, 8192, 130, (128, 2, 0, 0), False), (70, 4096, 5000, (128, 3, 0, 0), False),
+             (3000, 8192, 40, (128, 4, 0, 0), False), (1300, 16384, 40, (128, 8, 0, 0), False), (4096, 300, 513, (256, 0, 0, 0), False), (2047, 131072, 40, (256, 0, 0, 1), False),
+             (140, 33000, 4760, (256, 0, 0, 1), False), (1320, 6000, 3362, (256, 0, 0, 1), True), (513, 4096, 8100, (256, 0, 1, 0), True), (4096, 4096, 4608, (256, 0, 1, 0), True),
+             (260, 33000, 3828, (256, 0, 1, 1), False), (1300, 131072, 130, (256, 0, 1, 1), False), (810, 12000, 4993, (256, 0, 1, 1), True), (2500, 16384, 5000, (256, 0, 1, 1), True)]
+
+
+@pytest.mark.parametrize("rows,width,out,kind,waves", DIVISIONS)
+def test_every_division_of_a_product(w8, rows, width, out, kind, waves):
+    assert division(rows, width, out) == (kind, waves)
+    x, q, s = ref.make(rows, width, out, seed=rows + width + out, device="cuda")
+    bias = torch.randn(out, generator=torch.Generator("cuda").manual_seed(2), device="cuda").to(BF16)
+    packed = w8.PackedLinear(q, s)
+    want, tol, _ = ref.linear(x, q, s, bias)
+    for pad in (3, 8 + (-out) % 8):             # rows element by element, and in vectors
+        wide = torch.full((rows + 1, out + pad), 7.0, dtype=BF16, device="cuda")
+        y = w8.linear(x, packed, bias=bias, out=wide[:rows, :out])
+        near(y, want, tol)
+        assert bool((wide[rows:] == 7).all()) and bool((wide[:, out:] == 7).all())   # nothing behind the rows and columns
+        assert torch.equal(w8.linear(x, packed, bias=bias), y)                       # the same again
+
+
+@pytest.mark.parametrize("rows,width,inter,kind", [(2, 1024, 4096, (16, 2, 0, 0)), (17, 300, 5000, (32, 0, 0, 0)), (40, 300, 5000, (64, 0, 0, 0)), (70, 300, 5000, (128, 0, 0, 0)),
+                                                   (200, 300, 5000, (256, 0, 0, 0)), (257, 8192, 1000, (128, 2, 0, 0)), (200, 4096, 1280, (128, 3, 0, 0)),
+                                                   (1300, 16384, 40, (128, 8, 0, 0)), (513, 4096, 4090, (256, 0, 1, 0)), (2047, 4096, 8190, (256, 0, 1, 0))])
+def test_divisions_of_gate_and_up(w8, rows, width, inter, kind):
+    assert division(rows, width, inter, gated=True)[0] == kind
+    x, gate, up, down = make_ffn(rows, width, inter, rows + inter)
+    got = w8.gated_ffn(x, w8.PackedGateUp(*gate, *up), w8.PackedLinear(*down))
+    want, tol, _ = ref.ffn(x, *gate, *up, *down)
+    near(got, want, tol)
+
+
+def test_cut_tiles_on_several_streams_and_in_graphs(w8):
+    """Pieces of tiles, on single CTAs and on pairs, beside one another and beside other products, and replayed with other inputs."""
+    sizes = [(810, 12000, 4993), (140, 12000, 6624), (1320, 6000, 3362), (260, 33000, 3828), (60, 16384, 4096), (1, 8192, 8192)]
+    assert [division(*s)[0][2:] for s in sizes[:4]] == [(1, 1), (0, 1), (0, 1), (1, 1)]
+    work = []
+    for i, (rows, width, out) in enumerate(sizes):
+        x, q, s = ref.make(rows, width, out, seed=i, device="cuda")
+        work.append((x, w8.PackedLinear(q, s)))
+    want = [w8.linear(x, p) for x, p in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    got = [[] for _ in work]
+    for _ in range(10):
+        for i, (stream, (x, p)) in enumerate(zip(streams, work)):
+            with torch.cuda.stream(stream):
+                got[i].append(w8.linear(x, p))
+    torch.cuda.synchronize()
+    for stream in streams:
+        C.stream_check(stream.cuda_stream)
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = [w8.linear(x, p) for x, p in work]
+    for shift in (1, 2):
+        for x, _ in work:
+            x.copy_(x.roll(shift, 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w8.linear(x, p)) for a, (x, p) in zip(kept, work))
+        assert not any(torch.equal(a, w) for a, w in zip(kept, want))
+    C.stream_check()
