@@ -1,8 +1,9 @@
 """Build libcpmcu_b200.so in-tree with nvcc for sm_100a, and the Python module _ops.so over it with g++ against torch's headers.
 
 Usage: python cpm.cu_b200/build.py [--force]
-Both land next to the Python package (cpm.cu_b200/cpmcu/) so that it
-travels with the source tree; nothing is installed into site-packages.
+Both land next to the Python package (cpm.cu_b200/cpmcu/) so that they
+travel with the source tree; nothing is installed into site-packages.  The library is built first and
+stands alone: what goes wrong with the module, or a machine without torch, does not touch it.
 """
 import concurrent.futures
 import hashlib
@@ -31,16 +32,52 @@ def _nvcc():
     return "nvcc"
 
 
-def _stamp():
+def _hash(files, *words):
     h = hashlib.sha256()
-    for root in (CSRC, os.path.join(os.path.dirname(HERE), "include")):
-        for name in sorted(os.listdir(root)):
-            if name.endswith((".cu", ".cuh", ".h", ".cpp")):
-                with open(os.path.join(root, name), "rb") as f:
-                    h.update(name.encode())
-                    h.update(f.read())
-    h.update(" ".join(NVCC_FLAGS).encode())
+    for path in files:
+        with open(path, "rb") as f:
+            h.update(os.path.basename(path).encode())
+            h.update(f.read())
+    h.update(" ".join(words).encode())
     return h.hexdigest()
+
+
+def _sources(*endings):
+    return [os.path.join(root, name) for root in (CSRC, os.path.join(os.path.dirname(HERE), "include")) for name in sorted(os.listdir(root)) if name.endswith(endings)]
+
+
+def _stamp():
+    return _hash(_sources(".cu", ".cuh", ".h"), *NVCC_FLAGS)
+
+
+def _ops_stamp(command):
+    """Of the module: its source, the header of the library, and the torch and Python that it is compiled for."""
+    import torch
+    return _hash(_sources(".cpp", ".h"), torch.__version__, sys.version, *command)
+
+
+def _fresh(output, stamp_file, stamp):
+    if not (os.path.exists(output) and os.path.exists(stamp_file)):
+        return False
+    with open(stamp_file) as f:
+        return f.read() == stamp
+
+
+def _run(cmd, what):
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("%s:\n%s\n%s" % (what, res.stdout, res.stderr))
+
+
+def _write(path, text):
+    with open(path, "w") as f:
+        f.write(text)
+
+
+def _forget(stamp_file):
+    """Before a build: one that ends half-way leaves nothing that counts as built."""
+    if os.path.exists(stamp_file):
+        os.remove(stamp_file)
 
 
 def _ops_command(cuda_home):
@@ -57,36 +94,53 @@ def _ops_command(cuda_home):
                   "-ltorch_python"]
 
 
-def build(force=False, verbose=True):
+def build_library(force=False, verbose=True):
+    """libcpmcu_b200.so: nvcc alone."""
     os.makedirs(OBJ_DIR, exist_ok=True)
-    stamp_file = os.path.join(OBJ_DIR, "stamp")
-    stamp = _stamp()
-    if not force and os.path.exists(LIB) and os.path.exists(OPS) and os.path.exists(stamp_file) and open(stamp_file).read() == stamp:
+    stamp_file, stamp = os.path.join(OBJ_DIR, "stamp"), _stamp()
+    if not force and _fresh(LIB, stamp_file, stamp):
         return LIB
+    _forget(stamp_file)
     nvcc = _nvcc()
 
     def compile_one(src):
         obj = os.path.join(OBJ_DIR, src.replace(".cu", ".o"))
-        cmd = [nvcc] + NVCC_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError("nvcc failed for %s:\n%s\n%s" % (src, res.stdout, res.stderr))
+        _run([nvcc] + NVCC_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj], "nvcc failed for %s" % src)
         return obj
 
     with concurrent.futures.ThreadPoolExecutor(max_workers=4) as ex:
         objs = list(ex.map(compile_one, SOURCES))
-    cmd = [nvcc, "-shared", "-o", LIB] + objs + ["-gencode", "arch=compute_100a,code=sm_100a", "-lcudart"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
-    home = os.path.dirname(os.path.dirname(nvcc)) if os.path.isabs(nvcc) else "/usr/local/cuda"
-    res = subprocess.run(_ops_command(home), capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("g++ failed for torch_ops.cpp:\n%s\n%s" % (res.stdout, res.stderr))
-    with open(stamp_file, "w") as f:
-        f.write(stamp)
+    _run([nvcc, "-shared", "-o", LIB] + objs + ["-gencode", "arch=compute_100a,code=sm_100a", "-lcudart"], "link failed")
+    _write(stamp_file, stamp)
     if verbose:
         print("built", LIB)
+    return LIB
+
+
+def build_module(force=False, verbose=True):
+    """_ops.so over the library, with g++ against torch's headers; None where there is no torch: the library and its C entry points stand without it."""
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        print("no torch: %s is not built, and cpmcu.w8a8 and cpmcu.rotary cannot be imported" % os.path.basename(OPS))
+        return None
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    nvcc = _nvcc()
+    command = _ops_command(os.path.dirname(os.path.dirname(nvcc)) if os.path.isabs(nvcc) else "/usr/local/cuda")
+    stamp_file, stamp = os.path.join(OBJ_DIR, "stamp_ops"), _ops_stamp(command)
+    if not force and _fresh(OPS, stamp_file, stamp):
+        return OPS
+    _forget(stamp_file)
+    _run(command, "g++ failed for torch_ops.cpp")
+    _write(stamp_file, stamp)
+    if verbose:
+        print("built", OPS)
+    return OPS
+
+
+def build(force=False, verbose=True):
+    build_library(force, verbose)
+    build_module(force, verbose)
     return LIB
 
 
