@@ -75,7 +75,7 @@ struct Runtime {
     cudaStream_t stream = nullptr;
     int* d_error = nullptr;  // device error word, or-ed into by kernels
     int* h_error = nullptr;  // pinned copy of it
-    unsigned long long* d_op_errors = nullptr;  // counters of the operators on the caller's streams (op_errors.cuh)
+    unsigned* d_op_errors = nullptr;  // counters of the operators on the caller's streams (op_errors.cuh)
     unsigned* d_accept_ticket = nullptr;  // CTAs of the acceptance kernel that have read the tree (zero between launches)
     int num_sms = 148;
     int device = 0;

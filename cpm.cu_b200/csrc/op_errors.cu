@@ -1,7 +1,6 @@
 // Host side of op_errors.cuh.
 #include "op_errors.cuh"
 
-#include <algorithm>
 #include <mutex>
 #include <type_traits>
 #include <unordered_map>
@@ -12,6 +11,7 @@ constexpr int SETS = 1024;   // set 0 is shared; streams beyond the last one use
 
 struct Known {
     int set = 0;
+    std::mutex checking;   // of two checks of a stream at once the later one has the later counts
     OpCount own[OP_ERROR_KINDS] = {}, shared[OP_ERROR_KINDS] = {};   // told so far
 };
 struct Registry {
@@ -61,13 +61,13 @@ bool id_outside_captures(cudaStream_t s, unsigned long long& id) {
     return false;
 }
 
-// KernelError bits of the counters that grew
-int grown(const OpCount* now, OpCount* told) {
+// KernelError bits of the counters that moved
+int moved(const OpCount* now, OpCount* told) {
     constexpr int bit[OP_ERROR_KINDS] = {ERR_GEMM_TIMEOUT, ERR_KV_OVERFLOW};
     int bits = 0;
     for (int k = 0; k < OP_ERROR_KINDS; ++k) {
-        if (now[k] > told[k]) bits |= bit[k];
-        told[k] = std::max(told[k], now[k]);   // of two checks at once the later read may come here first
+        if (now[k] != told[k]) bits |= bit[k];
+        told[k] = now[k];
     }
     return bits;
 }
@@ -93,20 +93,19 @@ OpErrors new_op_errors(cudaStream_t s) {
     unsigned long long id;
     CUDA_CHECK(cudaStreamGetId(s, &id));
     Registry& r = registry();
-    int set;
+    Known* k;   // stays where it is
     {
         std::lock_guard<std::mutex> hold(r.lock);
-        set = known(r, id).set;
+        k = &known(r, id);
     }
+    std::lock_guard<std::mutex> hold(k->checking);
     OpCount own[OP_ERROR_KINDS], shared[OP_ERROR_KINDS];
     CUDA_CHECK(cudaStreamSynchronize(s));
-    CUDA_CHECK(cudaMemcpyAsync(own, counters(set), sizeof(own), cudaMemcpyDeviceToHost, s));
+    CUDA_CHECK(cudaMemcpyAsync(own, counters(k->set), sizeof(own), cudaMemcpyDeviceToHost, s));
     CUDA_CHECK(cudaMemcpyAsync(shared, counters(0), sizeof(shared), cudaMemcpyDeviceToHost, s));
     CUDA_CHECK(cudaStreamSynchronize(s));
-    std::lock_guard<std::mutex> hold(r.lock);
-    Known& k = known(r, id);
     OpErrors e;
-    e.shared = grown(shared, k.shared);
-    if (set != 0) e.own = grown(own, k.own);
+    e.shared = moved(shared, k->shared);
+    if (k->set != 0) e.own = moved(own, k->own);
     return e;
 }
