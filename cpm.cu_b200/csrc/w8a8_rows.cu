@@ -8,11 +8,14 @@
 // Bound: bytes.  One CTA per row, which stays in registers between the pass that finds the maximum and the one that rounds; rows too
 // long for that are read twice.  A row with an infinity or a NaN gets the scale NaN and integers 0, a row of zeros the scale 0.
 // 4096 rows of 16384: 36.8 us (5.5 TB/s), of 4096: 9.1 (5.5); 60 rows of 16384: 2.8, of 4096: 1.6.
+#include <algorithm>
+
 #include "w8a8_rows.cuh"
 
 namespace w8 {
 namespace {
 
+constexpr int CLEARING = 1 << 16;   // CTAs that clear counters
 struct QuantizeArgs {
     RowSource src;
     int K, pad_to;
@@ -21,7 +24,7 @@ struct QuantizeArgs {
     bool q_wide;     // rows of q are 8-byte aligned and have room for whole vectors
     float* scale;
     int* clear;
-    int n_clear;
+    int n_clear, clear_step;   // step: the threads that clear
 };
 
 // VPT > 0: a thread's VPT pieces of eight elements stay in registers; 0: the row is read twice.
@@ -36,8 +39,10 @@ __global__ void __launch_bounds__(MOST_THREADS<VPT>) quantize_kernel(const Quant
     if (static_cast<int>(threadIdx.x) * 8 < a.K && threadIdx.x % 8 == 0) Values<SRC, WIDE>::ask(a.src, row, a.K, threadIdx.x * 8);
     grid_dep_wait();
     grid_dep_trigger();
-    // 64 bits: there may be more than 2^31 threads
-    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < a.n_clear; i += static_cast<long long>(gridDim.x) * blockDim.x) a.clear[i] = 0;
+    if (blockIdx.x < static_cast<unsigned>(CLEARING)) {   // not by all: numbers of 2^31 threads do not fit 32 bits
+#pragma unroll 1
+        for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < a.n_clear; i += a.clear_step) a.clear[i] = 0;
+    }
     Values<SRC, WIDE> kept[VPT > 0 ? VPT : 1];
     float ss = 0.f;
     uint32_t top = 0u;
@@ -102,7 +107,12 @@ __global__ void __launch_bounds__(MOST_THREADS<VPT>) quantize_kernel(const Quant
 template <Source SRC, bool WIDE>
 void run_quantize(const QuantizeArgs& a, int rows, cudaStream_t s) {
     // the kernel, and how many of a row's vectors a thread has
-    auto go = [&](void (*kernel)(QuantizeArgs), int vectors, int each) { launch_on(kernel, rows, (ceil_div(vectors, each) + 31) / 32 * 32, 0, s, 1, true, a); };
+    auto go = [&](void (*kernel)(QuantizeArgs), int vectors, int each) {
+        const int threads = (ceil_div(vectors, each) + 31) / 32 * 32;
+        QuantizeArgs with = a;
+        with.clear_step = std::min(rows, CLEARING) * threads;
+        launch_on(kernel, rows, threads, 0, s, 1, true, with);
+    };
     const int vectors = ceil_div(a.K, 8);
     if (rows <= 2 * runtime().num_sms) {
         // few rows: a row's own time counts, and the fewer vectors a thread has the shorter it is (60 x 16384: 4.2 us with eight on 256 threads, 2.9
