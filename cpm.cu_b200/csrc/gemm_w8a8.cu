@@ -79,6 +79,15 @@ __device__ __forceinline__ void umma_block(uint32_t d, uint32_t wa, uint32_t xa,
     }
 }
 
+// The end of a CTA, thread 0: a wait that ran out is reported, and copies still in flight, which arrive at this CTA's barriers, land before it retires.  (A partner's
+// copies too: where a CTA's own waits all ended, the bytes of both have come.)
+__device__ __forceinline__ void finish(volatile int* abort_flag, OpCount* errors) {
+    if (*abort_flag == 0) return;
+    report(errors, OP_TIMEOUT);
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) {}
+}
+
 template <int MT>
 constexpr int PARTS_OF = MT / BATCH < MAX_PARTS ? MT / BATCH : MAX_PARTS;   // epilogue warps on a quarter
 template <int MT, bool PAIR>
@@ -422,10 +431,6 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
                 }
             }
-            if (!ok) {   // copies already in flight land before the CTA retires
-                const long long t0 = clock64();
-                while (clock64() - t0 < 2000000LL) {}
-            }
         } else {
             grid_dep_wait();
         }
@@ -481,7 +486,7 @@ product_s8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constan
         if constexpr (PAIR) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
         else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
-    if (threadIdx.x == 0 && *abort_flag) report(a.errors, OP_TIMEOUT);
+    if (threadIdx.x == 0) finish(abort_flag, a.errors);
 }
 
 // A tile per cluster: CTA `rank` of CS has k-blocks [rank * kblocks / CS, (rank + 1) * kblocks / CS).  Each CTA sends each peer that peer's share of the tokens
@@ -555,20 +560,15 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
             grid_dep_wait();
             int stage = 0;
             uint32_t phase = 0;
-            bool ok = true;
             for (int i = 0; i < kpc; ++i) {
                 uint8_t* dst = smem + stage * C::STAGE_BYTES;
                 if (i >= pre) {
-                    if (!ptx::mbar_wait(&empty[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+                    if (!ptx::mbar_wait(&empty[stage], phase ^ 1, abort_flag)) break;
                     ptx::mbar_arrive_expect_tx(&full[stage], C::STAGE_BYTES);
                     ptx::tma_load_2d(dst, &tm_w, &full[stage], 0, (tile * kblocks + kb_begin + i) * TILE_ROWS);
                 }
                 ptx::tma_load_2d(dst + BLOCK_BYTES, &tm_x, &full[stage], (kb_begin + i) * BLOCK_COLS, m_base);
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1; }
-            }
-            if (!ok) {   // copies already in flight land before the CTA retires
-                const long long t0 = clock64();
-                while (clock64() - t0 < 2000000LL) {}
             }
         } else {
             grid_dep_wait();
@@ -658,7 +658,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem_base, Cfg<MT, false>::TMEM_COLS);
     }
-    if (threadIdx.x == 0 && *abort_flag) report(a.errors, OP_TIMEOUT);
+    if (threadIdx.x == 0) finish(abort_flag, a.errors);
 }
 
 // ---------------------------------------------------------------- host
