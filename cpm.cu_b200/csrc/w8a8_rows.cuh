@@ -103,10 +103,11 @@ struct RowRound {
         }
         return low_bytes(y[0], y[1], y[2], y[3]);
     }
-    // the row's scale: NaN for a row with an infinity or a NaN, so that its outputs are NaN; 0 for a row of zeros, whatever its norm
+    // the row's scale: NaN for a row with an infinity or a NaN, so that its outputs are NaN, and for one whose squares do not fit fp32 (a factor of 0 would
+    // give zeros); 0 for a row of zeros, whatever its norm
     __device__ __forceinline__ static float scale(uint32_t bits, float factor) {
         if (bits == 0u) return 0.f;
-        return bits < 0x7f800000u ? __uint_as_float(bits) / 127.f * factor : __uint_as_float(0x7fffffffu);
+        return bits < 0x7f800000u && factor != 0.f ? __uint_as_float(bits) / 127.f * factor : __uint_as_float(0x7fffffffu);
     }
 };
 

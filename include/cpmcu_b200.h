@@ -483,7 +483,8 @@ int cpmcu_stream_check(void* stream);
  *   t = x, or with delta [rows, K] (bf16, may be NULL) t = bf16(x + delta_scale * delta), which goes to total [rows, K], apart from x
  *   q = round(127 v / max|v|) (to even at ties),  s = max|v| / 127 * f            one scale for each row
  *   y[m][n] = (sum over k of q[m][k] W[n][k]) * s[m] * S[n] + bias[n]             exact sums, rounded once, to bf16
- * A row with an infinity or a NaN gives NaN, a row of zeros the bias.  K <= 131072 (sums of 32 bits).  What a call writes (y, total, the
+ * A row with an infinity or a NaN gives NaN, and so does one whose products t * norm, or squares behind a norm, do not fit fp32 (magnitudes from 10^19 on); a row of
+ * zeros gives the bias.  K <= 131072 (sums of 32 bits).  What a call writes (y, total, the
  * workspace) shares no element with anything else that it takes.
  *
  * Packed weights are written once, by cpmcu_w8a8_pack, and the first of them are fetched before a launch waits for its predecessor in the

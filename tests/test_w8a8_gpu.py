@@ -718,3 +718,23 @@ def test_cut_tiles_on_several_streams_and_in_graphs(w8):
         assert all(torch.equal(a, w8.linear(x, p)) for a, (x, p) in zip(kept, work))
         assert not any(torch.equal(a, w) for a, w in zip(kept, want))
     C.stream_check()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_rows_whose_squares_do_not_fit(w8, rows):
+    """Behind a norm: NaN, not zeros; the largest rows that fit are right."""
+    x, q, s = ref.make(rows, 512, 300, seed=rows, device="cuda")
+    packed, weight = w8.PackedLinear(q, s), torch.linspace(0.5, 2, 512, device="cuda").to(BF16)
+    clean = w8.linear(x, packed, norm_weight=weight)
+    at = rows // 2
+    rest = torch.arange(rows, device="cuda") != at
+    big = x.clone()
+    big[at] = x[at] * 2.0 ** 55                       # squares up to some 2^121 each
+    want, tol, _ = ref.linear(big, q, s, norm_weight=weight)
+    near(w8.linear(big, packed, norm_weight=weight), want, tol)
+    big[at] = x[at] * 2.0 ** 70
+    y = w8.linear(big, packed, norm_weight=weight)
+    assert bool(torch.isnan(y[at]).all()) and torch.equal(y[rest], clean[rest])
+    z = torch.zeros_like(big)
+    y, total = w8.linear(z, packed, norm_weight=weight, delta=big)
+    assert torch.equal(total[at], big[at]) and bool(torch.isnan(y[at]).all()) and torch.equal(y[rest], clean[rest])
