@@ -16,7 +16,7 @@ def frequencies(rot_dims, base, scaling=None, length=None, max_position=None):
     """(inv_freq, factor): the rot_dims / 2 frequencies (fp32, CPU, computed in 64 bits) and the factor of sines and cosines.
 
     scaling: a checkpoint's rope_scaling dictionary ("rope_type" or "type", and the entries of that type); None or "default" is
-    base^(-2 i / rot_dims).  linear: positions divided by "factor".  dynamic: a base that grows with `length` beyond the trained length.  llama3: long waves
+    base^(-2 i / rot_dims).  linear: positions divided by "factor".  dynamic: a base that grows with `length` beyond max_position.  llama3: long waves
     divided by "factor", short ones kept, a ramp between.  yarn: a ramp over the pairs between the numbers of turns "beta_fast" and "beta_slow".
     longrope: "long_factor" if `length` is beyond the trained length, else "short_factor", for each pair.
     length: of the sequence that is served; max_position: of the checkpoint (max_position_embeddings), the trained length where the
@@ -45,7 +45,7 @@ def frequencies(rot_dims, base, scaling=None, length=None, max_position=None):
     elif kind == "linear":
         inv = inv / entry("factor")
     elif kind == "dynamic":
-        f, top = entry("factor"), trained()
+        f, top = entry("factor"), trained() if max_position is None else max_position
         n = max(length or top, top)
         if rot_dims > 2:
             inv = (base * ((f * n / top) - (f - 1)) ** (rot_dims / (rot_dims - 2))) ** -i

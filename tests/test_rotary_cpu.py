@@ -47,3 +47,15 @@ def test_refusals():
                  (64, 10000.0, {"rope_type": "longrope", "short_factor": [1.0], "long_factor": [1.0], "original_max_position_embeddings": 10})):
         with pytest.raises(ValueError):
             frequencies(*args)
+
+
+def test_dynamic_grows_beyond_the_checkpoint_s_positions():
+    """As the initialiser that the engine's own models use has it: also where the dictionary names a trained length."""
+    from cpmcu.rotary import frequencies
+    for trained, top, length in ((4096, 16384, 10000), (4096, 16384, 50000), (8192, 4096, 6000)):
+        scaling = {"rope_type": "dynamic", "factor": 4.0, "original_max_position_embeddings": trained}
+        inv, _ = frequencies(64, 10000.0, scaling, length=length, max_position=top)
+        want, _ = transformers_frequencies(64, 10000.0, scaling, length, top)
+        assert float(((inv.double() - want.double()) / want.double()).abs().max()) < 1e-5
+    alone, _ = frequencies(64, 10000.0, scaling, length=10000)                       # nothing else is known
+    assert torch.equal(alone, frequencies(64, 10000.0, {"rope_type": "dynamic", "factor": 4.0}, length=10000, max_position=8192)[0])
