@@ -87,7 +87,7 @@ def frequencies(rot_dims, base, scaling=None, length=None, max_position=None):
         if s.get("attention_factor") is not None:
             factor = float(s["attention_factor"])
         else:
-            f = s.get("factor") or (max_position / top if max_position else 1.0)
+            f = entry("factor", max_position and max_position / top)
             factor = 1.0 if f <= 1 else math.sqrt(1 + math.log(f) / math.log(top))
     else:
         raise ValueError(f"rope type {kind!r} is not one of default, linear, dynamic, llama3, yarn, longrope")

@@ -59,3 +59,13 @@ def test_dynamic_grows_beyond_the_checkpoint_s_positions():
         assert float(((inv.double() - want.double()) / want.double()).abs().max()) < 1e-5
     alone, _ = frequencies(64, 10000.0, scaling, length=10000)                       # nothing else is known
     assert torch.equal(alone, frequencies(64, 10000.0, {"rope_type": "dynamic", "factor": 4.0}, length=10000, max_position=8192)[0])
+
+
+def test_longrope_without_its_factor():
+    """It is that of the dictionary, or of the checkpoint's positions to the trained ones; with neither there is no right answer."""
+    from cpmcu.rotary import frequencies
+    scaling = {"rope_type": "longrope", "short_factor": [1.0] * 4, "long_factor": [2.0] * 4, "original_max_position_embeddings": 4096}
+    with pytest.raises(ValueError, match="'factor'"):
+        frequencies(8, 10000.0, scaling)
+    assert frequencies(8, 10000.0, scaling, max_position=32768)[1] == frequencies(8, 10000.0, {**scaling, "factor": 8.0})[1] > 1
+    assert frequencies(8, 10000.0, {**scaling, "attention_factor": 1.25})[1] == 1.25
