@@ -813,8 +813,6 @@ Division divide(int M, int tiles, int kblocks, bool gated) {
     return f.d;
 }
 
-int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TILE_ROWS); }
-
 }  // namespace
 
 Scratch product_scratch(int M, int N, int K) {

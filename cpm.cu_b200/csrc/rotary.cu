@@ -39,14 +39,7 @@ struct Elems {
     }
 };
 
-// Two pairs (a.lo, b.lo), (a.hi, b.hi) of packed values.  Unpacked by shifts and packed by the pair: conversions of single values go through the unit of
-// the special functions, a quarter of the rate.
-__device__ __forceinline__ float low(uint32_t two) { return __uint_as_float(two << 16); }
-__device__ __forceinline__ float high(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
-__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&p);
-}
+// Two pairs (a.lo, b.lo), (a.hi, b.hi) of packed values.
 __device__ __forceinline__ void turn_two(uint32_t& a, uint32_t& b, const float* cs, const float* sn) {
     const uint32_t x = a, y = b;
     a = two_bf16(fmaf(low(x), cs[0], -(low(y) * sn[0])), fmaf(high(x), cs[1], -(high(y) * sn[1])));

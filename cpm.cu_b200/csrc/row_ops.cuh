@@ -78,6 +78,15 @@ __device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.f +
 template <typename T>
 __device__ __forceinline__ float silu_of(float v) { return sizeof(T) == 2 ? silu_fast(v) : silu_f32(v); }
 
+// bf16 to fp32 and back by the pair: conversions of single values go through the unit of the special functions, a quarter of the rate, and bound a
+// pass over rows.
+__device__ __forceinline__ float low(uint32_t two) { return __uint_as_float(two << 16); }
+__device__ __forceinline__ float high(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
+__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+
 // ---- pairs of fp32 for the packed instructions
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float lo, float hi) {

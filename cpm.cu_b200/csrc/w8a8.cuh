@@ -29,6 +29,7 @@ struct Packed {
 enum Role : int { ROLE_PLAIN = 0, ROLE_GATE = 1, ROLE_UP = 2 };
 size_t packed_bytes(int N, int K, bool gated);
 Packed packed_view(const void* p, int N, int K, bool gated);
+inline int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TILE_ROWS); }
 void launch_pack(const int8_t* q, const float* scale, int N, int K, Role role, void* packed, cudaStream_t s);
 
 // What the integers of a row are made of.
@@ -67,14 +68,5 @@ void product_division(int M, int N, int K, bool gated, int32_t (&out)[6]);
 void launch_product(const Product& p, cudaStream_t s);
 // one row, straight from its source
 void launch_one_row(const RowSource& src, int N, int K, const Packed& w, const bf16* bias, bf16* y, float* act, cudaStream_t s);
-
-// bf16 to fp32 and back by the pair: conversions of single values go through the unit of the special functions, a quarter of the rate, and bound a
-// pass over rows.
-__device__ __forceinline__ float low(uint32_t two) { return __uint_as_float(two << 16); }
-__device__ __forceinline__ float high(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
-__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
-    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&p);
-}
 
 }  // namespace w8

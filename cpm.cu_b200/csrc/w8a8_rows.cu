@@ -175,8 +175,6 @@ __global__ void pack_kernel(const int8_t* __restrict__ q, const float* __restric
     __threadfence();   // in L2 before this CTA ends, which may be when the next launch fetches its first weights
 }
 
-int tiles_of(int N, bool gated) { return ceil_div(N, gated ? TILE_ROWS / 2 : TILE_ROWS); }
-
 }  // namespace
 
 size_t packed_bytes(int N, int K, bool gated) {
