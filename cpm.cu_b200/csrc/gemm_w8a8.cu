@@ -150,9 +150,7 @@ __device__ __forceinline__ void store16(bf16* y, long long ldy, int N, long long
 }
 
 // silu(gate) * up of a whole tile: lanes 0-63 hold the gate sums of 64 features, 64-127 the up sums of the same ones.  Warps q and q + 2 hand
-// each other the sums of half of the tokens of a batch, so that both compute.  fp32: what is rounded next is the row of 8-bit integers, and values next
-// to a border go where the formula has them.  So silu is the one of 32 bits: with an approximate exponential and quotient activations are off by up to
-// 1.7e-6 (|gate| up to 30), with these by 3e-7.  It costs 1 us of 45 at 60 x 4096, 16384 inside, and 12 of 715 at 4096 rows.
+// each other the sums of half of the tokens of a batch, so that both compute.  fp32: what is rounded next is the row of 8-bit integers.
 // xs: the scales of this warp's batches, one after another.
 template <int MT>
 __device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act, long long ld, int N, long long row0, int n0, const float* xs, float ws_gate,
@@ -174,7 +172,7 @@ __device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act
         for (int c = 0; c < HB; ++c) out[c * 32] = static_cast<int>(gates ? r[HB + c] : r[c]);
         ptx::named_bar_sync(pair_bar, 64);
         const int first = c0 + (gates ? 0 : HB);
-        float v[HB];
+        float v[HB], gate[HB], up[HB], least = 0.f;
 #pragma unroll
         for (int c = 0; c < HB; c += 4) {
             const float4 s4 = *reinterpret_cast<const float4*>(xs + c);
@@ -182,9 +180,15 @@ __device__ __forceinline__ void gate_tile(uint32_t t_addr, int m_cnt, float* act
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int mine = static_cast<int>(gates ? r[c + e] : r[HB + c + e]), other = in[(c + e) * 32];
-                const float g = static_cast<float>(gates ? mine : other) * s[e] * ws_gate, u = static_cast<float>(gates ? other : mine) * s[e] * ws_up;
-                v[c + e] = silu_f32(g) * u;
+                gate[c + e] = static_cast<float>(gates ? mine : other) * s[e] * ws_gate;
+                up[c + e] = static_cast<float>(gates ? other : mine) * s[e] * ws_up;
+                v[c + e] = silu_above(gate[c + e]) * up[c + e];
+                least = fminf(least, gate[c + e]);
             }
+        }
+        if (least <= SILU_LEAST) {
+#pragma unroll
+            for (int c = 0; c < HB; ++c) v[c] = silu(gate[c]) * up[c];
         }
         float* dst = act + (row0 + first) * ld + n0 + lane;
         if (column) {
@@ -648,7 +652,7 @@ product_s8_cluster_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
             ptx::named_bar_sync(1, 128);
             const int f = row & 63, n = tile * 64 + f;
             for (int t = row >> 6; t < cnt; t += 2) {
-                if (n < a.N) a.act[static_cast<long long>(m_base + t0 + t) * a.ldy + n] = silu_f32(meet[t * TILE_ROWS + f]) * meet[t * TILE_ROWS + 64 + f];
+                if (n < a.N) a.act[static_cast<long long>(m_base + t0 + t) * a.ldy + n] = silu(meet[t * TILE_ROWS + f]) * meet[t * TILE_ROWS + 64 + f];
             }
         }
     }

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) one_row_s8_kernel(const
         }
         if (writes) {
             const float v = static_cast<float>(acc[0]) * scale;
-            if constexpr (GATED) a.act[n] = silu_f32(v * ws) * (static_cast<float>(acc[SETS - 1]) * scale * ws_up);
+            if constexpr (GATED) a.act[n] = silu(v * ws) * (static_cast<float>(acc[SETS - 1]) * scale * ws_up);
             else a.y[n] = __float2bfloat16(fmaf(v, ws, bias));
         }
     }

@@ -738,3 +738,31 @@ def test_rows_whose_squares_do_not_fit(w8, rows):
     z = torch.zeros_like(big)
     y, total = w8.linear(z, packed, norm_weight=weight, delta=big)
     assert torch.equal(total[at], big[at]) and bool(torch.isnan(y[at]).all()) and torch.equal(y[rest], clean[rest])
+
+
+@pytest.mark.parametrize("rows", [1, 60, 1000])
+def test_activations_of_large_gates(rows):
+    """The same for gates from -126 to 126: small activations keep their digits as far as fp32 has them.  Below, the product with up magnifies two roundings to
+    a multiple of 2^-149, of the exponential and of the quotient."""
+    width, inter = 512, 320
+    g = torch.Generator("cuda").manual_seed(rows)
+    x = torch.randint(-127, 128, (rows, width), generator=g, device="cuda")
+    x[:, 7] = 127
+    weights = [torch.zeros(inter, width, dtype=torch.int8, device="cuda") for _ in range(2)]
+    at = torch.randint(0, width, (inter,), generator=g, device="cuda")
+    for w in weights:
+        w[torch.arange(inter, device="cuda"), at] = torch.randint(1, 128, (inter,), generator=g, device="cuda").to(torch.int8)
+    scales = [torch.full((inter,), 2.0 ** -7, device="cuda"), torch.full((inter,), 1.0, device="cuda")]
+    import cpmcu.w8a8 as w8
+    gate_up = w8.PackedGateUp(weights[0], scales[0], weights[1], scales[1])
+    down = w8.PackedLinear(torch.ones(width, inter, dtype=torch.int8, device="cuda"), torch.ones(width, device="cuda"))
+    size = C.load().cpmcu_w8a8_workspace_bytes(rows, width, width, inter)
+    workspace = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    xb, y = x.to(BF16), torch.empty(rows, width, dtype=BF16, device="cuda")
+    C.call("cpmcu_w8a8_ffn", xb.data_ptr(), width, gate_up.data.data_ptr(), down.data.data_ptr(), None, 1e-5, None, 1.0, None, y.data_ptr(), width, rows, width, inter,
+           workspace.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    got = workspace[:rows * inter * 4].view(torch.float32).view(rows, inter).double()
+    a, b = (x.double() @ w.double().t() * s.double() for w, s in zip(weights, scales))
+    want = a / (1 + torch.exp(-a)) * b
+    tol = want.abs() * 6 * 2.0 ** -24 + (a.abs() + 2) * b.abs() * 2.0 ** -149
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
