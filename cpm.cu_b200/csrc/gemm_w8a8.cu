@@ -8,8 +8,8 @@
 //               product); whole tiles in waves, and only those of the last wave are cut (stream-K), where that pays
 // whichever find_division() expects to end first.
 // Bound: the weights' bytes from HBM up to some 300 rows, the tensor pipe (and, with warm passes, the power cap) beyond.  60 x 16384 x 4096 14.2 us
-// (7.8 TB/s between the first block and the last), 4096 x 16384 x 4096 174 us (3.16 Pop/s), gate/up 4096 x 4096 x 2 * 16384 325 us (3.39, tensor pipe
-// 91 % active).
+// (5.8 TB/s between the first block and the last: 50 MB, 17 are asked for before), 4096 x 16384 x 4096 174 us (3.16 Pop/s), gate/up 4096 x 4096 x 2 * 16384
+// 325 us (3.39, tensor pipe 91 % active).
 //
 // Cut tiles: each piece leaves its int32 sums in a workspace slot, and the one counted last adds them up.  Integer sums have no order, so the
 // result does not depend on who is last, and no CTA waits for another one: the launch need not be resident as a whole, and may share the

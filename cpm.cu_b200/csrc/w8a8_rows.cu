@@ -7,7 +7,9 @@
 //
 // Bound: bytes.  One CTA per row, which stays in registers between the pass that finds the maximum and the one that rounds; rows too
 // long for that are read twice.  A row with an infinity or a NaN gets the scale NaN and integers 0, a row of zeros the scale 0.
-// 4096 rows of 16384: 36.8 us (5.5 TB/s), of 4096: 9.1 (5.5); 60 rows of 16384: 2.8, of 4096: 1.6.
+// 4096 rows of 16384: 35.4 us (5.7 TB/s), of 4096: 9.1 (5.5); 60 rows of 16384: 2.7, of 4096: 1.5.  Alone and cold (every launch by itself, from HBM): 4096 rows of 4096
+// 11.0, behind a norm 18.6, behind a residual sum and a norm 21.7; of 8192 17.6, 29.6, 37.0; 2000 rows of 5121 11.7 (with rows of q in whole vectors), 20.1, 40.9.
+// Behind a norm it is not the bytes: each row reads the norm's weights again, from L2, and meets twice.  Element by element it is the number of accesses, of 2 bytes.
 #include <algorithm>
 
 #include "w8a8_rows.cuh"
@@ -123,8 +125,9 @@ void run_quantize(const QuantizeArgs& a, int rows, cudaStream_t s) {
         return;
     }
     // Many rows: several CTAs beside one another on an SM; where they come in more than eight rounds, fewer threads with more vectors each (4096 rows of 4096: four
-    // vectors 9.1 us, two 10.0, behind a norm 23.1, 25.2; of 2048: two 5.5, one 6.2; but 400 of 4096: four 2.6, two 2.2; 2000 of 1536 behind a norm: two
-    // 11.6, one 10.8).  Element by element the fewest (2000 rows of 5121 behind a residual sum and a norm: two 44.8, four 52.2).
+    // vectors 9.1 us, two 10.0; of 2048: two 5.5, one 6.2; but 400 of 4096: four 2.6, two 2.2).  With a product of 64 columns behind them: 4096 rows of 4096 behind
+    // a norm four 23.1, two 25.2; 2000 of 1536 two 11.6, one 10.8; and element by element the fewest (2000 rows of 5121 behind a residual sum and a norm:
+    // two 44.8, four 52.2).
     const bool rounds = rows > 8 * runtime().num_sms;
     if (vectors > 2048) {
         go(quantize_kernel<SRC, 0, WIDE>, 256, 1);
