@@ -61,6 +61,14 @@ bool id_outside_captures(cudaStream_t s, unsigned long long& id) {
     return false;
 }
 
+// While a stream is captured in CUDA's default mode, no thread may wait or copy, on any stream: it would end that capture.  What a check waits for and copies is
+// no part of a capture, which the relaxed mode says.
+struct BesideCaptures {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    BesideCaptures() { CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode)); }
+    ~BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // KernelError bits of the counters that moved
 int moved(const OpCount* now, OpCount* told) {
     constexpr int bit[OP_ERROR_KINDS] = {ERR_GEMM_TIMEOUT, ERR_KV_OVERFLOW};
@@ -99,6 +107,7 @@ OpErrors new_op_errors(cudaStream_t s) {
         k = &known(r, id);
     }
     std::lock_guard<std::mutex> hold(k->checking);
+    const BesideCaptures beside;
     OpCount own[OP_ERROR_KINDS], shared[OP_ERROR_KINDS];
     CUDA_CHECK(cudaStreamSynchronize(s));
     CUDA_CHECK(cudaMemcpyAsync(own, counters(k->set), sizeof(own), cudaMemcpyDeviceToHost, s));

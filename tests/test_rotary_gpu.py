@@ -313,3 +313,44 @@ def test_errors_of_captured_graphs():
     root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "cpm.cu_b200")
     out = subprocess.run([sys.executable, "-c", GRAPH], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and "told" in out.stdout, out.stderr[-2000:]
+
+
+DURING = """
+import threading, torch, cpmcu.C as C, cpmcu.w8a8 as w8
+x = torch.ones(3, 64, dtype=torch.bfloat16, device="cuda")
+w = w8.PackedLinear.from_bf16(torch.ones(32, 64, dtype=torch.bfloat16, device="cuda"))
+want, other = w8.linear(x, w), torch.cuda.Stream()
+with torch.cuda.stream(other): w8.linear(x, w)       # torch's allocator has memory for that stream
+torch.cuda.synchronize()
+def elsewhere(check):
+    thread = threading.Thread(target=check)
+    thread.start()
+    thread.join()
+done = []
+for stream in (other.cuda_stream, 0):
+    def check():
+        with torch.cuda.stream(other): w8.linear(x, w)
+        C.stream_check(stream)
+        done.append(stream)
+    for how in (lambda: check(), lambda: elsewhere(check)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = w8.linear(x, w)
+            how()
+            z = y + 1
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(z, want + 1)
+assert len(done) == 4
+print("captured")
+"""
+
+
+def test_checks_of_other_streams_during_a_capture():
+    """From the thread that captures and from another one: the check ends, and the capture goes on."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "cpm.cu_b200")
+    out = subprocess.run([sys.executable, "-c", DURING], env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
