@@ -320,7 +320,6 @@ import threading, torch, cpmcu.C as C, cpmcu.w8a8 as w8
 x = torch.ones(3, 64, dtype=torch.bfloat16, device="cuda")
 w = w8.PackedLinear.from_bf16(torch.ones(32, 64, dtype=torch.bfloat16, device="cuda"))
 want, other = w8.linear(x, w), torch.cuda.Stream()
-with torch.cuda.stream(other): w8.linear(x, w)       # torch's allocator has memory for that stream
 torch.cuda.synchronize()
 def elsewhere(check):
     thread = threading.Thread(target=check)
@@ -329,11 +328,11 @@ def elsewhere(check):
 done = []
 for stream in (other.cuda_stream, 0):
     def check():
-        with torch.cuda.stream(other): w8.linear(x, w)
         C.stream_check(stream)
         done.append(stream)
     for how in (lambda: check(), lambda: elsewhere(check)):
         graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(other): held = w8.linear(x, w)
         with torch.cuda.graph(graph):
             y = w8.linear(x, w)
             how()
