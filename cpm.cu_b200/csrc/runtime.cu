@@ -53,6 +53,7 @@ Runtime make_runtime() {
     CUDA_CHECK(cudaMallocHost(&rt.h_error, sizeof(int)));
     CUDA_CHECK(cudaMalloc(&rt.d_accept_ticket, sizeof(unsigned)));
     CUDA_CHECK(cudaMemset(rt.d_accept_ticket, 0, sizeof(unsigned)));
+    CUDA_CHECK(cudaStreamSynchronize(nullptr));   // before a launch on a stream that does not wait for this one
     return rt;
 }
 }  // namespace
